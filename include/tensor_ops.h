@@ -354,6 +354,70 @@ typedef struct {
  * dilations).  M a multiple of 64. */
 void qconv_block_forward(const Tensor* X, const QConvBlock* block, Tensor* Y, ConvParams* params);
 
+/* ---------------------------------------------------------------------------
+ * Attention of a decoder layer, between its projection Gemms.  No counterpart in
+ * the reference.  One element type per call (float16, bfloat16 or float32);
+ * scores, softmax statistics and sums in float32 or more, one rounding at the end.
+ * The Gemm / Conv precision mode (tensor_ops_hip_set_exact) does not apply.  A key
+ * that a query does not see adds nothing, whatever K and V hold there, and a row
+ * that sees no key gives zeros.
+ *
+ * Workspace (may be NULL): device memory of any type for the partial results of
+ * calls that spread few rows over the GPU along the keys.  Without one an eager
+ * call takes such memory from the library's pool, and a call captured into a
+ * graph runs in one pass over the keys.  Calls that may overlap (two streams, two graphs) must not share one.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    int q_heads;     /* 3-D tensors: the query heads; 4-D: 0, or the same as the shape's */
+    int kv_heads;    /* 3-D tensors: the key heads; 4-D: 0, or the same as the shape's */
+    float scale;     /* factor of q.k; 0: 1 / sqrt(size of a key) */
+    int causal;      /* 1: query i sees the keys 0 .. i */
+} AttentionParams;
+/* Y = softmax(scale Q K' + Mask) V per head, the ONNX Attention operator without a past:
+ * Q [B, q_heads, Sq, D], K [B, kv_heads, Skv, D], V [B, kv_heads, Skv, Dv], Y [B, q_heads,
+ * Sq, Dv], or all 3-D [B, S, heads * size].  q_heads is a multiple of kv_heads: query head
+ * h reads key head h / (q_heads / kv_heads).  Mask (may be NULL) broadcasts to [B, q_heads,
+ * Sq, Skv]: uint8 / int8 (0 closes a key), or float32 / Q's type, added to the scores (-inf
+ * closes a key).  KVLen (may be NULL): int32 / int64 [B], the keys in use per batch.
+ * Host tensors are staged, as for every operator. */
+void attention_forward(const Tensor* Q, const Tensor* K, const Tensor* V, const Tensor* Mask, const Tensor* KVLen,
+                       Tensor* Y, const AttentionParams* params, Tensor* Workspace);
+typedef struct {
+    float scale;     /* factor of q.k; 0: 1 / sqrt(size of a key) */
+    int window;      /* > 0: a token sees the last `window` keys only, its own among them */
+    int max_kv;      /* what the caller knows of the longest KVLen (0: nothing): shapes the
+                        launch, never the result */
+} CacheAttentionParams;
+/* New tokens of several sequences over a paged cache that holds their keys and values
+ * already: Q [T, q_heads, D] with the tokens of sequence b in rows QStart[b] .. QStart[b + 1],
+ * caches [pages, kv_heads, page size, D / Dv], Pages [B, pages per sequence] (the sequence's
+ * pages in order), KVLen [B] (keys in use, the new tokens among them), Y [T, q_heads, Dv].
+ * Token i of n stands at position KVLen - n + i and sees the keys up to its own.  Pages,
+ * QStart and KVLen are int32 or int64 and read on the device: rows of Q behind the last
+ * sequence leave Y as it was, lengths are cut to what the table can name, and keys on pages
+ * that the cache does not have are not seen.  Device tensors only. */
+void cache_attention_forward(const Tensor* Q, const Tensor* KCache, const Tensor* VCache, const Tensor* Pages,
+                             const Tensor* QStart, const Tensor* KVLen, Tensor* Y, const CacheAttentionParams* params,
+                             Tensor* Workspace);
+typedef struct {
+    int q_heads;
+    int kv_heads;
+    float epsilon;      /* of the RMS norm */
+    int interleaved;    /* 1: pairs (2i, 2i + 1); 0: pairs (i, i + rotated / 2) */
+} QKNormRotaryParams;
+/* Packed projections QKV [T, (q_heads + 2 kv_heads) * D] -> Q [T, q_heads, D], K and V: per
+ * head of the queries and keys an RMS norm (QWeight / KWeight [D], NULL: none) and the
+ * rotation of its first 2 * Cos->shape[1] values by the tables' (Cos, Sin [positions,
+ * rotated / 2], NULL: none) row Positions[t]; values pass unchanged.  Without Slots K and V
+ * are [T, kv_heads, D]; with Slots [T] (page * page size + place in the page, each named once)
+ * they are the caches of cache_attention_forward and only the named slots are written.  A
+ * token whose position is negative or past the tables is left out (nothing of it is
+ * written); one whose slot is negative or past the cache has only its Q written.  Device
+ * tensors only; QKV must not overlap the outputs. */
+void qk_norm_rotary_forward(const Tensor* QKV, const Tensor* QWeight, const Tensor* KWeight, const Tensor* Cos,
+                            const Tensor* Sin, const Tensor* Positions, const Tensor* Slots, Tensor* Q, Tensor* K,
+                            Tensor* V, const QKNormRotaryParams* params);
+
 #ifdef __cplusplus
 }
 #endif

@@ -97,6 +97,22 @@ def make_op(node: P.NodeProto, dtypes: Dict[str, str], shapes: Dict[str, Tuple[i
         return Op.GlobalAveragePool(ins, outs, dtype=out_dt, version="17")
     if t == "DynamicQuantizeLinear":
         return Op.DynamicQuantizeLinear(ins, outs, version="17")
+    if t == "Attention":
+        # inputs: q, k, v, mask, past key, past value, lengths
+        for i, what in ((4, "a past key"), (5, "a past value")):
+            if len(ins) > i and ins[i]:
+                raise NotImplementedError(f"Attention (node {node.name!r}) with {what} is not supported by this build")
+        if float(node.attr("softcap", 0.0)) or len([o for o in outs if o]) > 1:
+            raise NotImplementedError(f"Attention (node {node.name!r}) with a softcap or present outputs is not "
+                                      "supported by this build")
+        if int(node.attr("is_causal", 0)) and len(ins) > 6 and ins[6]:
+            raise NotImplementedError(f"Attention (node {node.name!r}), causal with lengths, is not supported by this "
+                                      "build")
+        scale = node.attr("scale")
+        return Op.Attention((ins + [""] * 4)[:4] + ins[6:7], [o for o in outs if o],
+                            q_num_heads=int(node.attr("q_num_heads", 0)),
+                            kv_num_heads=int(node.attr("kv_num_heads", 0)), is_causal=int(node.attr("is_causal", 0)),
+                            scale=None if scale is None else float(scale), dtype=out_dt, version="23")
     raise NotImplementedError(f"ONNX operator {t!r} (node {node.name!r}) is not supported by this build")
 
 

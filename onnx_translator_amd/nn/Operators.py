@@ -25,7 +25,8 @@ from . import DTYPE_MAP, DTYPE_TO_NUMPY, DeviceArray, Ops, Tensor, Tensor_, PT
 
 __all__ = ["CConvParams", "CPoolParams", "CReduceParams", "RELU", "COS", "ABS", "ADD", "SUB", "MUL", "DIV",
            "QuantizeLinear", "DequantizeLinear", "Conv", "MaxPool", "Gemm", "Softmax", "Flatten", "Reshape",
-           "GlobalAveragePool", "DynamicQuantizeLinear", "ElementwiseChain", "CChainStep"]
+           "GlobalAveragePool", "DynamicQuantizeLinear", "ElementwiseChain", "CChainStep", "CAttentionParams",
+           "CCacheAttentionParams", "CQKNormRotaryParams", "Attention", "CacheAttention", "QKNormRotary"]
 
 
 class CConvParams(ctypes.Structure):
@@ -885,3 +886,162 @@ class ElementwiseChain(Ops):
 
     def forward_(self, x: Tensor_, *operands):
         return _values(self, Tensor_(*x.size, dtype=self.dtype))
+
+
+class CAttentionParams(ctypes.Structure):
+    """``AttentionParams`` of include/tensor_ops.h."""
+    _fields_ = [("q_heads", ctypes.c_int), ("kv_heads", ctypes.c_int), ("scale", ctypes.c_float),
+                ("causal", ctypes.c_int)]
+
+
+class CCacheAttentionParams(ctypes.Structure):
+    """``CacheAttentionParams`` of include/tensor_ops.h."""
+    _fields_ = [("scale", ctypes.c_float), ("window", ctypes.c_int), ("max_kv", ctypes.c_int)]
+
+
+class CQKNormRotaryParams(ctypes.Structure):
+    """``QKNormRotaryParams`` of include/tensor_ops.h."""
+    _fields_ = [("q_heads", ctypes.c_int), ("kv_heads", ctypes.c_int), ("epsilon", ctypes.c_float),
+                ("interleaved", ctypes.c_int)]
+
+
+class Attention(Ops):
+    """softmax(scale Q K' + mask) V per head (``attention_forward``): the ONNX Attention
+    operator without a past, for keys and values of any length (an encoder's states, say).
+
+    ``forward(q, k, v, attn_mask, kv_lengths)``: q [B, q_heads, Sq, D], k [B, kv_heads, Skv,
+    D], v [B, kv_heads, Skv, Dv], or all of them [B, S, heads * size] with ``q_num_heads`` and
+    ``kv_num_heads`` given.  ``attn_mask`` broadcasts to [B, q_heads, Sq, Skv]: bool / uint8
+    (0 closes a key), float32 or q's type (added to the scores); ``kv_lengths`` [B] int32 /
+    int64 are the keys in use.  ``scale=None`` is 1 / sqrt(D).  A query that sees no key gives
+    zeros."""
+
+    def __init__(self, inputs, outputs, q_num_heads=0, kv_num_heads=0, is_causal=0, scale=None, dtype=None,
+                 version="23"):
+        super().__init__(inputs, outputs)
+        self.q_num_heads, self.kv_num_heads = int(q_num_heads or 0), int(kv_num_heads or 0)
+        self.is_causal = 1 if is_causal else 0
+        self.scale = scale
+        self.dtype = dtype
+        self.version = version
+
+    def _shape(self, q, v):
+        if len(q.size) == 4:
+            return tuple(q.size[:3]) + (v.size[3],)
+        if len(q.size) != 3 or self.q_num_heads < 1 or self.kv_num_heads < 1:
+            raise ValueError("Attention takes 4-D tensors, or 3-D ones with q_num_heads and kv_num_heads")
+        return tuple(q.size[:2]) + (v.size[2] // self.kv_num_heads * self.q_num_heads,)
+
+    def forward(self, q: Tensor, k: Tensor, v: Tensor, attn_mask: Tensor = None, kv_lengths: Tensor = None,
+                workspace: Tensor = None):
+        p = CAttentionParams(self.q_num_heads, self.kv_num_heads, _scale(self.scale), self.is_causal)
+
+        def arrange(ins, out):
+            return (*ins[:5], out, ctypes.byref(p), ins[5])
+        t = self._run("attention_forward", [q, k, v, attn_mask, kv_lengths, workspace], self._shape(q, v),
+                      self.dtype or q.dtype, arrange=arrange)
+        return _values(self, t)
+
+    def forward_(self, q: Tensor_, k: Tensor_, v: Tensor_, *rest):
+        return _values(self, Tensor_(*self._shape(q, v), dtype=self.dtype or q.dtype))
+
+
+def _scale(scale):
+    """The factor of q.k as the library takes it (0: its default)."""
+    if scale is None:
+        return 0.0
+    if not float(scale) > 0:
+        raise ValueError(f"scale must be positive, got {scale}")
+    return float(scale)
+
+
+def _on_device(op, **tensors):
+    for name, t in tensors.items():
+        if t is not None and not isinstance(t.data, DeviceArray):
+            raise ValueError(f"{op}: {name} must be on the device (Tensor.to_device())")
+
+
+class CacheAttention(Ops):
+    """New tokens of several sequences over the pages of their key / value cache
+    (``cache_attention_forward``).
+
+    ``forward(q, key_cache, value_cache, pages, q_start, kv_len)``: q [T, q_heads, D], the
+    tokens of sequence b in rows q_start[b] .. q_start[b + 1]; caches [pages, kv_heads, page
+    size, D] as :class:`QKNormRotary` fills them; pages [B, n] (each sequence's pages in order);
+    kv_len [B], the keys in use with the new tokens among them.  A token sees the keys up to its
+    own, the last ``window`` of them if given.  ``max_kv`` tells the launch the longest kv_len
+    that the caller expects.  Rows of q behind the last sequence are not written.  Device
+    tensors only."""
+
+    def __init__(self, inputs, outputs, scale=None, window=0, max_kv=0, dtype=None, version="1"):
+        super().__init__(inputs, outputs)
+        self.scale, self.window, self.max_kv = scale, int(window), int(max_kv)
+        self.dtype = dtype
+        self.version = version
+
+    def forward(self, q: Tensor, key_cache: Tensor, value_cache: Tensor, pages: Tensor, q_start: Tensor,
+                kv_len: Tensor, workspace: Tensor = None):
+        _on_device("CacheAttention", q=q, key_cache=key_cache, value_cache=value_cache, pages=pages, q_start=q_start,
+                   kv_len=kv_len, workspace=workspace)
+        p = CCacheAttentionParams(_scale(self.scale), self.window, self.max_kv)
+
+        def arrange(ins, out):
+            return (*ins[:6], out, ctypes.byref(p), ins[6])
+        t = self._run("cache_attention_forward", [q, key_cache, value_cache, pages, q_start, kv_len, workspace],
+                      tuple(q.size[:2]) + (value_cache.size[3],), self.dtype or q.dtype, arrange=arrange)
+        return _values(self, t)
+
+    def forward_(self, q: Tensor_, key_cache: Tensor_, value_cache: Tensor_, *rest):
+        return _values(self, Tensor_(*(tuple(q.size[:2]) + (value_cache.size[3],)), dtype=self.dtype or q.dtype))
+
+
+class QKNormRotary(Ops):
+    """Packed projections to what the attention reads (``qk_norm_rotary_forward``): per-head RMS
+    norm of queries and keys, rotation by position, and the keys and values into a cache.
+
+    ``forward(qkv, q_weight, k_weight, cos, sin, positions)`` with qkv [T, (q_heads + 2
+    kv_heads) * D] gives [q, k, v] ([T, heads, D] each).  With ``key_cache``, ``value_cache``
+    ([pages, kv_heads, page size, D]) and ``slots`` [T] (page * page size + place in the page)
+    keys and values are written there instead and the outputs are [q, key_cache, value_cache].
+    Weights [D] may be None (no norm), and so may cos and sin [positions, rotated / 2] (no
+    rotation).  A token with a negative position is left out.  Device tensors only."""
+
+    def __init__(self, inputs, outputs, q_num_heads, kv_num_heads, epsilon=1e-6, interleaved=0, dtype=None,
+                 version="1"):
+        super().__init__(inputs, outputs)
+        self.q_num_heads, self.kv_num_heads = int(q_num_heads), int(kv_num_heads)
+        self.epsilon = float(epsilon)
+        self.interleaved = 1 if interleaved else 0
+        self.dtype = dtype
+        self.version = version
+
+    def _shapes(self, qkv):
+        heads = self.q_num_heads + 2 * self.kv_num_heads
+        if len(qkv.size) != 2 or self.q_num_heads < 1 or self.kv_num_heads < 1 or qkv.size[1] % heads:
+            raise ValueError("QKNormRotary takes [tokens, (q_heads + 2 kv_heads) * size]")
+        t, d = qkv.size[0], qkv.size[1] // heads
+        return [(t, h, d) for h in (self.q_num_heads, self.kv_num_heads, self.kv_num_heads)]
+
+    def forward(self, qkv: Tensor, q_weight: Tensor = None, k_weight: Tensor = None, cos: Tensor = None,
+                sin: Tensor = None, positions: Tensor = None, key_cache: Tensor = None, value_cache: Tensor = None,
+                slots: Tensor = None):
+        _on_device("QKNormRotary", qkv=qkv, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin,
+                   positions=positions, key_cache=key_cache, value_cache=value_cache, slots=slots)
+        if (key_cache is None) != (slots is None) or (value_cache is None) != (slots is None):
+            raise ValueError("QKNormRotary: a cache takes key_cache, value_cache and slots together")
+        dt, shapes = self.dtype or qkv.dtype, self._shapes(qkv)
+        made = [Tensor(*s, dtype=dt, data=DeviceArray(self.lib, s, dt, zero=False))
+                for s in (shapes[:1] if slots is not None else shapes)]
+        outs = made + ([key_cache, value_cache] if slots is not None else [])
+        p = CQKNormRotaryParams(self.q_num_heads, self.kv_num_heads, self.epsilon, self.interleaved)
+        ins = [t.data.ptr if t is not None else PT()
+               for t in (qkv, q_weight, k_weight, cos, sin, positions, slots)]
+        self._call("qk_norm_rotary_forward", *ins, *[t.data.ptr for t in outs], ctypes.byref(p))
+        return _values(self, outs)
+
+    def forward_(self, qkv: Tensor_, q_weight=None, k_weight=None, cos=None, sin=None, positions=None, key_cache=None,
+                 value_cache=None, slots=None):
+        dt, shapes = self.dtype or qkv.dtype, self._shapes(qkv)
+        if slots is not None:
+            shapes[1:] = [tuple(key_cache.size), tuple(value_cache.size)]
+        return _values(self, [Tensor_(*s, dtype=dt) for s in shapes])

@@ -228,6 +228,10 @@ class Ops:
                     _sig(lib, "tensor_ops_hip_version", ctypes.c_char_p, [])
                     _sig(lib, "tensor_ops_hip_set_exact", None, [ctypes.c_int])
                     _sig(lib, "init_cos_lut", None, [])
+                    V = ctypes.c_void_p
+                    _sig(lib, "attention_forward", None, [P] * 6 + [V, P])
+                    _sig(lib, "cache_attention_forward", None, [P] * 7 + [V, P])
+                    _sig(lib, "qk_norm_rotary_forward", None, [P] * 10 + [V])
                     lib.init_cos_lut()
                     cls._lib = lib
                     cls._lib_initialized = True
