@@ -24,7 +24,7 @@ CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libtensor_ops_hip.so")
 SOURCES = ["runtime.hip", "elementwise.hip", "qdq.hip", "reduce.hip", "gemm.hip", "conv.hip", "convdw.hip", "convh.hip", "qconv.hip",
-           "attention.hip", "rotary.hip"]
+           "attention.hip", "attention_f16.hip", "attention_bf16.hip", "attention_f32.hip", "rotary.hip"]
 
 HIPCC = os.environ.get("HIPCC", shutil.which("hipcc") or "/opt/rocm/bin/hipcc")
 FLAGS = [

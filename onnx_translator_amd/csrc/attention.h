@@ -39,6 +39,11 @@ struct AttnArgs {
     FastDiv fd_g, fd_ps;
     float scale;
     int causal, window;
+    // tiles: rows of tiles per batch (dense) or in all (paged), and the key splits of each
+    int tiles, nsplit;
+    float* part_o;                 // [nsplit][rows][Dv]: normalised results of a split
+    float2* part_ml;               // [nsplit][rows]: (maximum in log2 units, sum)
+    int64_t rows;                  // rows of Y: tokens x query heads
 };
 
 // A sequence's part of a call: n new tokens, len keys, token i at position first + i.
@@ -114,6 +119,23 @@ class DeviceScope {
     int was_ = 0;
     bool moved_ = false;
 };
+
+// A tile kernel's shape by the bytes of a padded row of K: rw waves of 32 rows each share the
+// keys, or (few) kw waves share the rows; bn keys per tile, two tiles of K and of V in LDS.
+struct AttnTile { int rw, kw, bn; };
+constexpr AttnTile attn_tile(int row_bytes, bool few) {
+    if (!few) return {4, 1, row_bytes <= 256 ? 64 : 32};
+    return row_bytes <= 256 ? AttnTile{1, 4, 128} : row_bytes <= 512 ? AttnTile{1, 2, 64} : AttnTile{1, 1, 32};
+}
+
+struct AttnPlan {
+    bool paged, few;
+    int d;                         // padded head size of the tile kernels; 0: a wave per row
+    unsigned blocks;
+};
+void launch_attention_f16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);
+void launch_attention_bf16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);
+void launch_attention_f32(const AttnArgs& a, const AttnPlan& p, hipStream_t s);
 
 constexpr float kLog2e = 1.4426950408889634f;
 

@@ -1,138 +1,14 @@
 // attention.hip — attention_forward (dense keys and values, masks, lengths) and
-// cache_attention_forward (new tokens over a paged cache) for gfx950.
-//
-//   y = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q.k_j + bias_j - max_j)
-//
-// over the keys a query sees.  One pass over the keys: a running maximum and sum,
-// the output rescaled where the maximum grows.  Scores, statistics and sums are
-// held in 32 bits or more; the result is rounded once.
-//
-// Keys that are not seen (past the length, later than the query, outside the
-// window, closed by the mask, or on a page that the cache does not have) add
-// nothing, whatever K and V hold there; a row that sees none gives zeros.
+// cache_attention_forward (new tokens over a paged cache): argument checks and launches.
+// The kernels are in attention_kernels.h.
 #include "attention.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace tohip {
 namespace {
 
-template <int DT> __device__ __forceinline__ float ld_f(const void* p, int64_t i) { return (float)ld_d<DT>(p, i); }
-
-__device__ __forceinline__ double lane_value(double v, int lane) {
-    const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
-    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)u, lane);
-    const unsigned hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(u >> 32), lane);
-    return __builtin_bit_cast(double, ((unsigned long long)hi << 32) | lo);
-}
-
-// ---- one row per wave ---------------------------------------------------------------
-// Any head size, alignment and content.  Lanes take 64 keys at a time for the scores,
-// then 64 columns of V for the sums, in double: nothing overflows on the way to a
-// finite result, and a key that is not seen is never multiplied.
-constexpr int kRowCols = 4;        // columns of V per lane and pass over the keys
-
-// Partial result of the keys [ks, ke) for query head h of token i: the maximum (of
-// scaled scores), the sum and, by store(d, value), the normalised output.
-template <int DT, bool PAGED, class ST>
-__device__ __forceinline__ void attn_row(const AttnArgs& a, const AttnSeq& s, int h, int i, int ks, int ke, float& m_out,
-                                         float& l_out, ST store) {
-    const int lane = (int)(threadIdx.x & 63), hk = (int)a.fd_g.div((uint32_t)h);
-    const int lo = max(ks, attn_lo(a, s, i)), hi = min(ke, attn_hi(a, s, i));
-    const int64_t qo = PAGED ? (s.tok0 + i) * a.qt + h * a.qh : s.b * a.qb + i * a.qt + h * a.qh;
-    const int64_t mo = s.b * a.mb + h * a.mh + i * a.mq;
-    for (int d0 = 0; d0 < a.Dv; d0 += 64 * kRowCols) {
-        float m = -INFINITY;
-        double l = 0.0, acc[kRowCols] = {};
-        for (int j0 = lo; j0 < hi; j0 += 64) {
-            const int j = j0 + lane;
-            bool seen = j < hi;
-            const int page = PAGED && seen ? attn_page(a, s.b, j) : 0;
-            seen = seen && page >= 0;
-            float t = -INFINITY;
-            KeyRow row = {0, 0};
-            if (seen) {
-                row = attn_key_row<PAGED>(a, s.b, page, j);
-                float bias = 0.0f;
-                if (a.mask) {
-                    const int64_t o = mo + (int64_t)j * a.mk;
-                    if (a.mask_dt == kU8 || a.mask_dt == kI8) {
-                        seen = ((const uint8_t*)a.mask)[o] != 0;
-                    } else {
-                        bias = a.mask_dt == kF32 ? ((const float*)a.mask)[o] : ld_f<DT>(a.mask, o);
-                        seen = !(bias == -INFINITY);
-                    }
-                }
-                if (seen) {
-                    double dot = 0.0;
-                    for (int d = 0; d < a.Dk; d++)
-                        dot += (double)ld_f<DT>(a.q, qo + d) * (double)ld_f<DT>(a.k, row.k + hk * a.kh + d);
-                    t = (float)(dot * (double)a.scale + (double)bias);
-                }
-            }
-            const unsigned long long sees = __ballot(seen);
-            if (!sees) continue;
-            const bool bad = __ballot(seen && t != t) != 0;
-            const float top = wave_allreduce(t != t ? -INFINITY : t, [](float x, float y) { return x > y ? x : y; });
-            const float mn = bad ? NAN : (top > m ? top : m);
-            if (mn == -INFINITY) continue;
-            const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * kLog2e);
-            const double p = seen ? (double)__builtin_amdgcn_exp2f((t - mn) * kLog2e) : 0.0;
-            l = l * (double)alpha + wave_allreduce(p, [](double x, double y) { return x + y; });
-#pragma unroll
-            for (int c = 0; c < kRowCols; c++) acc[c] *= (double)alpha;
-            m = mn;
-            for (int jj = 0; jj < 64; jj++) {
-                if (!((sees >> jj) & 1)) continue;
-                const double pj = lane_value(p, jj);
-                const int64_t ro = (int64_t)__builtin_bit_cast(long long, lane_value(__builtin_bit_cast(double, (long long)row.v), jj));
-#pragma unroll
-                for (int c = 0; c < kRowCols; c++) {
-                    const int d = d0 + c * 64 + lane;
-                    if (d < a.Dv) acc[c] += pj * (double)ld_f<DT>(a.v, ro + hk * a.vh + d);
-                }
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < kRowCols; c++) {
-            const int d = d0 + c * 64 + lane;
-            if (d < a.Dv) store(d, l == 0.0 ? 0.0f : (float)(acc[c] / l));
-        }
-        m_out = m;
-        l_out = (float)l;
-    }
-}
-
-template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a, int64_t rows) {
-    const int64_t step = (int64_t)gridDim.x * 4;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); r < rows; r += step) {
-        const int64_t t = r / a.Hq;
-        const int h = (int)(r - t * a.Hq);
-        int b, i;
-        if constexpr (PAGED) {
-            // the last sequence that starts at or before the token
-            int lo = 0, hi = a.B;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (a.qstart[mid] <= t) lo = mid + 1;
-                else hi = mid;
-            }
-            b = lo - 1;
-            if (b < 0) continue;
-        } else {
-            b = (int)(t / a.Sq);
-        }
-        const AttnSeq s = attn_seq<PAGED>(a, b);
-        const int64_t at = PAGED ? t - s.tok0 : t - (int64_t)b * a.Sq;
-        if (at < 0 || at >= s.n) continue;             // behind the last sequence: left as it is
-        i = (int)at;
-        const int64_t yo = PAGED ? t * a.yt + h * a.yh : b * a.yb + i * a.yt + h * a.yh;
-        float m, l;
-        attn_row<DT, PAGED>(a, s, h, i, 0, s.len, m, l, [&](int d, float v) { st_code<DT>(a.y, yo + d, v); });
-    }
-}
-
-// ---- host ---------------------------------------------------------------------------
 bool float_type(const Tensor* t) {
     return (int)t->dtype == kF16 || (int)t->dtype == kBF16 || (int)t->dtype == kF32;
 }
@@ -144,13 +20,53 @@ bool good_scale(float s, const char* name) {
     return false;
 }
 
-template <bool PAGED> void launch_rows(const AttnArgs& a, int dt, const char* name) {
-    const int64_t rows = (PAGED ? (int64_t)a.T : (int64_t)a.B * a.Sq) * a.Hq;
-    const unsigned grid = grid_for((size_t)rows, 4, 1u << 20);
-    if (dt == kF16) hipLaunchKernelGGL((k_attn_rows<kF16, PAGED>), dim3(grid), dim3(256), 0, stream(), a, rows);
-    else if (dt == kBF16) hipLaunchKernelGGL((k_attn_rows<kBF16, PAGED>), dim3(grid), dim3(256), 0, stream(), a, rows);
-    else hipLaunchKernelGGL((k_attn_rows<kF32, PAGED>), dim3(grid), dim3(256), 0, stream(), a, rows);
+bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Cuts the call into blocks and launches it.  kv: the most keys that a row may see, as far
+// as the host knows.
+void run_attention(AttnArgs& a, int dt, bool paged, int64_t kv, const Tensor* ws, const char* name) {
+    const int es = dt == kF32 ? 4 : 2, vec = 16 / es, dm = a.Dk > a.Dv ? a.Dk : a.Dv;
+    const int64_t tokens = paged ? (int64_t)a.T : (int64_t)a.B * a.Sq;
+    a.rows = tokens * a.Hq;
+    a.nsplit = 1;
+    AttnPlan p = {paged, false, 0, 0};
+    void* part = nullptr;
+    if (dm <= 256 && a.Dk % vec == 0 && a.Dv % vec == 0 && aligned(a.q) && aligned(a.k) && aligned(a.v) && aligned(a.y)) {
+        p.d = dm <= 64 ? 64 : dm <= 128 ? 128 : 256;
+        const int64_t per = paged ? (int64_t)a.T * a.G / a.B : (int64_t)a.Sq * a.G;      // rows per sequence
+        p.few = per <= 32;
+        const AttnTile t = attn_tile(p.d * es, p.few);
+        const int bm = 32 * t.rw;
+        const int64_t tiles = paged ? (int64_t)a.T * a.G / bm + a.B : ((int64_t)a.Sq * a.G + bm - 1) / bm;
+        const int64_t units = tiles * (paged ? 1 : a.B) * a.Hkv;
+        const int lds = 4 * t.bn * p.d * es, resident = num_cus() * (160 * 1024 / lds > 2 ? 2 : 160 * 1024 / lds);
+        int64_t split = units < resident ? resident / units : 1;
+        split = std::min<int64_t>({split, (kv + t.bn - 1) / t.bn, 128});
+        const int64_t each = a.rows * (a.Dv * 4 + 8);
+        if (split > 1 && ws) {
+            split = std::min<int64_t>(split, (int64_t)tensor_bytes(ws) / each);
+            part = ws->data;
+            if (!aligned(part)) split = 1;
+        } else if (split > 1) {
+            part = pool_alloc((size_t)(split * each), true);
+            if (!part) split = 1;
+        }
+        if (split > 1) {
+            a.nsplit = (int)split;
+            a.part_o = (float*)part;
+            a.part_ml = (float2*)(a.part_o + split * a.rows * a.Dv);
+        }
+        const int64_t blocks = units * a.nsplit;
+        if (tiles > 0x7FFFFFFF || blocks >= (int64_t(1) << 24)) {
+            p.d = 0;                                   // past the runtime's work-items per launch
+            a.nsplit = 1;
+        }
+        a.tiles = (int)tiles;
+        p.blocks = (unsigned)blocks;
+    }
+    (dt == kF16 ? launch_attention_f16 : dt == kBF16 ? launch_attention_bf16 : launch_attention_f32)(a, p, stream());
     check_launch(name);
+    if (part && !ws) pool_free(part);
 }
 
 }  // namespace
@@ -275,7 +191,7 @@ void attention_forward(const Tensor* Q, const Tensor* K, const Tensor* V, const 
     a.len.is64 = KVLen && (int)KVLen->dtype == kI64;
     a.y = st.out(Y, tensor_bytes(Y));
     if (*tensor_ops_hip_last_error()) return;
-    launch_rows<false>(a, (int)Q->dtype, name);
+    run_attention(a, (int)Q->dtype, false, a.Skv, Workspace, name);
     st.finish();
 }
 
@@ -362,7 +278,8 @@ void cache_attention_forward(const Tensor* Q, const Tensor* KCache, const Tensor
     a.qstart = {QStart->data, (int)QStart->dtype == kI64};
     a.len = {KVLen->data, (int)KVLen->dtype == kI64};
     DeviceScope scope;
-    launch_rows<true>(a, (int)Q->dtype, name);
+    const int64_t cap = (int64_t)a.max_pages * a.ps;
+    run_attention(a, (int)Q->dtype, true, params->max_kv ? std::min<int64_t>(params->max_kv, cap) : cap, Workspace, name);
 }
 
 }  // extern "C"
