@@ -40,7 +40,7 @@ struct AttnArgs {
     float scale;
     int causal, window;
     // tiles: rows of tiles per batch (dense) or in all (paged), and the key splits of each
-    int tiles, nsplit;
+    int tiles, nsplit, share;      // share: keys of a split
     float* part_o;                 // [nsplit][rows][Dv]: normalised results of a split
     float2* part_ml;               // [nsplit][rows]: (maximum in log2 units, sum)
     int64_t rows;                  // rows of Y: tokens x query heads
@@ -120,17 +120,16 @@ class DeviceScope {
     bool moved_ = false;
 };
 
-// A tile kernel's shape by the bytes of a padded row of K: rw waves of 32 rows each share the
-// keys, or (few) kw waves share the rows; bn keys per tile, two tiles of K and of V in LDS.
-struct AttnTile { int rw, kw, bn; };
-constexpr AttnTile attn_tile(int row_bytes, bool few) {
-    if (!few) return {4, 1, row_bytes <= 256 ? 64 : 32};
-    return row_bytes <= 256 ? AttnTile{1, 4, 128} : row_bytes <= 512 ? AttnTile{1, 2, 64} : AttnTile{1, 1, 32};
-}
+// Keys per tile of the prompts' kernel by the bytes of a padded row of K: two tiles of K and
+// of V in LDS (64 KB up to 512 bytes: two blocks per CU).
+constexpr int attn_tile_keys(int row_bytes) { return row_bytes <= 256 ? 64 : 32; }
+
+constexpr int kMaxSplits = 128;    // of the keys, joined by one wave per row
 
 struct AttnPlan {
-    bool paged, few;
+    bool paged;
     int d;                         // padded head size of the tile kernels; 0: a wave per row
+    int rows;                      // rows of a block: 16 or 32 (one wave), or 128 (four)
     unsigned blocks;
 };
 void launch_attention_f16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);

@@ -29,22 +29,32 @@ void run_attention(AttnArgs& a, int dt, bool paged, int64_t kv, const Tensor* ws
     const int64_t tokens = paged ? (int64_t)a.T : (int64_t)a.B * a.Sq;
     a.rows = tokens * a.Hq;
     a.nsplit = 1;
-    AttnPlan p = {paged, false, 0, 0};
+    AttnPlan p = {paged, 0, 0, 0};
     void* part = nullptr;
-    if (dm <= 256 && a.Dk % vec == 0 && a.Dv % vec == 0 && aligned(a.q) && aligned(a.k) && aligned(a.v) && aligned(a.y)) {
+    const int64_t per = paged ? (int64_t)a.T : (int64_t)a.Sq;      // tokens of a sequence at most
+    if (dm <= 256 && a.Dk % vec == 0 && a.Dv % vec == 0 && per * a.G < 0x7FFFFF00 && aligned(a.q) && aligned(a.k) &&
+        aligned(a.v) && aligned(a.y)) {
         p.d = dm <= 64 ? 64 : dm <= 128 ? 128 : 256;
-        const int64_t per = paged ? (int64_t)a.T * a.G / a.B : (int64_t)a.Sq * a.G;      // rows per sequence
-        p.few = per <= 32;
-        const AttnTile t = attn_tile(p.d * es, p.few);
-        const int bm = 32 * t.rw;
-        const int64_t tiles = paged ? (int64_t)a.T * a.G / bm + a.B : ((int64_t)a.Sq * a.G + bm - 1) / bm;
+        const int64_t mean = paged ? ((int64_t)a.T * a.G + a.B - 1) / a.B : per * a.G;      // rows of a sequence
+        p.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 128;
+        const int64_t tiles = paged ? (int64_t)a.T * a.G / p.rows + a.B : (per * a.G + p.rows - 1) / p.rows;
         const int64_t units = tiles * (paged ? 1 : a.B) * a.Hkv;
-        const int lds = 4 * t.bn * p.d * es, resident = num_cus() * (160 * 1024 / lds > 2 ? 2 : 160 * 1024 / lds);
-        int64_t split = units < resident ? resident / units : 1;
-        split = std::min<int64_t>({split, (kv + t.bn - 1) / t.bn, 128});
+        const int bn = p.rows == 128 ? attn_tile_keys(p.d * es) : 32;
+        const int lds = 4 * bn * p.d * es, resident = num_cus() * std::min(160 * 1024 / lds, p.rows == 128 ? 2 : 8);
+        // Keys per split.  Few rows: four blocks for every place on the GPU, as lengths differ, and
+        // two tiles at least (64 tokens over 130 .. 8192 keys: 219 us with four, 231 with
+        // sixteen, 356 with two; one token over 1025: 12.4 us with two tiles, 13.2 with one, 14.0
+        // with four, 18.2 with eight).  Prompts are split only where their blocks do not fill the
+        // GPU (12 sequences of 1 .. 512 tokens, 376 blocks: 59 us with four per place, 78 with
+        // one; 1024 blocks of 8192 keys: 553 unsplit, 620 in two).
+        int64_t share = std::max<int64_t>({units * kv / ((int64_t)resident * 4), 64, (kv + kMaxSplits - 1) / kMaxSplits});
+        if (p.rows == 128 && units >= resident) share = kv;
+        share = (share + 31) / 32 * 32;
+        int64_t split = kv > share ? (kv + share - 1) / share : 1;
         const int64_t each = a.rows * (a.Dv * 4 + 8);
         if (split > 1 && ws) {
             split = std::min<int64_t>(split, (int64_t)tensor_bytes(ws) / each);
+            share = split ? ((kv + split - 1) / split + 31) / 32 * 32 : kv;
             part = ws->data;
             if (!aligned(part)) split = 1;
         } else if (split > 1) {
@@ -53,6 +63,7 @@ void run_attention(AttnArgs& a, int dt, bool paged, int64_t kv, const Tensor* ws
         }
         if (split > 1) {
             a.nsplit = (int)split;
+            a.share = (int)share;
             a.part_o = (float*)part;
             a.part_ml = (float2*)(a.part_o + split * a.rows * a.Dv);
         }

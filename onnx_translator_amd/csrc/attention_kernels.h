@@ -13,6 +13,7 @@
 #pragma once
 
 #include <cmath>
+#include <type_traits>
 
 #include "attention.h"
 
@@ -135,61 +136,63 @@ template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_rows
 }
 
 // ---- tiles on the matrix cores ------------------------------------------------------
-// A wave owns 32 rows (query heads of tokens) and walks over the keys 32 at a time:
-//   S' = K Q'    32 keys x 32 rows: a lane holds 16 keys of one row, its other 16 are in
-//                the lane 32 further on, so maximum and sum of a row are a few register
-//                operations and one exchange between the halves of the wave;
-//   O' += V' P'  head size x 32 rows: the rescaling factor of a row is one lane's value,
+// A wave owns MR rows (query heads of tokens) and walks over the keys, 32 at a time:
+//   S' = K Q'    32 keys x MR rows: a lane holds a part of one row's keys (MR = 32: half of
+//                them, MR = 16: a quarter), so maximum and sum of a row are a few register
+//                operations and one or two exchanges inside the wave;
+//   O' += V' P'  head size x MR rows: the rescaling factor of a row is one lane's value,
 //                and P goes from the accumulators of S' straight into the operand: the
 //                product sums over keys in any order, so V's rows are simply read in the
 //                order in which the lanes hold their keys.
-// RW waves share the keys and own different rows (prompts), or KW waves own the same rows
-// and different keys (few rows, where reading the keys is the work) and join at the end.
-// Key and value tiles go from memory to LDS directly (no registers), two buffers deep, in
-// 16-byte chunks whose place in a row is turned by the row's number so that fragment
-// reads spread over the banks.
+// Tiles of K and V go from memory to LDS directly (no registers) in 16-byte chunks whose
+// place in a row is turned by the row's number, so that fragment reads spread over the
+// banks; V's columns are read by the transposing LDS loads (16-bit types).
+//   k_attn_tiles   prompts: four waves of 32 rows share the tiles, two deep;
+//   k_attn_few     few rows, where reading the keys is the work: a block is one wave.
 //
 // What a closed key holds does not matter as long as it is finite: its weight is zero.
 // Where a result comes out infinite or NaN (a closed key's value was, or values near the
 // type's largest overflowed a sum on the way), or a page of the sequence is missing, the
 // row is computed again by attn_row above, which looks at open keys only.
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bfloatx8 __attribute__((ext_vector_type(8)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
-typedef short shortx8 __attribute__((ext_vector_type(8)));
-typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+#define TOHIP_INLINE __attribute__((always_inline))
 
 template <int DT> constexpr int kElem = DT == kF32 ? 4 : 2;
 
-// One 16-byte chunk per lane of each operand: 8 values of 16 bits (one product), or 4 of
-// 32 bits (four products, the chunk's j-th values of both wave halves in the j-th).
-template <int DT> __device__ __forceinline__ floatx16 mfma_chunk(uint4 a, uint4 b, floatx16 c) {
+// One product step.  16 bits: operands of eight values per lane (a 16-byte chunk); 32 bits:
+// one value per lane.  MR = 32: 32x32 results, two lanes' values per column and step;
+// MR = 16: 16x16, four lanes'.
+template <int MR> struct AttnAcc { typedef floatx16 type; };
+template <> struct AttnAcc<16> { typedef floatx4 type; };
+template <int DT, int MR, class ACC> __device__ __forceinline__ ACC mfma16(uint4 a, uint4 b, ACC c) {
     if constexpr (DT == kF16) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
-    } else if constexpr (DT == kBF16) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bfloatx8, a), __builtin_bit_cast(bfloatx8, b), c, 0, 0, 0);
+        const halfx8 x = __builtin_bit_cast(halfx8, a), y = __builtin_bit_cast(halfx8, b);
+        if constexpr (MR == 32) return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
     } else {
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(u2f(a.x), u2f(b.x), c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(u2f(a.y), u2f(b.y), c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(u2f(a.z), u2f(b.z), c, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_32x32x2f32(u2f(a.w), u2f(b.w), c, 0, 0, 0);
+        const bfloatx8 x = __builtin_bit_cast(bfloatx8, a), y = __builtin_bit_cast(bfloatx8, b);
+        if constexpr (MR == 32) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
     }
 }
+template <int MR, class ACC> __device__ __forceinline__ ACC mfma32(float a, float b, ACC c) {
+    if constexpr (MR == 32) return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
 
-// Eight weights as the product's operand, each rounded to the nearest 16-bit value.
-template <int DT> __device__ __forceinline__ uint4 pack8(const float* p) {
-    if constexpr (DT == kF16) {
-        halfx8 h;
+// Values rounded to the nearest of the 16-bit type.
+template <int DT, int N> __device__ __forceinline__ auto round16(const float* p) {
+    typedef std::conditional_t<DT == kF16, _Float16, __bf16> T;
+    typedef T vec __attribute__((ext_vector_type(N)));
+    vec h;
 #pragma unroll
-        for (int i = 0; i < 8; i++) h[i] = (_Float16)p[i];
-        return __builtin_bit_cast(uint4, h);
-    } else {
-        bfloatx8 h;
-#pragma unroll
-        for (int i = 0; i < 8; i++) h[i] = (__bf16)p[i];
-        return __builtin_bit_cast(uint4, h);
-    }
+    for (int i = 0; i < N; i++) h[i] = (T)p[i];
+    return h;
 }
 
 // 16 bytes per lane from its own address into LDS, lane l to the l-th 16 bytes of `to`.
@@ -202,22 +205,71 @@ __device__ __forceinline__ void load_lds16(const void* from, char* to) {
 __device__ __forceinline__ uint2 read_turned(const char* p) {
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4*)p));
 }
-// All of this wave's loads have landed and its LDS reads have returned.
-__device__ __forceinline__ void wait_all_loads() { __builtin_amdgcn_s_waitcnt(0x0070); }
+// Several LDS reads and the wait for them in one go.  The loads that write LDS are waited for by
+// count (wait_loads); where the compiler sees the reads it adds a wait of its own, inside a loop
+// for everything in flight, the next tiles' loads among them.
+__device__ __forceinline__ uint32_t lds_address(const char* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+__device__ __forceinline__ void read_keys4(const uint32_t (&at)[4], uint4 (&v)[4]) {
+    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %6\n\tds_read_b128 %3, %7\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+                 : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]) : "memory");
+}
+__device__ __forceinline__ void read_keys8(const uint32_t (&at)[8], uint4 (&v)[8]) {
+    asm volatile("ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
+                 "ds_read_b128 %4, %12\n\tds_read_b128 %5, %13\n\tds_read_b128 %6, %14\n\tds_read_b128 %7, %15\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+                 : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]), "v"(at[6]), "v"(at[7]) : "memory");
+}
+// read_turned at four addresses, and STEP bytes further on.
+template <int STEP> __device__ __forceinline__ void read_values4(const uint32_t (&at)[4], uint2 (&x)[4], uint2 (&y)[4]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %4, %8 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %5, %9 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %2, %10\n\tds_read_b64_tr_b16 %6, %10 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %3, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
+                 : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(STEP) : "memory");
+}
+// Eight 32-bit values of one column: rows 0 .. 3 and G .. G + 3 of RB bytes each.
+template <int RB, int G> __device__ __forceinline__ void read_column8(uint32_t at, float (&v)[8]) {
+    asm volatile("ds_read_b32 %0, %8\n\tds_read_b32 %1, %8 offset:%9\n\tds_read_b32 %2, %8 offset:%10\n\t"
+                 "ds_read_b32 %3, %8 offset:%11\n\tds_read_b32 %4, %8 offset:%12\n\tds_read_b32 %5, %8 offset:%13\n\t"
+                 "ds_read_b32 %6, %8 offset:%14\n\tds_read_b32 %7, %8 offset:%15\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+                 : "v"(at), "n"(RB), "n"(2 * RB), "n"(3 * RB), "n"(G * RB), "n"((G + 1) * RB), "n"((G + 2) * RB), "n"((G + 3) * RB)
+                 : "memory");
+}
+// At most N of this wave's loads are in flight (they land in order), and its LDS reads have
+// returned.
+template <int N> __device__ __forceinline__ void wait_loads() {
+    constexpr int n = N > 63 ? 63 : N;
+    __builtin_amdgcn_s_waitcnt(0x0070 | (n & 15) | ((n >> 4) << 14));
+}
 // A value that all lanes hold, as a scalar.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // Place of chunk c in row r of a tile of CH chunks per row.  Keys are read by 16 or 32 rows
-// of one chunk; values by four rows of four neighbouring chunks (16 bits), or by rows r and
-// r + 4 of eight (32 bits).
+// of one chunk.  Values of 16 bits: by four (MR = 32) or eight rows (MR = 16) of four or
+// two neighbouring chunks; of 32 bits: by rows four apart, two of eight chunks or four of four.
 template <int CH> __device__ __forceinline__ int key_place(int r, int c) {
     return c ^ (CH == 8 ? (r >> 1) & 7 : r & 15);
 }
-template <int DT, int CH> __device__ __forceinline__ int value_place(int r, int c) {
-    if constexpr (DT == kF32) return c ^ (((r >> 2) & 1) << 3);
-    else return c ^ (CH == 8 ? ((r >> 1) & 1) << 2 : (r & 3) << 2);
+template <int DT, int CH, int MR> __device__ __forceinline__ int value_place(int r, int c) {
+    if constexpr (DT == kF32) return c ^ (MR == 32 ? ((r >> 2) & 1) << 3 : ((r >> 2) & 3) << 2);
+    else if constexpr (MR == 32) return c ^ (CH == 8 ? ((r >> 1) & 1) << 2 : (r & 3) << 2);
+    else return c ^ (CH == 8 ? ((r >> 1) & 3) << 1 : (r & 7) << 1);
 }
 
+// log2 units that a row's maximum may grow by before its sums are rescaled: weights stay
+// below 2^8 (and the float16 ones, raised by 2^6 out of its subnormal range, below 2^14).
+constexpr float kLazy = 8.0f;
+template <int DT> constexpr float kRaise = DT == kF16 ? 6.0f : 0.0f;
+
+// ---- blocks, rows, keys -----------------------------------------------------------------
 // The sequence whose tiles hold slot t: the last b with floor(start_b * G / BM) + b <= t.
 // (The slots of a sequence, one more than its whole tiles may need, follow from the starts
 // alone, so no list of tiles has to be made.)  64 sequences are tried at a time.
@@ -236,32 +288,37 @@ template <int BM> __device__ __forceinline__ int slot_sequence(const AttnArgs& a
         if (k > 1) lo += (k - 1) * step;
         n = min(step, a.B - lo);
     }
-    return __builtin_amdgcn_readfirstlane(lo);
+    return uniform(lo);
 }
 
-// log2 units that a row's maximum may grow by before its sums are rescaled: weights stay
-// below 2^8 (and the float16 ones, raised by 2^6 out of its subnormal range, below 2^14).
-constexpr float kLazy = 8.0f;
-template <int DT> constexpr float kRaise = DT == kF16 ? 6.0f : 0.0f;
+// A block's part of the call: `rows` rows from row0 of its sequence on (of key head hk), over
+// the keys [klo, khi); klo is a multiple of 32.
+struct AttnBlock {
+    AttnSeq s;
+    int hk, split, row0, rows, klo, khi;
+};
+// One of its rows.
+struct AttnRow {
+    int tok, head;
+    int64_t y, out;                            // element of Y, row among all rows of Y
+};
+template <bool PAGED> __device__ __forceinline__ AttnRow attn_row_at(const AttnArgs& a, const AttnBlock& k, int r) {
+    AttnRow w;
+    const uint32_t row = (uint32_t)(k.row0 + r);
+    w.tok = (int)a.fd_g.div(row);
+    w.head = k.hk * a.G + (int)(row - (uint32_t)w.tok * (uint32_t)a.G);
+    const int64_t token = PAGED ? k.s.tok0 + w.tok : (int64_t)k.s.b * a.Sq + w.tok;
+    w.out = token * a.Hq + w.head;
+    w.y = PAGED ? token * a.yt + w.head * a.yh : k.s.b * a.yb + w.tok * a.yt + w.head * a.yh;
+    return w;
+}
 
-template <int DT, int D, bool PAGED, bool MASK, int RW, int KW, int BN>
-__global__ __launch_bounds__(64 * RW * KW, D * kElem<DT> <= 256 ? 2 : 1) void k_attn_tiles(AttnArgs a) {
-    constexpr int ES = kElem<DT>, VEC = 16 / ES, CH = D / VEC, RB = D * ES, W = RW * KW;
-    constexpr int BM = 32 * RW, NSUB = BN / (32 * KW), NI = BN * RB / (1024 * W), RPI = 1024 / RB;
-    constexpr int NS = CH / 2;                 // chunk pairs of a head: products of S' per 32 keys
-    constexpr int ND = D / 32;                 // 32-column blocks of the result
-    static_assert(NSUB >= 1 && NI >= 1 && RPI >= 1, "tile");
-    // distinct arrays: a read of one does not wait for the loads in flight to the other
-    __shared__ __attribute__((aligned(1024))) char k0_[BN * RB], k1_[BN * RB], v0_[BN * RB], v1_[BN * RB];
-    __shared__ int missing;                    // a key's page was none of the cache's
-    const int t = (int)threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int lr = lane & 31, h = lane >> 5;
-
-    // ---- this block's rows and keys
+// false: nothing to do for this block (of `threads` threads).
+template <bool PAGED, int BM> __device__ __forceinline__ bool attn_block(const AttnArgs& a, int threads, AttnBlock& k) {
     uint32_t bid = blockIdx.x;
-    const int hk = (int)(bid % (uint32_t)a.Hkv);
+    k.hk = (int)(bid % (uint32_t)a.Hkv);
     bid /= (uint32_t)a.Hkv;
-    const int split = (int)(bid % (uint32_t)a.nsplit);
+    k.split = (int)(bid % (uint32_t)a.nsplit);
     bid /= (uint32_t)a.nsplit;
     int b, tile;
     if constexpr (PAGED) {
@@ -269,326 +326,536 @@ __global__ __launch_bounds__(64 * RW * KW, D * kElem<DT> <= 256 ? 2 : 1) void k_
         const int64_t slot = (int64_t)a.tiles - 1 - bid;
         b = slot_sequence<BM>(a, slot);
         const int64_t tl = slot - slot_base<BM>(a, b);
-        tile = uniform(tl < 0 ? -1 : (int)tl);
-        if (tile < 0) return;
+        tile = uniform(tl < 0 || tl > 0x7FFFFFFF / BM ? -1 : (int)tl);
+        if (tile < 0) return false;
     } else {
         const uint32_t tl = bid % (uint32_t)a.tiles;
         tile = a.tiles - 1 - (int)tl;
         b = (int)(bid / (uint32_t)a.tiles);
     }
-    AttnSeq s = attn_seq<PAGED>(a, b);
-    s.n = uniform(s.n);
-    s.len = uniform(s.len);
-    s.first = uniform(s.first);
-    const int64_t nrows = (int64_t)s.n * a.G;
-    const int64_t row0 = (int64_t)tile * BM;
-    if (row0 >= nrows) return;
-    const int rows = (int)min((int64_t)BM, nrows - row0);
-    const int tok0 = (int)(row0 / a.G);                          // first and last token of the block
-    const int tok1 = (int)((row0 + rows - 1) / a.G);
-    // keys of the block, cut to this split's share (whole tiles)
-    int klo = attn_lo(a, s, tok0), khi = attn_hi(a, s, tok1);
-    if (a.nsplit > 1) {
-        const int share = ((khi - klo + a.nsplit - 1) / a.nsplit + BN - 1) / BN * BN;
-        const int64_t at = (int64_t)klo + (int64_t)split * share;
-        khi = (int)min((int64_t)khi, at + share);
-        klo = (int)min((int64_t)khi, at);
+    k.s = attn_seq<PAGED>(a, b);
+    k.s.n = uniform(k.s.n);
+    k.s.len = uniform(k.s.len);
+    k.s.first = uniform(k.s.first);
+    const int nrows = k.s.n * a.G;             // below 2^31: the host sees to it
+    k.row0 = tile * BM;
+    if (k.row0 >= nrows) return false;
+    k.rows = min(BM, nrows - k.row0);
+    const int tok0 = (int)a.fd_g.div((uint32_t)k.row0), tok1 = (int)a.fd_g.div((uint32_t)(k.row0 + k.rows - 1));
+    k.klo = attn_lo(a, k.s, tok0) & ~31;
+    k.khi = attn_hi(a, k.s, tok1);
+    if (a.nsplit > 1) {                        // this split's share
+        const int64_t at = (int64_t)k.klo + (int64_t)k.split * a.share;
+        if (k.split + 1 < a.nsplit) k.khi = (int)min((int64_t)k.khi, at + a.share);      // the last one takes what is left
+        if (at >= k.khi) {                     // no keys: it weighs nothing
+            for (int r = (int)threadIdx.x; r < k.rows; r += threads)
+                a.part_ml[(int64_t)k.split * a.rows + attn_row_at<PAGED>(a, k, r).out] = make_float2(-INFINITY, 0.0f);
+            return false;
+        }
+        k.klo = (int)at;
     }
-    const int last = s.len - 1;
+    return true;
+}
 
-    // ---- this lane's row
-    const int wrow = KW > 1 ? 0 : wave * 32;                     // the wave's first row in the block
-    const int my = min(wrow + lr, rows - 1);
-    const bool live = wrow + lr < rows;
-    const int64_t row = row0 + my;
-    const int tok = (int)(row / a.G), head = hk * a.G + (int)(row - (int64_t)tok * a.G);
-    const int lo = max(klo, attn_lo(a, s, tok)), hi = min(khi, attn_hi(a, s, tok));
-    // keys that some row of the wave sees, and those that all see
-    const int wtok0 = (int)((row0 + min(wrow, rows - 1)) / a.G), wtok1 = (int)((row0 + min(wrow + 31, rows - 1)) / a.G);
-    const int any_lo = max(klo, attn_lo(a, s, wtok0)), any_hi = min(khi, attn_hi(a, s, wtok1));
-    const int all_lo = max(klo, attn_lo(a, s, wtok1)), all_hi = min(khi, attn_hi(a, s, wtok0));
-    const bool wlive = wrow < rows;
+// ---- a wave's sums ------------------------------------------------------------------------
+// EARLY: LDS fragments are read ahead of a group of products, where no other wave of the SIMD
+// works meanwhile.
+template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnWave {
+    typedef typename AttnAcc<MR>::type Acc;
+    static constexpr int ES = kElem<DT>, VEC = 16 / ES, CH = D / VEC, RB = D * ES;
+    static constexpr int GR = 64 / MR;         // lanes of a row
+    static constexpr int NP = 32 / GR;         // keys of a lane, of 32
+    static constexpr int NS = CH / GR;         // chunks of a row of Q in a lane
+    static constexpr int NO = D / MR, NR = MR * MR / 64;       // result blocks, registers of each
 
     uint4 q[NS];
-    {
-        const int64_t qo = PAGED ? (s.tok0 + tok) * a.qt + head * a.qh : s.b * a.qb + tok * a.qt + head * a.qh;
+    Acc o[NO];
+    float m, l, c;                             // maximum so far, this lane's part of the sum, exp2's factor
+    int lr, h;                                 // the lane's row, and which of the row's lanes it is
+    int lo, hi;                                // keys that the row sees
+    int any_lo, any_hi, all_lo, all_hi;        // that some row of the wave sees, and all of them
+    int64_t mo;                                // the row's mask
+    bool live;
+
+    // key i of this lane's, of 32; and column i of a result block's registers
+    TOHIP_INLINE __device__ int key(int i) const { return 4 * GR * (i >> 2) + 4 * h + (i & 3); }
+
+    // Rows [r0, r0 + MR) of the block; those past its end repeat the last and are not stored.
+    TOHIP_INLINE __device__ AttnRow begin(const AttnArgs& a, const AttnBlock& k, int r0) {
+        const int lane = (int)(threadIdx.x & 63);
+        lr = lane & (MR - 1);
+        h = lane / MR;
+        live = r0 + lr < k.rows;
+        const AttnRow w = attn_row_at<PAGED>(a, k, min(r0 + lr, k.rows - 1));
+        lo = max(k.klo, attn_lo(a, k.s, w.tok));
+        hi = min(k.khi, attn_hi(a, k.s, w.tok));
+        const int tok0 = (int)a.fd_g.div((uint32_t)(k.row0 + min(r0, k.rows - 1)));
+        const int tok1 = (int)a.fd_g.div((uint32_t)(k.row0 + min(r0 + MR - 1, k.rows - 1)));
+        any_lo = max(k.klo, attn_lo(a, k.s, tok0));
+        any_hi = r0 < k.rows ? min(k.khi, attn_hi(a, k.s, tok1)) : 0;
+        all_lo = max(k.klo, attn_lo(a, k.s, tok1));
+        all_hi = min(k.khi, attn_hi(a, k.s, tok0));
+        const int64_t qo = PAGED ? (k.s.tok0 + w.tok) * a.qt + w.head * a.qh : k.s.b * a.qb + w.tok * a.qt + w.head * a.qh;
         const uint4* qp = reinterpret_cast<const uint4*>((const char*)a.q + qo * ES);
         const int qch = a.Dk / VEC;
 #pragma unroll
         for (int i = 0; i < NS; i++) {
-            const int c = 2 * i + h;
-            q[i] = live && c < qch ? qp[c] : uint4{0, 0, 0, 0};
+            const int ch = GR * i + h;
+            q[i] = live && ch < qch ? qp[ch] : uint4{0, 0, 0, 0};
+        }
+        mo = MASK ? k.s.b * a.mb + w.head * a.mh + w.tok * a.mq : 0;
+#pragma unroll
+        for (int d = 0; d < NO; d++)
+#pragma unroll
+            for (int i = 0; i < NR; i++) o[d][i] = 0.0f;
+        m = -INFINITY;
+        l = 0.0f;
+        c = MASK ? kLog2e : a.scale * kLog2e;
+        return w;
+    }
+
+    // Waits for Q here: waited for at its first use, inside the walk, the compiler would wait for
+    // every load in flight there, each time round.
+    TOHIP_INLINE __device__ void have_q() {
+#pragma unroll
+        for (int i = 0; i < NS; i++) asm volatile("" : "+v"(q[i].x), "+v"(q[i].y), "+v"(q[i].z), "+v"(q[i].w));
+    }
+
+    // q.k of the 32 keys in rows sub .. of a tile (without a mask unscaled), -inf where not seen.
+    TOHIP_INLINE __device__ void scores(const AttnArgs& a, const char* kt, int sub, int jb, float (&x)[NP]) {
+        Acc s[NP / NR];
+#pragma unroll
+        for (int u = 0; u < NP / NR; u++) {
+#pragma unroll
+            for (int i = 0; i < NR; i++) s[u][i] = 0.0f;
+        }
+        constexpr int U = NP / NR, NF = NS * U, G = !EARLY ? 1 : NF < 8 ? NF : 8;
+#pragma unroll
+        for (int g = 0; g < NF; g += G) {
+            uint4 kf[G];
+            uint32_t at[G];
+#pragma unroll
+            for (int f = 0; f < G; f++) {
+                const int i = (g + f) / U, r = (g + f) % U * MR + lr;
+                const char* p = kt + (sub + r) * RB + key_place<CH>(r, GR * i + h) * 16;
+                if constexpr (EARLY) at[f] = lds_address(p);
+                else kf[f] = *reinterpret_cast<const uint4*>(p);
+            }
+            if constexpr (G == 4) read_keys4(at, kf);
+            if constexpr (G == 8) read_keys8(at, kf);
+#pragma unroll
+            for (int f = 0; f < G; f++) {
+                const int i = (g + f) / U, u = (g + f) % U;
+                if constexpr (DT == kF32) {
+                    s[u] = mfma32<MR>(u2f(kf[f].x), u2f(q[i].x), s[u]);
+                    s[u] = mfma32<MR>(u2f(kf[f].y), u2f(q[i].y), s[u]);
+                    s[u] = mfma32<MR>(u2f(kf[f].z), u2f(q[i].z), s[u]);
+                    s[u] = mfma32<MR>(u2f(kf[f].w), u2f(q[i].w), s[u]);
+                } else {
+                    s[u] = mfma16<DT, MR>(kf[f], q[i], s[u]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NP; i++) x[i] = s[i / NR][i % NR];
+        if constexpr (MASK) {
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                const int j = jb + key(i);
+                float bias = -INFINITY;
+                if (j >= lo && j < hi) {
+                    const int64_t at = mo + (int64_t)j * a.mk;
+                    if (a.mask_dt == kU8 || a.mask_dt == kI8) bias = ((const uint8_t*)a.mask)[at] ? 0.0f : -INFINITY;
+                    else if (a.mask_dt == kF32) bias = ((const float*)a.mask)[at];
+                    else bias = ld_f<DT>(a.mask, at);
+                }
+                x[i] = bias == -INFINITY ? -INFINITY : __builtin_fmaf(x[i], a.scale, bias);
+            }
+        } else if (jb < all_lo || jb + 32 > all_hi) {
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                const int j = jb + key(i);
+                x[i] = j >= lo && j < hi ? x[i] : -INFINITY;
+            }
         }
     }
-    const int64_t mo = MASK ? s.b * a.mb + head * a.mh + tok * a.mq : 0;
 
-    // ---- loads: instruction i of this wave fills rows (i W + wave) RPI ..
-    const char* kbase = (const char*)a.k + hk * a.kh * ES;
-    const char* vbase = (const char*)a.v + hk * a.vh * ES;
-    const int lrow = lane / CH, lslot = lane % CH, kch = a.Dk / VEC, vch = a.Dv / VEC;
-    int page[PAGED ? NI : 1];
-    auto find_pages = [&](int j0) {
-        if constexpr (PAGED) {
+    // The scores as weights against the running maximum, which grows with them.
+    TOHIP_INLINE __device__ void weigh(float (&x)[NP]) {
+        float top = x[0];
 #pragma unroll
-            for (int i = 0; i < NI; i++) page[i] = attn_page(a, b, min(j0 + (i * W + wave) * RPI + lrow, last));
-        }
-    };
-    auto load = [&](char* kt, char* vt, int j0) {
-#pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const int r = (i * W + wave) * RPI + lrow, j = min(j0 + r, last);
-            int pg = PAGED ? page[i] : 0;
-            if (PAGED && pg < 0) {
-                missing = 1;
-                pg = 0;
-            }
-            const KeyRow at = attn_key_row<PAGED>(a, b, pg, j);
-            const int kc = key_place<CH>(r, lslot), vc = value_place<DT, CH>(r, lslot);
-            if (kc < kch) load_lds16(kbase + at.k * ES + kc * 16, kt + (i * W + wave) * 1024);
-            if (vc < vch) load_lds16(vbase + at.v * ES + vc * 16, vt + (i * W + wave) * 1024);
-        }
-    };
-
-    // ---- the sums
-    floatx16 o[ND];
-#pragma unroll
-    for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;             // the row's maximum so far; this lane's part of the sum
-    const float c = MASK ? kLog2e : a.scale * kLog2e;
-
-    auto work = [&](const char* kt, const char* vt, int j0) {
-#pragma unroll
-        for (int n = 0; n < NSUB; n++) {
-            const int sub = KW > 1 ? (n * KW + wave) * 32 : n * 32, jb = j0 + sub;
-            if (!wlive || jb >= any_hi || jb + 32 <= any_lo) continue;
-            floatx16 x;
-#pragma unroll
-            for (int i = 0; i < 16; i++) x[i] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < NS; i++) {
-                const uint4 kf = *reinterpret_cast<const uint4*>(kt + (sub + lr) * RB + key_place<CH>(lr, 2 * i + h) * 16);
-                x = mfma_chunk<DT>(kf, q[i], x);
-            }
-            if constexpr (MASK) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int j = jb + 8 * (i >> 2) + 4 * h + (i & 3);
-                    float bias = -INFINITY;
-                    if (j >= lo && j < hi) {
-                        const int64_t at = mo + (int64_t)j * a.mk;
-                        if (a.mask_dt == kU8 || a.mask_dt == kI8) bias = ((const uint8_t*)a.mask)[at] ? 0.0f : -INFINITY;
-                        else if (a.mask_dt == kF32) bias = ((const float*)a.mask)[at];
-                        else bias = ld_f<DT>(a.mask, at);
-                    }
-                    x[i] = bias == -INFINITY ? -INFINITY : __builtin_fmaf(x[i], a.scale, bias);
-                }
-            } else if (jb < all_lo || jb + 32 > all_hi) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int j = jb + 8 * (i >> 2) + 4 * h + (i & 3);
-                    x[i] = j >= lo && j < hi ? x[i] : -INFINITY;
-                }
-            }
-            float top = x[0];
-#pragma unroll
-            for (int i = 1; i < 16; i++) top = fmaxf(top, x[i]);
-            float ta, tb;
-            permlane_pair<32>(top, ta, tb);
+        for (int i = 1; i < NP; i++) top = fmaxf(top, x[i]);
+        float ta, tb;
+        if constexpr (GR == 4) {
+            permlane_pair<16>(top, ta, tb);
             top = fmaxf(ta, tb);
-            if (__ballot((top - m) * c > kLazy)) {
-                const float mn = fmaxf(m, top);
-                const float f = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < ND; d++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) o[d][i] *= f;
-                m = mn;
-            }
-            const float base = m == -INFINITY ? 0.0f : m;
-            float p[16];
-            if constexpr (MASK) {
-                // the difference first: a mask of the type's lowest value times log2 e would overflow
-#pragma unroll
-                for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i] - base, c, kRaise<DT>));
-            } else {
-                const float off = kRaise<DT> - base * c;
-#pragma unroll
-                for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, off));
-            }
-#pragma unroll
-            for (int i = 0; i < 16; i++) l += p[i];
-            if constexpr (DT == kF32) {
-                // weight i of both wave halves: keys 8 (i / 4) + i % 4 and 4 further on
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int r = sub + 8 * (i >> 2) + 4 * h + (i & 3);
-#pragma unroll
-                    for (int d = 0; d < ND; d++) {
-                        const float vf = *reinterpret_cast<const float*>(vt + r * RB + value_place<DT, CH>(r, d * 8 + (lr >> 2)) * 16 + (lr & 3) * 4);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, p[i], o[d], 0, 0, 0);
-                    }
-                }
-            } else {
-                const int r4 = (lane & 15) >> 2, cc = (lane >> 4 & 1) * 2 + ((lane & 3) >> 1), in = (lane & 1) * 8;
-#pragma unroll
-                for (int kk = 0; kk < 2; kk++) {
-                    const uint4 pf = pack8<DT>(p + 8 * kk);
-                    const int r = sub + 16 * kk + 4 * h + r4;
-#pragma unroll
-                    for (int d = 0; d < ND; d++) {
-                        const uint2 va = read_turned(vt + r * RB + value_place<DT, CH>(r, d * 4 + cc) * 16 + in);
-                        const uint2 vb = read_turned(vt + (r + 8) * RB + value_place<DT, CH>(r + 8, d * 4 + cc) * 16 + in);
-                        o[d] = mfma_chunk<DT>(uint4{va.x, va.y, vb.x, vb.y}, pf, o[d]);
-                    }
-                }
-            }
         }
-    };
+        permlane_pair<32>(top, ta, tb);
+        top = fmaxf(ta, tb);
+        if (__ballot((top - m) * c > kLazy)) {
+            const float mn = fmaxf(m, top);
+            const float f = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < NO; d++)
+#pragma unroll
+                for (int i = 0; i < NR; i++) o[d][i] *= f;
+            m = mn;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        if constexpr (MASK) {
+            // the difference first: a mask of the type's lowest value times log2 e would overflow
+#pragma unroll
+            for (int i = 0; i < NP; i++) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i] - base, c, kRaise<DT>));
+        } else {
+            const float off = kRaise<DT> - base * c;
+#pragma unroll
+            for (int i = 0; i < NP; i++) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, off));
+        }
+#pragma unroll
+        for (int i = 0; i < NP; i++) l += x[i];
+    }
 
-    // ---- the walk: while tile n is worked on, tile n + 1 is on its way, and the pages of n + 2
-    if (t == 0) missing = 0;
-    if (kch < CH) {                            // columns past the head size: zeros that no load touches
-        for (int i = t; i < BN * CH; i += 64 * W) {
-            reinterpret_cast<uint4*>(k0_)[i] = uint4{0, 0, 0, 0};
-            reinterpret_cast<uint4*>(k1_)[i] = uint4{0, 0, 0, 0};
+    // The weighted values of the 32 keys in rows sub .. of a tile.
+    TOHIP_INLINE __device__ void add(const char* vt, int sub, const float (&p)[NP]) {
+        if constexpr (DT == kF32) {
+#pragma unroll
+            for (int d = 0; d < NO; d++) {
+                // (a lane's rows are turned by the same amount)
+                const char* at = vt + (sub + 4 * h) * RB + value_place<DT, CH, MR>(4 * h, d * (MR / 4) + (lr >> 2)) * 16 + (lr & 3) * 4;
+#pragma unroll
+                for (int g = 0; g < NP; g += 8) {
+                    float vf[8];
+                    if constexpr (EARLY) {
+                        read_column8<RB, 4 * GR>(lds_address(at + GR * g * RB), vf);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            vf[i] = *reinterpret_cast<const float*>(at + (4 * GR * ((g + i) >> 2) + (i & 3)) * RB);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) o[d] = mfma32<MR>(vf[i], p[g + i], o[d]);
+                }
+            }
+        } else {
+            const int lane = (int)(threadIdx.x & 63), r4 = (lane & 15) >> 2;
+            const int cc = (MR == 32 ? ((lane >> 4) & 1) * 2 : 0) + ((lane & 3) >> 1), in = (lane & 1) * 8;
+            constexpr int G = EARLY ? (NO < 4 ? NO : 4) : 1;
+            static_assert(G == 1 || G == 4 || NO == 2, "groups");
+#pragma unroll
+            for (int kk = 0; kk < NP / 8; kk++) {
+                const uint4 pf = __builtin_bit_cast(uint4, round16<DT, 8>(p + 8 * kk));
+                const int r = sub + 8 * GR * kk + 4 * h + r4;
+#pragma unroll
+                for (int g = 0; g < NO; g += G) {
+                    uint2 x[G], y[G];
+                    uint32_t at[G];
+#pragma unroll
+                    for (int f = 0; f < G; f++) {
+                        // (row r + 4 GR is turned by the same amount as row r)
+                        const char* v = vt + r * RB + value_place<DT, CH, MR>(r, (g + f) * (MR / 8) + cc) * 16 + in;
+                        if constexpr (G == 4) {
+                            at[f] = lds_address(v);
+                        } else {
+                            x[f] = read_turned(v);
+                            y[f] = read_turned(v + 4 * GR * RB);
+                        }
+                    }
+                    if constexpr (G == 4) read_values4<4 * GR * RB>(at, x, y);
+#pragma unroll
+                    for (int f = 0; f < G; f++) o[g + f] = mfma16<DT, MR>(uint4{x[f].x, x[f].y, y[f].x, y[f].y}, pf, o[g + f]);
+                }
+            }
         }
     }
-    __syncthreads();
-    const int jbeg = klo, jend = khi;
-    if (jbeg < jend) {
-        find_pages(jbeg);
-        load(k0_, v0_, jbeg);
-        find_pages(jbeg + BN);
-        auto step = [&](int j0, const char* kt, const char* vt, char* kn, char* vn) {
-            wait_all_loads();
-            __builtin_amdgcn_s_barrier();      // every wave's part of this tile is there, and the other buffer is free
-            __builtin_amdgcn_sched_barrier(0);
-            if (j0 + BN < jend) {
-                load(kn, vn, j0 + BN);
-                find_pages(j0 + 2 * BN);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            work(kt, vt, j0);
-        };
-        for (int j0 = jbeg; j0 < jend; j0 += 2 * BN) {
-            step(j0, k0_, v0_, k1_, v1_);
-            if (j0 + BN < jend) step(j0 + BN, k1_, v1_, k0_, v0_);
-        }
-    }
-    __syncthreads();
 
-    // ---- the end: join the waves' keys, divide, store
-    {
+    // Divides, stores, and has rows whose result is not finite (or all: again) computed again.
+    TOHIP_INLINE __device__ void end(const AttnArgs& a, const AttnBlock& k, int r0, const AttnRow& w, bool again) {
         float la, lb;
+        if constexpr (GR == 4) {
+            permlane_pair<16>(l, la, lb);
+            l = la + lb;
+        }
         permlane_pair<32>(l, la, lb);
         l = la + lb;
-    }
-    float m2 = m == -INFINITY ? -INFINITY : m * c - kRaise<DT>;      // log2 units, as l is scaled
-    if constexpr (KW > 1) {
-        static_assert(2 * BN * RB >= KW * 32 * 8, "room for the statistics");
-        float* st = reinterpret_cast<float*>(k0_);                 // [KW][32][2]
-        if (h == 0) {
-            st[(wave * 32 + lr) * 2] = m2;
-            st[(wave * 32 + lr) * 2 + 1] = l;
-        }
-        __syncthreads();
-        float mm = -INFINITY, ll = 0.0f;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const bool parts = a.nsplit > 1;
+        bool bad = again;
 #pragma unroll
-        for (int w = 0; w < KW; w++) mm = fmaxf(mm, st[(w * 32 + lr) * 2]);
+        for (int d = 0; d < NO; d++) {
 #pragma unroll
-        for (int w = 0; w < KW; w++) {
-            const float mw = st[(w * 32 + lr) * 2];
-            ll += mw == -INFINITY ? st[(w * 32 + lr) * 2 + 1] : st[(w * 32 + lr) * 2 + 1] * __builtin_amdgcn_exp2f(mw - mm);
-        }
-        const float f = m2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m2 - mm);
-        // one wave after another adds its part to the first one's
-        float* sum = reinterpret_cast<float*>(v0_);                // [D][32], up to 32 KB
-        static_assert(KW == 1 || BN * RB >= D * 32 * 4, "room for the sums");
-        for (int w = 1; w < KW; w++) {
-            __syncthreads();
-            if (wave == w) {
+            for (int g = 0; g < NR / 4; g++) {
+                const int col = d * MR + key(4 * g);
+                if (col >= a.Dv) continue;
+                float r[4];
 #pragma unroll
-                for (int d = 0; d < ND; d++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) sum[(d * 16 + i) * 64 + lane] = o[d][i] * f;
-            }
-            __syncthreads();
-            if (wave == 0) {
-#pragma unroll
-                for (int d = 0; d < ND; d++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) o[d][i] = (w == 1 ? o[d][i] * f : o[d][i]) + sum[(d * 16 + i) * 64 + lane];
-            }
-        }
-        if (wave != 0) return;
-        m2 = mm;
-        l = ll;
-    }
-    if (!wlive) return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int64_t token = PAGED ? s.tok0 + tok : (int64_t)s.b * a.Sq + tok;
-    const int64_t orow = token * a.Hq + head;                      // of the rows of Y
-    const bool split_out = a.nsplit > 1;
-    bool bad = missing != 0;
-#pragma unroll
-    for (int d = 0; d < ND; d++) {
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const int col = d * 32 + 8 * g + 4 * h;
-            if (col >= a.Dv) continue;
-            float r[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                r[e] = l == 0.0f ? 0.0f : o[d][4 * g + e] * inv;
-                bad |= !(__builtin_fabsf(r[e]) <= 3.402823466e38f);
-            }
-            if (!live) continue;
-            if (split_out) {
-                *reinterpret_cast<float4*>(a.part_o + ((int64_t)split * a.rows + orow) * a.Dv + col) = make_float4(r[0], r[1], r[2], r[3]);
-            } else {
-                const int64_t yo = PAGED ? token * a.yt + head * a.yh : s.b * a.yb + tok * a.yt + head * a.yh;
-                if constexpr (DT == kF32) {
-                    *reinterpret_cast<float4*>((float*)a.y + yo + col) = make_float4(r[0], r[1], r[2], r[3]);
+                for (int e = 0; e < 4; e++) {
+                    r[e] = l == 0.0f ? 0.0f : o[d][4 * g + e] * inv;
+                    bad |= !(__builtin_fabsf(r[e]) <= 3.402823466e38f);
+                }
+                if (!live) continue;
+                if (parts) {
+                    *reinterpret_cast<float4*>(a.part_o + ((int64_t)k.split * a.rows + w.out) * a.Dv + col) = make_float4(r[0], r[1], r[2], r[3]);
+                } else if constexpr (DT == kF32) {
+                    *reinterpret_cast<float4*>((float*)a.y + w.y + col) = make_float4(r[0], r[1], r[2], r[3]);
                 } else {
-                    uint16_t e[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) e[i] = DT == kF16 ? enc_f16(r[i]) : enc_bf16(r[i]);
-                    *reinterpret_cast<uint2*>((uint16_t*)a.y + yo + col) = uint2{e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16};
+                    *reinterpret_cast<uint2*>((uint16_t*)a.y + w.y + col) = __builtin_bit_cast(uint2, round16<DT, 4>(r));
                 }
             }
         }
-    }
-    if (split_out && live && h == 0) a.part_ml[(int64_t)split * a.rows + orow] = make_float2(m2, l);
-    // rows to be computed again, one after the other by the whole wave
-    unsigned long long again = __ballot(bad && live);
-    again = (again | again >> 32) & 0xFFFFFFFFull;
-    for (; again; again &= again - 1) {
-        const int r = __builtin_ctzll(again);
-        const int64_t rw = row0 + wrow + r;
-        const int tk = (int)(rw / a.G), hd = hk * a.G + (int)(rw - (int64_t)tk * a.G);
-        const int64_t tkn = PAGED ? s.tok0 + tk : (int64_t)s.b * a.Sq + tk, orw = tkn * a.Hq + hd;
-        float rm = -INFINITY, rl = 0.0f;
-        if (split_out) {
-            float* po = a.part_o + ((int64_t)split * a.rows + orw) * a.Dv;
-            attn_row<DT, PAGED>(a, s, hd, tk, klo, khi, rm, rl, [&](int d, float v) { po[d] = v; });
-            if (lane == 0) a.part_ml[(int64_t)split * a.rows + orw] = make_float2(rm * kLog2e, rl);
-        } else {
-            const int64_t yo = PAGED ? tkn * a.yt + hd * a.yh : s.b * a.yb + tk * a.yt + hd * a.yh;
-            attn_row<DT, PAGED>(a, s, hd, tk, klo, khi, rm, rl, [&](int d, float v) { st_code<DT>(a.y, yo + d, v); });
+        // l is scaled by 2^(kRaise - m c): its exponent, in log2 units
+        if (parts && live && h == 0)
+            a.part_ml[(int64_t)k.split * a.rows + w.out] = make_float2(m == -INFINITY ? -INFINITY : m * c - kRaise<DT>, l);
+        unsigned long long rows = __ballot(bad && live);
+        rows |= rows >> 32;
+        if constexpr (GR == 4) rows |= rows >> 16;
+        rows &= (1ull << MR) - 1;
+        for (; rows; rows &= rows - 1) {
+            const AttnRow x = attn_row_at<PAGED>(a, k, r0 + __builtin_ctzll(rows));
+            float rm = -INFINITY, rl = 0.0f;
+            if (parts) {
+                float* po = a.part_o + ((int64_t)k.split * a.rows + x.out) * a.Dv;
+                attn_row<DT, PAGED>(a, k.s, x.head, x.tok, k.klo, k.khi, rm, rl, [&](int d, float v) { po[d] = v; });
+                if ((threadIdx.x & 63) == 0) a.part_ml[(int64_t)k.split * a.rows + x.out] = make_float2(rm * kLog2e, rl);
+            } else {
+                attn_row<DT, PAGED>(a, k.s, x.head, x.tok, k.klo, k.khi, rm, rl, [&](int d, float v) { st_code<DT>(a.y, x.y + d, v); });
+            }
         }
     }
+};
+
+// ---- loads of a tile ------------------------------------------------------------------------
+// A tile of keys starts at a multiple of 32.  Instruction i of wave w fills the rows
+// (i W + w) RPI .. of K's or V's tile.  The first rows' offsets are worked out by one lane each,
+// all at once; a lane's offset from them is kept in a register: worked out per lane and
+// instruction, the addresses of paged keys took longer than the loads themselves.  Rows past the last key
+// repeat it.  Pages whose size an instruction's rows do not divide are looked up row by row.
+// A wave holds 64 of the sequence's page numbers in a register: looked up in memory for each
+// tile, they were a second trip to it per tile (32 keys of one wave: 1.4 us).
+// Columns past the head size repeat the last chunk: Q is zero there, and where the product of
+// a value that is not finite is not either, the row is computed again.
+template <int DT, int D, bool PAGED, int MR, int W> struct AttnLoads {
+    static constexpr int ES = kElem<DT>, VEC = 16 / ES, CH = D / VEC, RB = D * ES, RPI = 1024 / RB;
+    const char *kbase, *vbase;
+    int table;                                 // lane n: page from + n of the sequence
+    int wave, lane, lrow, lslot, kch, vch, kstep, vstep, last, b;
+    int from;
+    int64_t koff, voff;                        // of the found tile: lane n has its row n RPI's
+    bool even;
+    int worst;                                 // < 0: some key's page was none of the cache's
+
+    TOHIP_INLINE __device__ void begin(const AttnArgs& a, const AttnBlock& k, int w) {
+        lane = (int)(threadIdx.x & 63);
+        kbase = (const char*)a.k + k.hk * a.kh * ES;
+        vbase = (const char*)a.v + k.hk * a.vh * ES;
+        wave = w;
+        lrow = lane / CH;
+        lslot = lane % CH;
+        kch = a.Dk / VEC;
+        vch = a.Dv / VEC;
+        kstep = (int)a.kt * ES;
+        vstep = (int)a.vt * ES;
+        last = k.s.len - 1;
+        b = k.s.b;
+        even = !PAGED || (a.ps & (RPI - 1)) == 0;
+        worst = 0;
+        koff = voff = 0;
+        table = -1;
+        from = -64;                            // nothing in it yet
+    }
+    TOHIP_INLINE __device__ int entry(const AttnArgs& a, int j) const { return __shfl(table, (int)a.fd_ps.div((uint32_t)j) - from); }
+    // Looks up the pages of the tile of KEYS keys at j0, and where its instructions' rows begin.
+    template <int KEYS> TOHIP_INLINE __device__ void find(const AttnArgs& a, int j0) {
+        const int end = min(j0 + KEYS - 1, last), j = min(j0 + lane * RPI, end);
+        int pg = 0;
+        if constexpr (PAGED) {
+            if ((int)a.fd_ps.div((uint32_t)end) >= from + 64) {
+                from = (int)a.fd_ps.div((uint32_t)min(j0, last));
+                const int i = min(from + lane, (int)a.fd_ps.div((uint32_t)last));
+                const int64_t p = a.pages[(int64_t)b * a.max_pages + i];
+                table = p >= 0 && p < a.npages ? (int)p : -1;
+            }
+            if (!even) return;
+            pg = entry(a, j);
+            if (__ballot(pg < 0)) worst = -1;
+            pg = max(pg, 0);
+        }
+        const KeyRow at = attn_key_row<PAGED>(a, b, pg, j);
+        koff = at.k * ES;
+        voff = at.v * ES;
+    }
+    // One operand's tile (V: the values').
+    template <bool V, int NI> TOHIP_INLINE __device__ void load(const AttnArgs& a, char* to, int j0) {
+        const char* base = V ? vbase : kbase;
+        const int step = V ? vstep : kstep, ch = (V ? vch : kch) - 1;
+        auto chunk = [&](int r) TOHIP_INLINE {
+            return (uint32_t)min(V ? value_place<DT, CH, MR>(r, lslot) : key_place<CH>(r, lslot), ch) * 16u;
+        };
+        auto first = [&](int i) TOHIP_INLINE {                 // the address of the instruction's first row
+            const uint64_t off = (uint64_t)(V ? voff : koff);
+            const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)off, i * W + wave);
+            const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(off >> 32), i * W + wave);
+            return base + (((uint64_t)hi << 32) | lo);
+        };
+        if (even && j0 + NI * W * RPI - 1 <= last) {
+#pragma unroll
+            for (int i = 0; i < NI; i++)
+                load_lds16(first(i) + ((uint32_t)(lrow * step) + chunk((i * W + wave) * RPI + lrow)), to + (i * W + wave) * 1024);
+        } else if (even) {
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int r0 = (i * W + wave) * RPI, j = min(j0 + r0, last);
+                load_lds16(first(i) + ((uint32_t)(min(lrow, last - j) * step) + chunk(r0 + lrow)), to + (i * W + wave) * 1024);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int r = (i * W + wave) * RPI + lrow, j = min(j0 + r, last);
+                int pg = 0;
+                if constexpr (PAGED) {
+                    pg = entry(a, j);
+                    if (__ballot(pg < 0)) worst = -1;
+                    pg = max(pg, 0);
+                }
+                const KeyRow at = attn_key_row<PAGED>(a, b, pg, j);
+                load_lds16(base + (V ? at.v : at.k) * ES + chunk(r), to + (i * W + wave) * 1024);
+            }
+        }
+    }
+};
+
+// Prompts: four waves of 32 rows share tiles of BN keys.  While tile n is worked on, tile n + 1
+// is on its way.
+template <int DT, int D, bool PAGED, bool MASK, int BN>
+__global__ __launch_bounds__(256, D * kElem<DT> <= 256 ? 2 : 1) void k_attn_tiles(AttnArgs a) {
+    typedef AttnWave<DT, D, PAGED, MASK, 32, false> Wave;
+    constexpr int RB = Wave::RB, NI = BN * RB / 4096;
+    static_assert(NI >= 1, "tile");
+    // distinct arrays: a read of one does not wait for the loads in flight to the other
+    __shared__ __attribute__((aligned(1024))) char k0_[BN * RB], k1_[BN * RB], v0_[BN * RB], v1_[BN * RB];
+    __shared__ int missing;                    // a key's page was none of the cache's
+    const int t = (int)threadIdx.x, wave = uniform(t >> 6);
+    AttnBlock k;
+    if (!attn_block<PAGED, 128>(a, 256, k)) return;
+    Wave w;
+    const AttnRow row = w.begin(a, k, wave * 32);
+    AttnLoads<DT, D, PAGED, 32, 4> ld;
+    ld.begin(a, k, wave);
+    if (t == 0) missing = 0;
+    __syncthreads();
+    auto work = [&](const char* kt, const char* vt, int j0) TOHIP_INLINE {
+#pragma unroll
+        for (int sub = 0; sub < BN; sub += 32) {
+            if (j0 + sub >= w.any_hi || j0 + sub + 32 <= w.any_lo) continue;
+            float x[Wave::NP];
+            w.scores(a, kt, sub, j0 + sub, x);
+            w.weigh(x);
+            w.add(vt, sub, x);
+        }
+    };
+    auto step = [&](int j0, const char* kt, const char* vt, char* kn, char* vn) TOHIP_INLINE {
+        wait_loads<0>();
+        __builtin_amdgcn_s_barrier();          // every wave's part of this tile is there, and the other buffer is free
+        __builtin_amdgcn_sched_barrier(0);
+        if (j0 + BN < k.khi) {
+            ld.template load<false, NI>(a, kn, j0 + BN);
+            ld.template load<true, NI>(a, vn, j0 + BN);
+            ld.template find<BN>(a, j0 + 2 * BN);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        work(kt, vt, j0);
+    };
+    if (k.klo < k.khi) {
+        ld.template find<BN>(a, k.klo);
+        if (PAGED) w.have_q();
+        ld.template load<false, NI>(a, k0_, k.klo);
+        ld.template load<true, NI>(a, v0_, k.klo);
+        ld.template find<BN>(a, k.klo + BN);
+        if (!PAGED) w.have_q();
+        for (int j0 = k.klo; j0 < k.khi; j0 += 2 * BN) {
+            step(j0, k0_, v0_, k1_, v1_);
+            if (j0 + BN < k.khi) step(j0 + BN, k1_, v1_, k0_, v0_);
+        }
+    }
+    if (PAGED && ld.worst < 0) missing = 1;
+    __syncthreads();
+    if (wave * 32 < k.rows) w.end(a, k, wave * 32, row, missing != 0);
+}
+
+// Few rows: a block is one wave, so nothing waits for another.  K and V have two buffers of
+// 32 keys each; K's is filled again as soon as its scores are made and V's as soon as it is
+// added, so three of the four are in flight while one is worked on (filled a whole tile at a
+// time, 64 tokens over 8192 keys took 261 us).
+template <int DT, int D, bool PAGED, bool MASK, int MR>
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D * kElem<DT> <= 256 ? 2 : 1))) void k_attn_few(AttnArgs a) {
+    typedef AttnWave<DT, D, PAGED, MASK, MR, (MR == 16 || D <= 128)> Wave;      // (as far as registers go)
+    constexpr int RB = Wave::RB, NI = 32 * RB / 1024;
+    __shared__ __attribute__((aligned(1024))) char k0_[32 * RB], k1_[32 * RB], v0_[32 * RB], v1_[32 * RB];
+    AttnBlock k;
+    if (!attn_block<PAGED, MR>(a, 64, k)) return;
+    Wave w;
+    const AttnRow row = w.begin(a, k, 0);
+    AttnLoads<DT, D, PAGED, MR, 1> ld;
+    ld.begin(a, k, 0);
+    // In flight behind a tile's K: its V, and K and V of the next tile if there is one; behind
+    // its V: those, and K of the tile after that.
+    auto step = [&](int j0, char* kt, char* vt, bool next, bool third) TOHIP_INLINE {
+        float x[Wave::NP];
+        if (next) wait_loads<3 * NI>();
+        else wait_loads<NI>();
+        __builtin_amdgcn_sched_barrier(0);
+        w.scores(a, kt, 0, j0, x);
+        if (third) ld.template load<false, NI>(a, kt, j0 + 64);
+        __builtin_amdgcn_sched_barrier(0);
+        w.weigh(x);
+        if (third) wait_loads<3 * NI>();
+        else if (next) wait_loads<2 * NI>();
+        else wait_loads<0>();
+        __builtin_amdgcn_sched_barrier(0);
+        w.add(vt, 0, x);
+        if (third) {
+            ld.template load<true, NI>(a, vt, j0 + 64);
+            ld.template find<32>(a, j0 + 96);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (k.klo < k.khi) {
+        ld.template find<32>(a, k.klo);
+        if (PAGED) w.have_q();
+        ld.template load<false, NI>(a, k0_, k.klo);
+        ld.template load<true, NI>(a, v0_, k.klo);
+        if (k.klo + 32 < k.khi) {
+            ld.template find<32>(a, k.klo + 32);
+            ld.template load<false, NI>(a, k1_, k.klo + 32);
+            ld.template load<true, NI>(a, v1_, k.klo + 32);
+            ld.template find<32>(a, k.klo + 64);
+        }
+        if (!PAGED) w.have_q();
+        // (a loop of its own for the steps with nothing conditional about their loads, or the
+        // compiler, which does not see which waits belong to which loads, waits for all of them)
+        int j0 = k.klo;
+        for (; j0 + 96 < k.khi; j0 += 64) {
+            step(j0, k0_, v0_, true, true);
+            step(j0 + 32, k1_, v1_, true, true);
+        }
+        for (; j0 < k.khi; j0 += 64) {
+            step(j0, k0_, v0_, j0 + 32 < k.khi, j0 + 64 < k.khi);
+            if (j0 + 32 < k.khi) step(j0 + 32, k1_, v1_, j0 + 64 < k.khi, false);
+        }
+    }
+    w.end(a, k, 0, row, PAGED && ld.worst < 0);
 }
 
 // ---- the splits of a row together -----------------------------------------------------
-// y = sum_s w_s o_s / sum_s w_s, w_s = l_s 2^(m_s - max): four columns per thread.
-template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, int quads) {
-    const int64_t n = a.rows * quads, step = (int64_t)gridDim.x * 256;
-    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < n; u += step) {
-        const int64_t row = u / quads;
-        const int col = (int)(u - row * quads) * 4;
+// y = sum_s w_s o_s, w_s = l_s 2^(m_s - max) / sum: a wave per row.  Lanes hold the splits'
+// weights, two each; then groups of Dv / 4 lanes add every group's share of the splits, four
+// columns per lane, with four splits' loads in flight (one split after the other, by a thread
+// per four columns, took 38 us for 47 splits of 16 rows).
+template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
+    const int lane = (int)threadIdx.x & 63, quads = a.Dv / 4, groups = 64 / quads;
+    const int grp = lane / quads, col = (lane - grp * quads) * 4;
+    const int64_t step = (int64_t)gridDim.x * 4;
+    for (int64_t row = (int64_t)blockIdx.x * 4 + uniform((int)(threadIdx.x >> 6)); row < a.rows; row += step) {
         const int64_t token = row / a.Hq;
         const int head = (int)(row - token * a.Hq);
         int64_t yo;
@@ -599,44 +866,66 @@ template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_join
             const int64_t b = token / a.Sq;
             yo = b * a.yb + (token - b * a.Sq) * a.yt + head * a.yh;
         }
-        float m = -INFINITY;
-        for (int s = 0; s < a.nsplit; s++) m = fmaxf(m, a.part_ml[s * a.rows + row].x);
-        auto weight = [&](float2 ml) { return ml.y * (ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m)); };
-        float total = 0.0f, r[4] = {};
-        for (int s = 0; s < a.nsplit; s++) {
-            const float2 ml = a.part_ml[s * a.rows + row];
-            if (ml.y != 0.0f) total += weight(ml);
-        }
+        const float2 none = make_float2(-INFINITY, 0.0f);
+        const float2 ml0 = lane < a.nsplit ? a.part_ml[lane * a.rows + row] : none;
+        const float2 ml1 = lane + 64 < a.nsplit ? a.part_ml[(lane + 64) * a.rows + row] : none;
+        const float m = wave_allreduce(fmaxf(ml0.x, ml1.x), [](float x, float y) { return fmaxf(x, y); });
+        auto weight = [&](float2 ml) {         // 0 for a split that saw no key
+            return ml.y == 0.0f ? 0.0f : ml.y * (ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m));
+        };
+        const float w0 = weight(ml0), w1 = weight(ml1);
+        const float total = wave_allreduce(w0 + w1, [](float x, float y) { return x + y; });
         // divided before the sum, which then cannot leave the range of its terms
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        for (int s = 0; s < a.nsplit; s++) {
-            const float2 ml = a.part_ml[s * a.rows + row];
-            if (ml.y == 0.0f) continue;                      // saw no key
-            const float w = weight(ml) * inv;
-            if (w == 0.0f) continue;                         // weighs nothing
-            const float4 v = *reinterpret_cast<const float4*>(a.part_o + (s * a.rows + row) * a.Dv + col);
-            r[0] = __builtin_fmaf(w, v.x, r[0]);
-            r[1] = __builtin_fmaf(w, v.y, r[1]);
-            r[2] = __builtin_fmaf(w, v.z, r[2]);
-            r[3] = __builtin_fmaf(w, v.w, r[3]);
-        }
+        float r[4] = {};
+        for (int s0 = 0; s0 < a.nsplit; s0 += 4 * groups) {
+            float w[4];
+            float4 v[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) st_code<DT>(a.y, yo + col + e, r[e]);
+            for (int i = 0; i < 4; i++) {
+                const int s = s0 + i * groups + grp;
+                w[i] = (s < 64 ? __shfl(w0, s & 63) : 0.0f) + (s >= 64 ? __shfl(w1, s & 63) : 0.0f);
+                if (s >= a.nsplit || grp >= groups) w[i] = 0.0f;
+                // a split that weighs nothing is not read: it may have stored nothing
+                v[i] = make_float4(0, 0, 0, 0);
+                if (w[i] != 0.0f) v[i] = *reinterpret_cast<const float4*>(a.part_o + (s * a.rows + row) * a.Dv + col);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float f = w[i] * inv;
+                if (f == 0.0f) continue;
+                r[0] = __builtin_fmaf(f, v[i].x, r[0]);
+                r[1] = __builtin_fmaf(f, v[i].y, r[1]);
+                r[2] = __builtin_fmaf(f, v[i].z, r[2]);
+                r[3] = __builtin_fmaf(f, v[i].w, r[3]);
+            }
+        }
+        for (int g = 1; g < groups; g++) {     // the groups' parts, in order
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float o = __shfl(r[e], (lane + g * quads) & 63);
+                if (grp == 0) r[e] += o;
+            }
+        }
+        if (grp == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) st_code<DT>(a.y, yo + col + e, r[e]);
+        }
     }
 }
 
 // ---- launches -------------------------------------------------------------------------
-// How a call is cut into blocks: worked out on the host (attention.hip) from sizes alone.
-template <int DT, int D, int RW, int KW, int BN> void launch_tiles_of(const AttnArgs& a, bool paged, unsigned blocks, hipStream_t s) {
-    constexpr int threads = 64 * RW * KW;
-    if (paged) hipLaunchKernelGGL((k_attn_tiles<DT, D, true, false, RW, KW, BN>), dim3(blocks), dim3(threads), 0, s, a);
-    else if (a.mask) hipLaunchKernelGGL((k_attn_tiles<DT, D, false, true, RW, KW, BN>), dim3(blocks), dim3(threads), 0, s, a);
-    else hipLaunchKernelGGL((k_attn_tiles<DT, D, false, false, RW, KW, BN>), dim3(blocks), dim3(threads), 0, s, a);
+// How a call is cut into blocks is worked out on the host (attention.hip), from sizes alone.
+template <int DT, int D, bool PAGED, bool MASK> void launch_tiles_of(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
+    constexpr int BN = attn_tile_keys(D * kElem<DT>);
+    if (p.rows == 16) hipLaunchKernelGGL((k_attn_few<DT, D, PAGED, MASK, 16>), dim3(p.blocks), dim3(64), 0, s, a);
+    else if (p.rows == 32) hipLaunchKernelGGL((k_attn_few<DT, D, PAGED, MASK, 32>), dim3(p.blocks), dim3(64), 0, s, a);
+    else hipLaunchKernelGGL((k_attn_tiles<DT, D, PAGED, MASK, BN>), dim3(p.blocks), dim3(256), 0, s, a);
 }
 template <int DT, int D> void launch_tiles_d(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
-    constexpr AttnTile big = attn_tile(D * kElem<DT>, false), few = attn_tile(D * kElem<DT>, true);
-    if (p.few) launch_tiles_of<DT, D, few.rw, few.kw, few.bn>(a, p.paged, p.blocks, s);
-    else launch_tiles_of<DT, D, big.rw, big.kw, big.bn>(a, p.paged, p.blocks, s);
+    if (p.paged) launch_tiles_of<DT, D, true, false>(a, p, s);
+    else if (a.mask) launch_tiles_of<DT, D, false, true>(a, p, s);
+    else launch_tiles_of<DT, D, false, false>(a, p, s);
 }
 template <int DT> void launch_attention(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
     if (!p.d) {
@@ -649,10 +938,9 @@ template <int DT> void launch_attention(const AttnArgs& a, const AttnPlan& p, hi
     else if (p.d == 128) launch_tiles_d<DT, 128>(a, p, s);
     else launch_tiles_d<DT, 256>(a, p, s);
     if (a.nsplit > 1) {
-        const int quads = a.Dv / 4;
-        const unsigned grid = grid_for((size_t)a.rows * quads, 256, 1u << 20);
-        if (p.paged) hipLaunchKernelGGL((k_attn_join<DT, true>), dim3(grid), dim3(256), 0, s, a, quads);
-        else hipLaunchKernelGGL((k_attn_join<DT, false>), dim3(grid), dim3(256), 0, s, a, quads);
+        const unsigned grid = grid_for((size_t)a.rows, 4, 1u << 20);
+        if (p.paged) hipLaunchKernelGGL((k_attn_join<DT, true>), dim3(grid), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_attn_join<DT, false>), dim3(grid), dim3(256), 0, s, a);
     }
 }
 
