@@ -120,10 +120,6 @@ class DeviceScope {
     bool moved_ = false;
 };
 
-// Keys per tile of the prompts' kernel by the bytes of a padded row of K: two tiles of K and
-// of V in LDS (64 KB up to 512 bytes: two blocks per CU).
-constexpr int attn_tile_keys(int row_bytes) { return row_bytes <= 256 ? 64 : 32; }
-
 constexpr int kMaxSplits = 128;    // of the keys, joined by one wave per row
 
 struct AttnPlan {

@@ -37,10 +37,19 @@ void run_attention(AttnArgs& a, int dt, bool paged, int64_t kv, const Tensor* ws
         p.d = dm <= 64 ? 64 : dm <= 128 ? 128 : 256;
         const int64_t mean = paged ? ((int64_t)a.T * a.G + a.B - 1) / a.B : per * a.G;      // rows of a sequence
         p.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 128;
-        const int64_t tiles = paged ? (int64_t)a.T * a.G / p.rows + a.B : (per * a.G + p.rows - 1) / p.rows;
-        const int64_t units = tiles * (paged ? 1 : a.B) * a.Hkv;
-        const int bn = p.rows == 128 ? attn_tile_keys(p.d * es) : 32;
-        const int lds = 4 * bn * p.d * es, resident = num_cus() * std::min(160 * 1024 / lds, p.rows == 128 ? 2 : 8);
+        auto units_of = [&](int rows) {
+            const int64_t t = paged ? (int64_t)a.T * a.G / rows + a.B : (per * a.G + rows - 1) / rows;
+            return t * (paged ? 1 : a.B) * a.Hkv;
+        };
+        // 256 rows per block where such blocks fill the GPU twice over (one fits a CU): K and V
+        // pass through LDS half as often (1024 blocks of 128 rows over 8192 keys 591 us, 512 of
+        // 256 540; of 64 values per head 120 and 100.  256 blocks over 300 .. 1500 keys: 35.6,
+        // twice as many of 128 rows 33.7).
+        if (p.rows == 128 && p.d * es <= 256 && es == 2 && units_of(256) >= 2 * num_cus()) p.rows = 256;
+        const int64_t units = units_of(p.rows), tiles = units / ((paged ? 1 : a.B) * (int64_t)a.Hkv);
+        const int bn = p.rows == 128 && p.d * es <= 256 ? 64 : 32;
+        const int lds = 4 * bn * p.d * es;
+        const int resident = num_cus() * (p.rows == 256 ? 1 : std::min(160 * 1024 / lds, p.rows == 128 ? 2 : 8));
         // Keys per split.  Few rows: four blocks for every place on the GPU, as lengths differ, and
         // two tiles at least (64 tokens over 130 .. 8192 keys: 219 us with four, 231 with
         // sixteen, 356 with two; one token over 1025: 12.4 us with two tiles, 13.2 with one, 14.0
@@ -48,7 +57,7 @@ void run_attention(AttnArgs& a, int dt, bool paged, int64_t kv, const Tensor* ws
         // GPU (12 sequences of 1 .. 512 tokens, 376 blocks: 59 us with four per place, 78 with
         // one; 1024 blocks of 8192 keys: 553 unsplit, 620 in two).
         int64_t share = std::max<int64_t>({units * kv / ((int64_t)resident * 4), 64, (kv + kMaxSplits - 1) / kMaxSplits});
-        if (p.rows == 128 && units >= resident) share = kv;
+        if (p.rows >= 128 && units >= resident) share = kv;
         share = (share + 31) / 32 * 32;
         int64_t split = kv > share ? (kv + share - 1) / share : 1;
         const int64_t each = a.rows * (a.Dv * 4 + 8);

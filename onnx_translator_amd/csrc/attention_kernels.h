@@ -225,7 +225,7 @@ __device__ __forceinline__ void read_keys8(const uint32_t (&at)[8], uint4 (&v)[8
                  : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]), "v"(at[6]), "v"(at[7]) : "memory");
 }
 // read_turned at four addresses, and STEP bytes further on.
-template <int STEP> __device__ __forceinline__ void read_values4(const uint32_t (&at)[4], uint2 (&x)[4], uint2 (&y)[4]) {
+template <int STEP> __device__ __forceinline__ void read_values(const uint32_t (&at)[4], uint2 (&x)[4], uint2 (&y)[4]) {
     asm volatile("ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %4, %8 offset:%12\n\t"
                  "ds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %5, %9 offset:%12\n\t"
                  "ds_read_b64_tr_b16 %2, %10\n\tds_read_b64_tr_b16 %6, %10 offset:%12\n\t"
@@ -233,6 +233,11 @@ template <int STEP> __device__ __forceinline__ void read_values4(const uint32_t 
                  "s_waitcnt lgkmcnt(0)"
                  : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
                  : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(STEP) : "memory");
+}
+template <int STEP> __device__ __forceinline__ void read_values(const uint32_t (&at)[2], uint2 (&x)[2], uint2 (&y)[2]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %2, %4 offset:%6\n\t"
+                 "ds_read_b64_tr_b16 %1, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(y[0]), "=&v"(y[1]) : "v"(at[0]), "v"(at[1]), "n"(STEP) : "memory");
 }
 // Eight 32-bit values of one column: rows 0 .. 3 and G .. G + 3 of RB bytes each.
 template <int RB, int G> __device__ __forceinline__ void read_column8(uint32_t at, float (&v)[8]) {
@@ -358,8 +363,7 @@ template <bool PAGED, int BM> __device__ __forceinline__ bool attn_block(const A
 }
 
 // ---- a wave's sums ------------------------------------------------------------------------
-// EARLY: LDS fragments are read ahead of a group of products, where no other wave of the SIMD
-// works meanwhile.
+// EARLY: LDS fragments are read ahead of a group of products.
 template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnWave {
     typedef typename AttnAcc<MR>::type Acc;
     static constexpr int ES = kElem<DT>, VEC = 16 / ES, CH = D / VEC, RB = D * ES;
@@ -421,8 +425,8 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
         for (int i = 0; i < NS; i++) asm volatile("" : "+v"(q[i].x), "+v"(q[i].y), "+v"(q[i].z), "+v"(q[i].w));
     }
 
-    // q.k of the 32 keys in rows sub .. of a tile (without a mask unscaled), -inf where not seen.
-    TOHIP_INLINE __device__ void scores(const AttnArgs& a, const char* kt, int sub, int jb, float (&x)[NP]) {
+    // q.k of the 32 keys in rows sub .. of a tile.
+    TOHIP_INLINE __device__ void products(const char* kt, int sub, float (&x)[NP]) {
         Acc s[NP / NR];
 #pragma unroll
         for (int u = 0; u < NP / NR; u++) {
@@ -458,20 +462,47 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
         }
 #pragma unroll
         for (int i = 0; i < NP; i++) x[i] = s[i / NR][i % NR];
+    }
+
+    // Scores of the 32 keys from jb on (without a mask still unscaled), -inf where not seen.
+    TOHIP_INLINE __device__ void close(const AttnArgs& a, int jb, float (&x)[NP]) {
+        const bool inside = jb >= all_lo && jb + 32 <= all_hi;
         if constexpr (MASK) {
+            float bias[NP];
+            if (inside && a.mk) {              // four keys at a time
 #pragma unroll
-            for (int i = 0; i < NP; i++) {
-                const int j = jb + key(i);
-                float bias = -INFINITY;
-                if (j >= lo && j < hi) {
-                    const int64_t at = mo + (int64_t)j * a.mk;
-                    if (a.mask_dt == kU8 || a.mask_dt == kI8) bias = ((const uint8_t*)a.mask)[at] ? 0.0f : -INFINITY;
-                    else if (a.mask_dt == kF32) bias = ((const float*)a.mask)[at];
-                    else bias = ld_f<DT>(a.mask, at);
+                for (int i = 0; i < NP; i += 4) {
+                    const int64_t at = mo + jb + key(i);
+                    if (a.mask_dt == kU8 || a.mask_dt == kI8) {
+                        uint32_t w;
+                        __builtin_memcpy(&w, (const uint8_t*)a.mask + at, 4);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) bias[i + e] = (w >> (8 * e)) & 0xFF ? 0.0f : -INFINITY;
+                    } else if (DT == kF32 || a.mask_dt == kF32) {
+                        __builtin_memcpy(bias + i, (const float*)a.mask + at, 16);
+                    } else {
+                        uint16_t w[4];
+                        __builtin_memcpy(w, (const uint16_t*)a.mask + at, 8);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) bias[i + e] = ld_f<DT>(w, e);
+                    }
                 }
-                x[i] = bias == -INFINITY ? -INFINITY : __builtin_fmaf(x[i], a.scale, bias);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NP; i++) {
+                    const int j = jb + key(i);
+                    bias[i] = -INFINITY;
+                    if (j >= lo && j < hi) {
+                        const int64_t at = mo + (int64_t)j * a.mk;
+                        if (a.mask_dt == kU8 || a.mask_dt == kI8) bias[i] = ((const uint8_t*)a.mask)[at] ? 0.0f : -INFINITY;
+                        else if (a.mask_dt == kF32) bias[i] = ((const float*)a.mask)[at];
+                        else bias[i] = ld_f<DT>(a.mask, at);
+                    }
+                }
             }
-        } else if (jb < all_lo || jb + 32 > all_hi) {
+#pragma unroll
+            for (int i = 0; i < NP; i++) x[i] = bias[i] == -INFINITY ? -INFINITY : __builtin_fmaf(x[i], a.scale, bias[i]);
+        } else if (!inside) {
 #pragma unroll
             for (int i = 0; i < NP; i++) {
                 const int j = jb + key(i);
@@ -480,8 +511,8 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
         }
     }
 
-    // The scores as weights against the running maximum, which grows with them.
-    TOHIP_INLINE __device__ void weigh(float (&x)[NP]) {
+    // The largest of a row's scores.
+    TOHIP_INLINE __device__ float top_of(const float (&x)[NP]) {
         float top = x[0];
 #pragma unroll
         for (int i = 1; i < NP; i++) top = fmaxf(top, x[i]);
@@ -491,17 +522,10 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
             top = fmaxf(ta, tb);
         }
         permlane_pair<32>(top, ta, tb);
-        top = fmaxf(ta, tb);
-        if (__ballot((top - m) * c > kLazy)) {
-            const float mn = fmaxf(m, top);
-            const float f = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
-            l *= f;
-#pragma unroll
-            for (int d = 0; d < NO; d++)
-#pragma unroll
-                for (int i = 0; i < NR; i++) o[d][i] *= f;
-            m = mn;
-        }
+        return fmaxf(ta, tb);
+    }
+    // Scores to weights against the maximum m, and their sum.
+    TOHIP_INLINE __device__ float weights(float (&x)[NP]) {
         const float base = m == -INFINITY ? 0.0f : m;
         if constexpr (MASK) {
             // the difference first: a mask of the type's lowest value times log2 e would overflow
@@ -512,12 +536,47 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
 #pragma unroll
             for (int i = 0; i < NP; i++) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, off));
         }
+        float sum[2] = {x[0], x[1]};
 #pragma unroll
-        for (int i = 0; i < NP; i++) l += x[i];
+        for (int i = 2; i < NP; i++) sum[i & 1] += x[i];
+        return sum[0] + sum[1];
+    }
+    // The sums, which stand against the maximum `was`, against m.
+    TOHIP_INLINE __device__ void rescale(float was) {
+        const float f = m == was ? 1.0f : __builtin_amdgcn_exp2f((was - m) * c);
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < NO; d++)
+#pragma unroll
+            for (int i = 0; i < NR; i++) o[d][i] *= f;
+    }
+    TOHIP_INLINE __device__ void weigh(float (&x)[NP]) {
+        const float top = top_of(x);
+        if (__ballot((top - m) * c > kLazy)) {
+            const float was = m;
+            m = fmaxf(m, top);
+            rescale(was);
+        }
+        l += weights(x);
     }
 
+    // A lane's weights: 16-bit types packed as the product's operand.
+    static constexpr int NPV = DT == kF32 ? NP : 1, NKK = DT == kF32 ? 1 : NP / 8;
+    struct Weights {
+        uint4 h[NKK];
+        float f[NPV];
+    };
+    TOHIP_INLINE __device__ static void pack(const float (&x)[NP], Weights& p) {
+        if constexpr (DT == kF32) {
+#pragma unroll
+            for (int i = 0; i < NP; i++) p.f[i] = x[i];
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < NKK; kk++) p.h[kk] = __builtin_bit_cast(uint4, round16<DT, 8>(x + 8 * kk));
+        }
+    }
     // The weighted values of the 32 keys in rows sub .. of a tile.
-    TOHIP_INLINE __device__ void add(const char* vt, int sub, const float (&p)[NP]) {
+    TOHIP_INLINE __device__ void add(const char* vt, int sub, const Weights& p) {
         if constexpr (DT == kF32) {
 #pragma unroll
             for (int d = 0; d < NO; d++) {
@@ -534,7 +593,7 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
                             vf[i] = *reinterpret_cast<const float*>(at + (4 * GR * ((g + i) >> 2) + (i & 3)) * RB);
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; i++) o[d] = mfma32<MR>(vf[i], p[g + i], o[d]);
+                    for (int i = 0; i < 8; i++) o[d] = mfma32<MR>(vf[i], p.f[g + i], o[d]);
                 }
             }
         } else {
@@ -544,7 +603,7 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
             static_assert(G == 1 || G == 4 || NO == 2, "groups");
 #pragma unroll
             for (int kk = 0; kk < NP / 8; kk++) {
-                const uint4 pf = __builtin_bit_cast(uint4, round16<DT, 8>(p + 8 * kk));
+                const uint4 pf = p.h[kk];
                 const int r = sub + 8 * GR * kk + 4 * h + r4;
 #pragma unroll
                 for (int g = 0; g < NO; g += G) {
@@ -561,7 +620,7 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
                             y[f] = read_turned(v + 4 * GR * RB);
                         }
                     }
-                    if constexpr (G == 4) read_values4<4 * GR * RB>(at, x, y);
+                    if constexpr (G == 4) read_values<4 * GR * RB>(at, x, y);
 #pragma unroll
                     for (int f = 0; f < G; f++) o[g + f] = mfma16<DT, MR>(uint4{x[f].x, x[f].y, y[f].x, y[f].y}, pf, o[g + f]);
                 }
@@ -724,35 +783,24 @@ template <int DT, int D, bool PAGED, int MR, int W> struct AttnLoads {
     }
 };
 
-// Prompts: four waves of 32 rows share tiles of BN keys.  While tile n is worked on, tile n + 1
-// is on its way.
-template <int DT, int D, bool PAGED, bool MASK, int BN>
-__global__ __launch_bounds__(256, D * kElem<DT> <= 256 ? 2 : 1) void k_attn_tiles(AttnArgs a) {
-    typedef AttnWave<DT, D, PAGED, MASK, 32, false> Wave;
-    constexpr int RB = Wave::RB, NI = BN * RB / 4096;
+// Prompts: W waves of 32 rows share tiles of BN keys, two deep: while tile n is worked on, tile
+// n + 1 is on its way.
+template <int DT, int D, bool PAGED, bool MASK, int W, int BN>
+__global__ __launch_bounds__(64 * W, D * kElem<DT> <= 256 ? 2 : 1) void k_attn_tiles(AttnArgs a) {
+    typedef AttnWave<DT, D, PAGED, MASK, 32, (D <= 128)> Wave;      // (as far as registers go)
+    constexpr int RB = Wave::RB, NI = BN * RB / (1024 * W);
     static_assert(NI >= 1, "tile");
-    // distinct arrays: a read of one does not wait for the loads in flight to the other
     __shared__ __attribute__((aligned(1024))) char k0_[BN * RB], k1_[BN * RB], v0_[BN * RB], v1_[BN * RB];
     __shared__ int missing;                    // a key's page was none of the cache's
     const int t = (int)threadIdx.x, wave = uniform(t >> 6);
     AttnBlock k;
-    if (!attn_block<PAGED, 128>(a, 256, k)) return;
+    if (!attn_block<PAGED, 32 * W>(a, 64 * W, k)) return;
     Wave w;
     const AttnRow row = w.begin(a, k, wave * 32);
-    AttnLoads<DT, D, PAGED, 32, 4> ld;
+    AttnLoads<DT, D, PAGED, 32, W> ld;
     ld.begin(a, k, wave);
     if (t == 0) missing = 0;
     __syncthreads();
-    auto work = [&](const char* kt, const char* vt, int j0) TOHIP_INLINE {
-#pragma unroll
-        for (int sub = 0; sub < BN; sub += 32) {
-            if (j0 + sub >= w.any_hi || j0 + sub + 32 <= w.any_lo) continue;
-            float x[Wave::NP];
-            w.scores(a, kt, sub, j0 + sub, x);
-            w.weigh(x);
-            w.add(vt, sub, x);
-        }
-    };
     auto step = [&](int j0, const char* kt, const char* vt, char* kn, char* vn) TOHIP_INLINE {
         wait_loads<0>();
         __builtin_amdgcn_s_barrier();          // every wave's part of this tile is there, and the other buffer is free
@@ -763,7 +811,18 @@ __global__ __launch_bounds__(256, D * kElem<DT> <= 256 ? 2 : 1) void k_attn_tile
             ld.template find<BN>(a, j0 + 2 * BN);
             __builtin_amdgcn_sched_barrier(0);
         }
-        work(kt, vt, j0);
+#pragma unroll
+        for (int sub = 0; sub < BN; sub += 32) {
+            const int jb = j0 + sub;
+            if (jb >= w.any_hi || jb + 32 <= w.any_lo) continue;
+            float x[Wave::NP];
+            typename Wave::Weights p;
+            w.products(kt, sub, x);
+            w.close(a, jb, x);
+            w.weigh(x);
+            Wave::pack(x, p);
+            w.add(vt, sub, p);
+        }
     };
     if (k.klo < k.khi) {
         ld.template find<BN>(a, k.klo);
@@ -804,15 +863,18 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D * kElem<DT
         if (next) wait_loads<3 * NI>();
         else wait_loads<NI>();
         __builtin_amdgcn_sched_barrier(0);
-        w.scores(a, kt, 0, j0, x);
+        w.products(kt, 0, x);
         if (third) ld.template load<false, NI>(a, kt, j0 + 64);
         __builtin_amdgcn_sched_barrier(0);
+        w.close(a, j0, x);
         w.weigh(x);
         if (third) wait_loads<3 * NI>();
         else if (next) wait_loads<2 * NI>();
         else wait_loads<0>();
         __builtin_amdgcn_sched_barrier(0);
-        w.add(vt, 0, x);
+        typename Wave::Weights p;
+        Wave::pack(x, p);
+        w.add(vt, 0, p);
         if (third) {
             ld.template load<true, NI>(a, vt, j0 + 64);
             ld.template find<32>(a, j0 + 96);
@@ -917,10 +979,10 @@ template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_join
 // ---- launches -------------------------------------------------------------------------
 // How a call is cut into blocks is worked out on the host (attention.hip), from sizes alone.
 template <int DT, int D, bool PAGED, bool MASK> void launch_tiles_of(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
-    constexpr int BN = attn_tile_keys(D * kElem<DT>);
     if (p.rows == 16) hipLaunchKernelGGL((k_attn_few<DT, D, PAGED, MASK, 16>), dim3(p.blocks), dim3(64), 0, s, a);
     else if (p.rows == 32) hipLaunchKernelGGL((k_attn_few<DT, D, PAGED, MASK, 32>), dim3(p.blocks), dim3(64), 0, s, a);
-    else hipLaunchKernelGGL((k_attn_tiles<DT, D, PAGED, MASK, BN>), dim3(p.blocks), dim3(256), 0, s, a);
+    else if (p.rows == 128) hipLaunchKernelGGL((k_attn_tiles<DT, D, PAGED, MASK, 4, D * kElem<DT> <= 256 ? 64 : 32>), dim3(p.blocks), dim3(256), 0, s, a);
+    else if constexpr (D * kElem<DT> <= 256) hipLaunchKernelGGL((k_attn_tiles<DT, D, PAGED, MASK, 8, 128>), dim3(p.blocks), dim3(512), 0, s, a);
 }
 template <int DT, int D> void launch_tiles_d(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
     if (p.paged) launch_tiles_of<DT, D, true, false>(a, p, s);
