@@ -52,20 +52,26 @@ struct AttnSeq {
     int64_t tok0;                  // paged: its first row of Q
 };
 
-template <bool PAGED> __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int b) {
+// Sequence b of a paged call, from its first row of Q and the next one's.  Starts and lengths
+// come from the device: whatever they hold, no token outside Q and no key outside the table's
+// capacity is touched.
+__device__ __forceinline__ AttnSeq attn_seq_at(const AttnArgs& a, int b, int64_t t0, int64_t t1) {
+    const int64_t c0 = t0 < 0 ? 0 : t0 > a.T ? a.T : t0, c1 = t1 < c0 ? c0 : t1 > a.T ? a.T : t1;
+    const int64_t cap = (int64_t)a.max_pages * a.ps, l = a.len[b];
     AttnSeq s;
     s.b = b;
+    s.tok0 = c0;
+    s.n = (int)(c1 - c0);
+    s.len = (int)(l < 0 ? 0 : l > cap ? cap : l);
+    s.first = s.len - s.n;
+    return s;
+}
+template <bool PAGED> __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int b) {
     if constexpr (PAGED) {
-        // Starts and lengths come from the device: whatever they hold, no token outside
-        // Q and no key outside the table's capacity is touched.
-        const int64_t t0 = a.qstart[b], t1 = a.qstart[b + 1];
-        const int64_t c0 = t0 < 0 ? 0 : t0 > a.T ? a.T : t0, c1 = t1 < c0 ? c0 : t1 > a.T ? a.T : t1;
-        const int64_t cap = (int64_t)a.max_pages * a.ps, l = a.len[b];
-        s.tok0 = c0;
-        s.n = (int)(c1 - c0);
-        s.len = (int)(l < 0 ? 0 : l > cap ? cap : l);
-        s.first = s.len - s.n;
+        return attn_seq_at(a, b, a.qstart[b], a.qstart[b + 1]);
     } else {
+        AttnSeq s;
+        s.b = b;
         s.tok0 = 0;
         s.n = a.Sq;
         s.len = a.Skv;
@@ -74,8 +80,8 @@ template <bool PAGED> __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs
             s.len = (int)(l < 0 ? 0 : l > a.Skv ? a.Skv : l);
         }
         s.first = 0;
+        return s;
     }
-    return s;
 }
 
 // Keys [lo, hi) that token i of a sequence sees before any mask tensor.

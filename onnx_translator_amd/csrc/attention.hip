@@ -50,13 +50,15 @@ void run_attention(AttnArgs& a, int dt, bool paged, int64_t kv, const Tensor* ws
         const int bn = p.rows == 128 && p.d * es <= 256 ? 64 : 32;
         const int lds = 4 * bn * p.d * es;
         const int resident = num_cus() * (p.rows == 256 ? 1 : std::min(160 * 1024 / lds, p.rows == 128 ? 2 : 8));
-        // Keys per split.  Few rows: four blocks for every place on the GPU, as lengths differ, and
-        // two tiles at least (64 tokens over 130 .. 8192 keys: 219 us with four, 231 with
-        // sixteen, 356 with two; one token over 1025: 12.4 us with two tiles, 13.2 with one, 14.0
-        // with four, 18.2 with eight).  Prompts are split only where their blocks do not fill the
-        // GPU (12 sequences of 1 .. 512 tokens, 376 blocks: 59 us with four per place, 78 with
-        // one; 1024 blocks of 8192 keys: 553 unsplit, 620 in two).
-        int64_t share = std::max<int64_t>({units * kv / ((int64_t)resident * 4), 64, (kv + kMaxSplits - 1) / kMaxSplits});
+        // Keys per split: four blocks for every place on the GPU, as lengths differ, and two tiles
+        // at least (64 tokens over 130 .. 8192 keys: 219 us with four, 231 with sixteen, 356 with
+        // two; one token over 1025: 12.4 us with two tiles, 13.2 with one, 14.0 with four, 18.2
+        // with eight; 96 blocks of 577 f32 keys: 39 with 128 keys, 45 with 64, 57 with 256).
+        // Prompts are split only where their blocks do not fill the GPU (12 sequences of 1 .. 512
+        // tokens, 376 blocks: 59 us with four per place, 78 with one; 1024 blocks of 8192 keys:
+        // 553 unsplit, 620 in two).
+        int64_t share = std::max<int64_t>({units * kv / ((int64_t)resident * 4), p.rows >= 128 ? 128 : 64,
+                                           (kv + kMaxSplits - 1) / kMaxSplits});
         if (p.rows >= 128 && units >= resident) share = kv;
         share = (share + 31) / 32 * 32;
         int64_t split = kv > share ? (kv + share - 1) / share : 1;

@@ -283,9 +283,16 @@ template <int BM> __device__ __forceinline__ int64_t slot_base(const AttnArgs& a
     t0 = t0 < 0 ? 0 : t0 > a.T ? a.T : t0;
     return t0 * a.G / BM + b;
 }
-template <int BM> __device__ __forceinline__ int slot_sequence(const AttnArgs& a, int64_t t) {
+template <int BM> __device__ __forceinline__ AttnSeq slot_sequence(const AttnArgs& a, int64_t t) {
     int lo = 0, n = a.B;                       // the answer is in [lo, lo + n)
     const int lane = (int)(threadIdx.x & 63);
+    if (n < 64) {                              // all starts in one load
+        const int64_t v = a.qstart[min(lane, n)];
+        const int start = (int)(v < 0 ? 0 : v > a.T ? a.T : v);
+        const bool le = lane < n && (int64_t)start * a.G / BM + lane <= t;
+        const int b = max(0, (int)__popcll(__ballot(le)) - 1);
+        return attn_seq_at(a, b, __builtin_amdgcn_readlane(start, b), __builtin_amdgcn_readlane(start, b + 1));
+    }
     while (n > 1) {
         const int step = (n + 63) / 64, b = lo + lane * step;
         const bool le = lane * step < n && slot_base<BM>(a, b) <= t;
@@ -293,7 +300,7 @@ template <int BM> __device__ __forceinline__ int slot_sequence(const AttnArgs& a
         if (k > 1) lo += (k - 1) * step;
         n = min(step, a.B - lo);
     }
-    return uniform(lo);
+    return attn_seq<true>(a, uniform(lo));
 }
 
 // A block's part of the call: `rows` rows from row0 of its sequence on (of key head hk), over
@@ -301,6 +308,7 @@ template <int BM> __device__ __forceinline__ int slot_sequence(const AttnArgs& a
 struct AttnBlock {
     AttnSeq s;
     int hk, split, row0, rows, klo, khi;
+    int table, from;                           // pages from .. from + 63 of the sequence, one per lane
 };
 // One of its rows.
 struct AttnRow {
@@ -325,20 +333,29 @@ template <bool PAGED, int BM> __device__ __forceinline__ bool attn_block(const A
     bid /= (uint32_t)a.Hkv;
     k.split = (int)(bid % (uint32_t)a.nsplit);
     bid /= (uint32_t)a.nsplit;
-    int b, tile;
+    int tile;
     if constexpr (PAGED) {
         // the last slots first: the later tokens of a prompt have the most keys
         const int64_t slot = (int64_t)a.tiles - 1 - bid;
-        b = slot_sequence<BM>(a, slot);
-        const int64_t tl = slot - slot_base<BM>(a, b);
+        k.s = slot_sequence<BM>(a, slot);
+        const int64_t tl = slot - (k.s.tok0 * a.G / BM + k.s.b);
+        // without a window the first page follows from the split alone: its number is on its way
+        // together with the length
+        k.from = -64;
+        k.table = -1;
+        if (!a.window && a.max_pages > 0) {
+            const int64_t j = a.nsplit > 1 ? (int64_t)k.split * a.share : 0;
+            k.from = min((int)a.fd_ps.div((uint32_t)min(j, (int64_t)0x7FFFFFFF)), a.max_pages - 1);
+            const int64_t p = a.pages[(int64_t)k.s.b * a.max_pages + min(k.from + (int)(threadIdx.x & 63), a.max_pages - 1)];
+            k.table = p >= 0 && p < a.npages ? (int)p : -1;
+        }
         tile = uniform(tl < 0 || tl > 0x7FFFFFFF / BM ? -1 : (int)tl);
         if (tile < 0) return false;
     } else {
         const uint32_t tl = bid % (uint32_t)a.tiles;
         tile = a.tiles - 1 - (int)tl;
-        b = (int)(bid / (uint32_t)a.tiles);
+        k.s = attn_seq<PAGED>(a, (int)(bid / (uint32_t)a.tiles));
     }
-    k.s = attn_seq<PAGED>(a, b);
     k.s.n = uniform(k.s.n);
     k.s.len = uniform(k.s.len);
     k.s.first = uniform(k.s.first);
@@ -672,13 +689,11 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
         for (; rows; rows &= rows - 1) {
             const AttnRow x = attn_row_at<PAGED>(a, k, r0 + __builtin_ctzll(rows));
             float rm = -INFINITY, rl = 0.0f;
-            if (parts) {
-                float* po = a.part_o + ((int64_t)k.split * a.rows + x.out) * a.Dv;
-                attn_row<DT, PAGED>(a, k.s, x.head, x.tok, k.klo, k.khi, rm, rl, [&](int d, float v) { po[d] = v; });
-                if ((threadIdx.x & 63) == 0) a.part_ml[(int64_t)k.split * a.rows + x.out] = make_float2(rm * kLog2e, rl);
-            } else {
-                attn_row<DT, PAGED>(a, k.s, x.head, x.tok, k.klo, k.khi, rm, rl, [&](int d, float v) { st_code<DT>(a.y, x.y + d, v); });
-            }
+            attn_row<DT, PAGED>(a, k.s, x.head, x.tok, k.klo, k.khi, rm, rl, [&](int d, float v) {
+                if (parts) a.part_o[((int64_t)k.split * a.rows + x.out) * a.Dv + d] = v;
+                else st_code<DT>(a.y, x.y + d, v);
+            });
+            if (parts && (threadIdx.x & 63) == 0) a.part_ml[(int64_t)k.split * a.rows + x.out] = make_float2(rm * kLog2e, rl);
         }
     }
 };
@@ -719,8 +734,8 @@ template <int DT, int D, bool PAGED, int MR, int W> struct AttnLoads {
         even = !PAGED || (a.ps & (RPI - 1)) == 0;
         worst = 0;
         koff = voff = 0;
-        table = -1;
-        from = -64;                            // nothing in it yet
+        table = PAGED ? k.table : -1;
+        from = PAGED ? k.from : -64;           // (-64: nothing in it yet)
     }
     TOHIP_INLINE __device__ int entry(const AttnArgs& a, int j) const { return __shfl(table, (int)a.fd_ps.div((uint32_t)j) - from); }
     // Looks up the pages of the tile of KEYS keys at j0, and where its instructions' rows begin.
@@ -767,7 +782,7 @@ template <int DT, int D, bool PAGED, int MR, int W> struct AttnLoads {
                 load_lds16(first(i) + ((uint32_t)(min(lrow, last - j) * step) + chunk(r0 + lrow)), to + (i * W + wave) * 1024);
             }
         } else {
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < NI; i++) {
                 const int r = (i * W + wave) * RPI + lrow, j = min(j0 + r, last);
                 int pg = 0;
@@ -786,7 +801,7 @@ template <int DT, int D, bool PAGED, int MR, int W> struct AttnLoads {
 // Prompts: W waves of 32 rows share tiles of BN keys, two deep: while tile n is worked on, tile
 // n + 1 is on its way.
 template <int DT, int D, bool PAGED, bool MASK, int W, int BN>
-__global__ __launch_bounds__(64 * W, D * kElem<DT> <= 256 ? 2 : 1) void k_attn_tiles(AttnArgs a) {
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D * kElem<DT> <= 128 && W == 4 && !MASK ? 3 : D * kElem<DT> <= 256 ? 2 : 1))) void k_attn_tiles(AttnArgs a) {
     typedef AttnWave<DT, D, PAGED, MASK, 32, (D <= 128)> Wave;      // (as far as registers go)
     constexpr int RB = Wave::RB, NI = BN * RB / (1024 * W);
     static_assert(NI >= 1, "tile");
@@ -911,11 +926,12 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D * kElem<DT
 // ---- the splits of a row together -----------------------------------------------------
 // y = sum_s w_s o_s, w_s = l_s 2^(m_s - max) / sum: a wave per row.  Lanes hold the splits'
 // weights, two each; then groups of Dv / 4 lanes add every group's share of the splits, four
-// columns per lane, with four splits' loads in flight (one split after the other, by a thread
-// per four columns, took 38 us for 47 splits of 16 rows).
+// columns per lane, kJoin splits at a time (one split after the other, by a thread per four
+// columns, took 38 us for 47 splits of 16 rows).
+constexpr int kJoin = 4;
 template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     const int lane = (int)threadIdx.x & 63, quads = a.Dv / 4, groups = 64 / quads;
-    const int grp = lane / quads, col = (lane - grp * quads) * 4;
+    const int grp = lane / quads, col = (lane - grp * quads) * 4;      // (lanes past the last group repeat the last split)
     const int64_t step = (int64_t)gridDim.x * 4;
     for (int64_t row = (int64_t)blockIdx.x * 4 + uniform((int)(threadIdx.x >> 6)); row < a.rows; row += step) {
         const int64_t token = row / a.Hq;
@@ -931,6 +947,18 @@ template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_join
         const float2 none = make_float2(-INFINITY, 0.0f);
         const float2 ml0 = lane < a.nsplit ? a.part_ml[lane * a.rows + row] : none;
         const float2 ml1 = lane + 64 < a.nsplit ? a.part_ml[(lane + 64) * a.rows + row] : none;
+        float4 v[kJoin];
+        auto read = [&](int s0) TOHIP_INLINE {
+#pragma unroll
+            for (int i = 0; i < kJoin; i++) {
+                const int s = min(s0 + i * groups + grp, a.nsplit - 1);
+                v[i] = *reinterpret_cast<const float4*>(a.part_o + (s * a.rows + row) * a.Dv + col);
+            }
+        };
+        // Few rows: on their way while the weights are worked out (9.5 -> 9.0 us for one token
+        // over 1500 keys).  Many: only what weighs something is read.
+        const bool ahead = a.rows <= 4096;
+        if (ahead) read(0);
         const float m = wave_allreduce(fmaxf(ml0.x, ml1.x), [](float x, float y) { return fmaxf(x, y); });
         auto weight = [&](float2 ml) {         // 0 for a split that saw no key
             return ml.y == 0.0f ? 0.0f : ml.y * (ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m));
@@ -940,26 +968,23 @@ template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_join
         // divided before the sum, which then cannot leave the range of its terms
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         float r[4] = {};
-        for (int s0 = 0; s0 < a.nsplit; s0 += 4 * groups) {
-            float w[4];
-            float4 v[4];
+        for (int s0 = 0; s0 < a.nsplit; s0 += kJoin * groups) {
+            if (ahead && s0) read(s0);
+            float f[kJoin];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < kJoin; i++) {
                 const int s = s0 + i * groups + grp;
-                w[i] = (s < 64 ? __shfl(w0, s & 63) : 0.0f) + (s >= 64 ? __shfl(w1, s & 63) : 0.0f);
-                if (s >= a.nsplit || grp >= groups) w[i] = 0.0f;
-                // a split that weighs nothing is not read: it may have stored nothing
-                v[i] = make_float4(0, 0, 0, 0);
-                if (w[i] != 0.0f) v[i] = *reinterpret_cast<const float4*>(a.part_o + (s * a.rows + row) * a.Dv + col);
+                const float wa = __shfl(w0, s & 63), wb = __shfl(w1, s & 63);
+                f[i] = s < a.nsplit && grp < groups ? (s < 64 ? wa : wb) * inv : 0.0f;
+                if (!ahead && f[i] != 0.0f) v[i] = *reinterpret_cast<const float4*>(a.part_o + (s * a.rows + row) * a.Dv + col);
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float f = w[i] * inv;
-                if (f == 0.0f) continue;
-                r[0] = __builtin_fmaf(f, v[i].x, r[0]);
-                r[1] = __builtin_fmaf(f, v[i].y, r[1]);
-                r[2] = __builtin_fmaf(f, v[i].z, r[2]);
-                r[3] = __builtin_fmaf(f, v[i].w, r[3]);
+            for (int i = 0; i < kJoin; i++) {
+                if (f[i] == 0.0f) continue;    // weighs nothing: it may have stored nothing
+                r[0] = __builtin_fmaf(f[i], v[i].x, r[0]);
+                r[1] = __builtin_fmaf(f[i], v[i].y, r[1]);
+                r[2] = __builtin_fmaf(f[i], v[i].z, r[2]);
+                r[3] = __builtin_fmaf(f[i], v[i].w, r[3]);
             }
         }
         for (int g = 1; g < groups; g++) {     // the groups' parts, in order
@@ -970,8 +995,8 @@ template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_join
             }
         }
         if (grp == 0) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) st_code<DT>(a.y, yo + col + e, r[e]);
+            if constexpr (DT == kF32) *reinterpret_cast<float4*>((float*)a.y + yo + col) = make_float4(r[0], r[1], r[2], r[3]);
+            else *reinterpret_cast<uint2*>((uint16_t*)a.y + yo + col) = __builtin_bit_cast(uint2, round16<DT, 4>(r));
         }
     }
 }
