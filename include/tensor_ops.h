@@ -360,12 +360,16 @@ void qconv_block_forward(const Tensor* X, const QConvBlock* block, Tensor* Y, Co
  * scores, softmax statistics and sums in float32 or more, one rounding at the end.
  * The Gemm / Conv precision mode (tensor_ops_hip_set_exact) does not apply.  A key
  * that a query does not see adds nothing, whatever K and V hold there, and a row
- * that sees no key gives zeros.
+ * that sees no key (or whose scores are all -inf) gives zeros.  Outputs overlap no
+ * input.
  *
- * Workspace (may be NULL): device memory of any type for the partial results of
- * calls that spread few rows over the GPU along the keys.  Without one an eager
- * call takes such memory from the library's pool, and a call captured into a
- * graph runs in one pass over the keys.  Calls that may overlap (two streams, two graphs) must not share one.
+ * Workspace (may be NULL): device memory of any type, 16-byte aligned, for the
+ * partial results of calls that spread few rows over the GPU along the keys: per
+ * split (at most 128) 4 * Dv + 8 bytes for every query head of every token.  Without
+ * one an eager call takes such memory from the library's pool, and a call captured
+ * into a graph runs in one pass over the keys, which is slower where rows are few;
+ * a smaller one serves for fewer splits.  Calls that may overlap (on two streams, in
+ * two graphs that are replayed at once) must not share one.
  * ------------------------------------------------------------------------- */
 typedef struct {
     int q_heads;     /* 3-D tensors: the query heads; 4-D: 0, or the same as the shape's */

@@ -111,6 +111,13 @@ template <bool PAGED> __device__ __forceinline__ KeyRow attn_key_row(const AttnA
     }
 }
 
+// Whether two tensors' memory overlaps.
+inline bool overlaps(const Tensor* a, const Tensor* b) {
+    if (!a || !b || !a->size || !b->size) return false;
+    const char *x = (const char*)a->data, *y = (const char*)b->data;
+    return x < y + tensor_bytes(b) && y < x + tensor_bytes(a);
+}
+
 // Device of the caller for the length of a call: launches go to the library's device.
 class DeviceScope {
   public:

@@ -20,6 +20,8 @@ bool good_scale(float s, const char* name) {
     return false;
 }
 
+constexpr int64_t kMaxKeys = 0x7FFFFFFF - 4096;      // key numbers past the last tile stay in 31 bits
+
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Cuts the call into blocks and launches it.  kv: the most keys that a row may see, as far
@@ -32,7 +34,8 @@ void run_attention(AttnArgs& a, int dt, bool paged, int64_t kv, const Tensor* ws
     AttnPlan p = {paged, 0, 0, 0};
     void* part = nullptr;
     const int64_t per = paged ? (int64_t)a.T : (int64_t)a.Sq;      // tokens of a sequence at most
-    if (dm <= 256 && a.Dk % vec == 0 && a.Dv % vec == 0 && per * a.G < 0x7FFFFF00 && aligned(a.q) && aligned(a.k) &&
+    if (dm <= 256 && a.Dk % vec == 0 && a.Dv % vec == 0 && per * a.G < 0x7FFFFF00 && a.kt * es < (1 << 26) &&
+        a.vt * es < (1 << 26) && aligned(a.q) && aligned(a.k) &&
         aligned(a.v) && aligned(a.y)) {
         p.d = dm <= 64 ? 64 : dm <= 128 ? 128 : 256;
         const int64_t mean = paged ? ((int64_t)a.T * a.G + a.B - 1) / a.B : per * a.G;      // rows of a sequence
@@ -79,7 +82,8 @@ void run_attention(AttnArgs& a, int dt, bool paged, int64_t kv, const Tensor* ws
             a.part_ml = (float2*)(a.part_o + split * a.rows * a.Dv);
         }
         const int64_t blocks = units * a.nsplit;
-        if (tiles > 0x7FFFFFFF || blocks >= (int64_t(1) << 24)) {
+        const int threads = p.rows >= 128 ? 2 * p.rows : 64;
+        if (tiles > 0x7FFFFFFF || blocks * threads >= (int64_t(1) << 32)) {
             p.d = 0;                                   // past the runtime's work-items per launch
             a.nsplit = 1;
         }
@@ -152,6 +156,11 @@ void attention_forward(const Tensor* Q, const Tensor* K, const Tensor* V, const 
     if (Y->shape[0] != a.B || (packed ? Y->shape[1] != a.Sq || Y->shape[2] != a.Hq * a.Dv
                                       : Y->shape[1] != a.Hq || Y->shape[2] != a.Sq || Y->shape[3] != a.Dv)) {
         set_error("%s: Y must have Q's shape with V's head size", name);
+        return;
+    }
+    if (a.Skv > kMaxKeys) { set_error("%s: K holds 2^31 keys or more per head", name); return; }
+    if (overlaps(Y, Q) || overlaps(Y, K) || overlaps(Y, V) || overlaps(Y, Mask)) {
+        set_error("%s: Y overlaps an input", name);
         return;
     }
     if (!good_scale(params->scale, name)) return;
@@ -266,8 +275,12 @@ void cache_attention_forward(const Tensor* Q, const Tensor* KCache, const Tensor
     if (params->window < 0 || params->max_kv < 0) { set_error("%s: window and max_kv must not be negative", name); return; }
     a.B = Pages->shape[0];
     a.max_pages = Pages->shape[1];
-    if ((int64_t)a.max_pages * a.ps > 0x7FFFFFFF - 4096) {
+    if ((int64_t)a.max_pages * a.ps > kMaxKeys) {
         set_error("%s: Pages hold 2^31 keys or more per sequence", name);
+        return;
+    }
+    if (overlaps(Y, Q) || overlaps(Y, KCache) || overlaps(Y, VCache)) {
+        set_error("%s: Y overlaps an input", name);
         return;
     }
     if (Workspace && (!tensor_sane(Workspace, name) || (Workspace->size && !is_dev(classify(Workspace->data))))) {

@@ -656,7 +656,8 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
         l = la + lb;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const bool parts = a.nsplit > 1;
-        bool bad = again;
+        // (no weight although a key was seen: the scores are past what float32 holds in log2 units)
+        bool bad = again || (l == 0.0f && m > -INFINITY);
 #pragma unroll
         for (int d = 0; d < NO; d++) {
 #pragma unroll

@@ -382,6 +382,10 @@ extern "C" void qk_norm_rotary_forward(const Tensor* QKV, const Tensor* QWeight,
         set_error("%s: epsilon must not be negative, got %g", name, (double)params->epsilon);
         return;
     }
+    if (overlaps(QKV, Q) || overlaps(QKV, K) || overlaps(QKV, V) || overlaps(Q, K) || overlaps(Q, V) || overlaps(K, V)) {
+        set_error("%s: QKV, Q, K and V must not overlap", name);
+        return;
+    }
     if (!ensure_device()) return;
     if (!QKV->size) return;
     a.epsilon = params->epsilon;

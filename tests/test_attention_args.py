@@ -214,3 +214,121 @@ def test_onnx_attention_node():
                              (["q", "k", "v"], {}, ["y", "present"]), (["q", "k", "v", "", "", "", "n"], {"is_causal": 1}, ["y"])):
         with pytest.raises(NotImplementedError):
             make_op(_node(ins, attrs, outs), {}, {})
+
+
+# ------------------------------------------------------------------ dispatch -----
+def names(result):
+    launches, err = result
+    assert not err, err
+    return [l.kernel.split("<")[0] for l in launches]
+
+
+def variant(result):
+    """Rows of a block of the tile kernel that a call launches."""
+    k = result[0][0].kernel
+    assert not result[1]
+    args = k[k.index("<") + 1:k.rindex(">")].replace(" ", "").split(",")
+    return int(args[4]) if k.startswith("k_attn_few") else 32 * int(args[4]) if k.startswith("k_attn_tiles") else 0
+
+
+@pytest.mark.parametrize("q,k,dt,rows", [
+    ((1, 8, 1, 64), (1, 2, 500, 64), O.F16, 16), ((1, 8, 4, 128), (1, 2, 500, 128), O.BF16, 16), ((1, 8, 5, 64), (1, 2, 500, 64), O.F32, 32),
+    ((1, 8, 8, 64), (1, 2, 500, 64), O.F16, 32), ((1, 8, 9, 64), (1, 2, 500, 64), O.F16, 128), ((64, 8, 64, 64), (64, 8, 500, 64), O.F16, 256),
+    ((64, 8, 64, 64), (64, 8, 500, 64), O.F32, 128), ((64, 8, 64, 256), (64, 8, 500, 256), O.F16, 128),
+    ((64, 8, 64, 256), (64, 8, 500, 256), O.F32, 128),
+    ((1, 8, 40, 20), (1, 2, 500, 20), O.F16, 0), ((1, 8, 40, 20), (1, 2, 500, 20), O.F32, 128), ((1, 8, 40, 264), (1, 2, 500, 264), O.F16, 0),
+    ((1, 8, 1, 30), (1, 2, 500, 30), O.F32, 0)], ids=lambda v: str(v))
+def test_rows_of_a_block(rec, q, k, dt, rows):
+    r = attn(rec, q=q, k=k, v=k, dt=dt)
+    assert variant(r) == rows and (rows or names(r) == ["k_attn_rows"])
+
+
+def test_keys_split_where_blocks_are_few(rec):
+    few, many = ((1, 8, 1, 64), (1, 8, 1500, 64)), ((512, 8, 64, 64), (512, 8, 1500, 64))
+    assert names(attn(rec, q=few[0], k=few[1], v=few[1])) == ["k_attn_few", "k_attn_join"]
+    assert names(attn(rec, q=many[0], k=many[1], v=many[1])) == ["k_attn_tiles"]
+    short = (1, 8, 64, 64)
+    assert names(attn(rec, q=few[0], k=short, v=short)) == ["k_attn_few"]
+    # neither memory nor a capture: one pass over the keys
+    rec.no_memory(True)
+    try:
+        assert names(attn(rec, q=few[0], k=few[1], v=few[1])) == ["k_attn_few"]
+        assert names(cache(rec, pages=(3, 400))) == ["k_attn_few"]
+    finally:
+        rec.no_memory(False)
+    rec.capturing(True)
+    try:
+        assert names(attn(rec, q=few[0], k=few[1], v=few[1])) == ["k_attn_few"]
+        assert names(cache(rec, pages=(3, 400))) == ["k_attn_few"]
+        assert names(rotary(rec, slots=(5,), k=CACHE, v=CACHE)) == ["k_rotary_chunks"]
+    finally:
+        rec.capturing(False)
+    assert names(cache(rec, pages=(3, 400))) == ["k_attn_few", "k_attn_join"]
+    # what the caller says of the lengths shapes the launch
+    assert names(cache(rec, pages=(3, 400), max_kv=64)) == ["k_attn_few"]
+
+
+def test_a_workspace_splits_under_capture(rec):
+    t = rec.tensor
+    p = Op.CAttentionParams(0, 0, 0.0, 0)
+    rec.capturing(True)
+    try:
+        for size, kernels in ((1 << 20, ["k_attn_few", "k_attn_join"]), (8 * 264 * 2, ["k_attn_few", "k_attn_join"]), (8 * 264 * 2 - 1, ["k_attn_few"])):
+            r = rec.call("attention_forward", t((1, 8, 1, 64), O.F16), t((1, 8, 1500, 64), O.F16), t((1, 8, 1500, 64), O.F16), O.PT(),
+                         O.PT(), t((1, 8, 1, 64), O.F16), ctypes.byref(p), t((size,), O.U8))
+            assert names(r) == kernels, size
+        r = rec.call("attention_forward", t((1, 8, 1, 64), O.F16), t((1, 8, 1500, 64), O.F16), t((1, 8, 1500, 64), O.F16), O.PT(),
+                     O.PT(), t((1, 8, 1, 64), O.F16), ctypes.byref(p), t((1 << 20,), O.U8, offset=8))
+        assert names(r) == ["k_attn_few"]       # not aligned
+    finally:
+        rec.capturing(False)
+
+
+@pytest.mark.parametrize("offset", [2, 8])
+def test_operands_off_their_alignment(rec, offset):
+    t = rec.tensor
+    p = Op.CAttentionParams(0, 0, 0.0, 0)
+    for which in range(4):
+        ops = [t((1, 8, 40, 64), O.F16, offset=offset if i == which else 0) for i in range(4)]
+        assert names(rec.call("attention_forward", *ops[:3], O.PT(), O.PT(), ops[3], ctypes.byref(p), O.PT())) == ["k_attn_rows"]
+
+
+def test_launches_within_the_runtimes_limit(rec):
+    """Blocks past 2^32 work-items: a wave per row instead (the recorder refuses what the runtime would)."""
+    big = (1 << 20, 64, 1, 64)
+    r = attn(rec, q=big, k=big, v=big)
+    assert names(r) == ["k_attn_rows"]
+    assert names(attn(rec, q=(1 << 18, 64, 1, 64), k=(1 << 18, 64, 1, 64), v=(1 << 18, 64, 1, 64))) == ["k_attn_few"]
+    assert names(rotary(rec, x=(1 << 24, 512), pos=(1 << 24,), q=(1 << 24, 4, 64), k=(1 << 24, 2, 64), v=(1 << 24, 2, 64))) == ["k_rotary_chunks"]
+
+
+def test_rotary_kernels(rec):
+    assert names(rotary(rec)) == ["k_rotary_chunks"]
+    assert names(rotary(rec, cos=(100, 12), sin=(100, 12))) == ["k_rotary_any"]           # 24 rotated: no whole chunk pairs
+    assert names(rotary(rec, x=(5, 8 * 20), wq=(20,), wk=(20,), cos=None, sin=None, pos=None, q=(5, 4, 20), k=(5, 2, 20), v=(5, 2, 20))) == ["k_rotary_any"]
+
+
+def test_outputs_overlap_no_input(rec):
+    t = rec.tensor
+    P = O.PT()
+    at = t((2, 2, 5, 64), O.F16)
+    same = rec.lib.tensor_wrap_device(at.contents.data + 64, O._ints((2, 2, 5, 64)), 4, O.F16)
+    other = [t((2, 2, 5, 64), O.F16) for _ in range(2)]
+    p = Op.CAttentionParams(0, 0, 0.0, 0)
+    for ops in ((at, other[0], other[1]), (other[0], at, other[1]), (other[0], other[1], at)):
+        rec.lib.tensor_ops_hip_clear_error()
+        rec.lib.attention_forward(*ops, P, P, same, ctypes.byref(p), P)
+        assert b"overlaps" in rec.lib.tensor_ops_hip_last_error()
+    q, cache_ = t((4, 2, 64), O.F16), t((3, 2, 4, 64), O.F16)
+    rec.lib.cache_attention_forward(q, cache_, cache_, t((1, 3), O.I32), t((2,), O.I32), t((1,), O.I32), q,
+                                    ctypes.byref(Op.CCacheAttentionParams(0.0, 0, 0)), P)
+    assert b"overlaps" in rec.lib.tensor_ops_hip_last_error()
+    x, y, kv = t((4, 6 * 64), O.F16), t((4, 2, 64), O.F16), t((4, 2, 64), O.F16)
+    rec.lib.qk_norm_rotary_forward(x, P, P, P, P, P, P, y, kv, kv, ctypes.byref(Op.CQKNormRotaryParams(2, 2, 0.0, 0)))
+    assert b"must not overlap" in rec.lib.tensor_ops_hip_last_error()
+
+
+def test_too_many_keys(rec):
+    big = (1, 1, (1 << 31) - 100, 8)
+    launches, err = attn(rec, q=(1, 1, 1, 8), k=big, v=big)
+    assert "2^31 keys" in err and not launches

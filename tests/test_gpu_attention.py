@@ -161,6 +161,56 @@ def test_large_scores(hip):
     DenseProblem(1, 2, 1, 33, 200, 64, "bfloat16", std=1000.0, scale=1e-3, seed=12).check(hip)
 
 
+# Enough blocks of 256 rows to fill the GPU twice over.
+@pytest.mark.parametrize("dtype", ("float16", "bfloat16"))
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sq,skv,kw", [(40, 300, {}), (257, 129, dict(causal=True)), (40, 1, {}), (33, 70, dict(lengths=[0, 1, 70, 33, 64, 65, 2, 69])),
+                                       (40, 131, dict(mask=True))], ids=["plain", "causal", "one key", "lengths", "mask"])
+def test_many_blocks(hip, sq, skv, kw, d, dtype):
+    kw = dict(kw)
+    if kw.pop("mask", None):
+        kw["mask"] = np.random.default_rng(1).random((8, 1, sq, skv)) < 0.6
+    DenseProblem(8, 64, 64, sq, skv, d, dtype, seed=sq, **kw).check(hip, heads=[0, 31, 63])
+
+
+@pytest.mark.parametrize("dtype", ("float16", "bfloat16"))
+@pytest.mark.parametrize("page,window", [(16, 0), (3, 0), (64, 40)])
+def test_cache_many_blocks(hip, page, window, dtype):
+    seqs = [(40, 90), (1, 700), (257, 257), (3, 3), (130, 400), (0, 9), (64, 65), (33, 128)]
+    CacheProblem(seqs, 64, 64, 128 if page == 16 else 64, page, dtype, window=window, seed=page, pad_rows=2).check(hip, heads=[0, 40, 63])
+
+
+# More keys than a row has splits of two tiles, and than one register of page numbers.
+@pytest.mark.parametrize("dtype,d", [("float16", 64), ("float32", 64), ("bfloat16", 256), ("float32", 256)])
+def test_very_long_keys(hip, dtype, d):
+    DenseProblem(1, 1, 1, 1, 20011, d, dtype, seed=1).check(hip)
+    CacheProblem([(1, 9001), (1, 5)], 2, 1, d, 4, dtype, seed=2).check(hip)
+    CacheProblem([(40, 5000)], 1, 1, d, 1, dtype, seed=2).check(hip)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_workspace(hip, dtype):
+    """A workspace of any size: too small for a split, for some of them, and for all."""
+    for sq, skv in ((1, 1500), (100, 900)):
+        for size in (1, 5000, 40000, 1 << 24):
+            DenseProblem(1, 4, 2, sq, skv, 64, dtype, seed=3).check(hip, workspace=size)
+    for size in (1, 5000, 1 << 24):
+        CacheProblem([(1, 1500), (3, 700)], 4, 2, 64, 16, dtype, seed=4).check(hip, workspace=size)
+
+
+@pytest.mark.parametrize("dtype", ("bfloat16", "float32"))
+def test_scores_past_log2_units(hip, dtype):
+    """Scores near float32's largest: one key still takes everything."""
+    p = DenseProblem(1, 1, 1, 3, 40, 64, dtype, scale=1.0, seed=5)
+    p.q64[:], p.k64[:] = 0.0, 0.0
+    p.q64[..., 0], p.k64[..., 0] = 1e19, np.linspace(-2.9e19, 2.9e19, 40)
+    import torch
+    from tests.attention_ref import TORCH, check
+    p.q, p.k = torch.from_numpy(p.q64).to(TORCH[dtype]), torch.from_numpy(p.k64).to(TORCH[dtype])
+    got = p.run(hip)
+    check(got, np.broadcast_to(p.v64[:, :, 39:40], got.shape), np.zeros_like(got), dtype)
+
+
 # ------------------------------------------------------------------- cache -------
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", SIZES)
