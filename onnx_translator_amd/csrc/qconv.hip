@@ -654,12 +654,14 @@ __global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(PROJ &
     const int step_end = min(total, kQSteps * s_end);
     // Next stage to load: sst, its first channel step cs (even: a stage is two
     // steps of one tap) and tap (kh, kw); past the group's last stage the last
-    // is loaded again (its copy is never read).  One global load per row on
+    // is loaded again (its copy is never read), also by a second group that
+    // has no stage at all (one stage in total: stage s_beg would begin past the
+    // weight rows, the last row's past the buffer).  One global load per row on
     // every path keeps the compiler's count of loads in flight exact, so its
     // waits stay partial.
-    int sst = s_beg, cs = 0, kh = 0, kw = 0;
-    if (KG > 1 && s_beg > 0) {
-        const int st0 = kQSteps * s_beg;
+    int sst = min(s_beg, nst_all - 1), cs = 0, kh = 0, kw = 0;
+    if (KG > 1 && sst > 0) {
+        const int st0 = kQSteps * sst;
         if (st0 < g.steps) {
             const int tap = st0 / g.csteps;
             cs = st0 - tap * g.csteps;
