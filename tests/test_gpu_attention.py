@@ -231,6 +231,20 @@ def test_cache_windows(hip, window, dtype):
     CacheProblem([(1, 300), (70, 200), (1, 1), (33, 33)], 4, 2, 64, 16, dtype, window=window, seed=window).check(hip)
 
 
+@pytest.mark.parametrize("dtype", ("float16", "float32"))
+@pytest.mark.parametrize("hq", [2, 12, 40])
+@pytest.mark.parametrize("count", [63, 64, 65, 130, 4097])
+def test_cache_many_sequences(hip, count, hq, dtype):
+    """More sequences than one load of starts holds, with some that have no token (the last ones
+    among them), for each kind of block: 2, 12 and 40 rows of a key head per token."""
+    rng = np.random.default_rng(count)
+    new = rng.choice([0, 1, 1, 1, 2, 5], count)
+    new[-2:] = 0
+    seqs = [(int(n), int(n + e)) for n, e in zip(new, rng.integers(0, 12, count))]
+    heads = None if count < 1000 else [0, hq - 1]
+    CacheProblem(seqs, hq, 1, 64, 4, dtype, pad_rows=3, seed=count).check(hip, heads=heads)
+
+
 @pytest.mark.parametrize("index", ["int32", "int64"])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_cache_ragged_batches(hip, dtype, index):
