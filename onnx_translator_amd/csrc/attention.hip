@@ -52,17 +52,20 @@ void run_attention(AttnArgs& a, int dt, bool paged, int64_t kv, const Tensor* ws
         const int64_t units = units_of(p.rows), tiles = units / ((paged ? 1 : a.B) * (int64_t)a.Hkv);
         const int bn = p.rows == 128 && p.d * es <= 256 ? 64 : 32;
         const int lds = 4 * bn * p.d * es;
-        const int resident = num_cus() * (p.rows == 256 ? 1 : std::min(160 * 1024 / lds, p.rows == 128 ? 2 : 8));
+        // blocks on a CU at once (by registers: three of four waves for 64 values of 16 bits)
+        const int most = p.rows == 128 ? (p.d * es <= 128 && !a.mask ? 3 : 2) : 8;
+        const int resident = num_cus() * (p.rows == 256 ? 1 : std::min(160 * 1024 / lds, most));
         // Keys per split: four blocks for every place on the GPU, as lengths differ, and two tiles
         // at least (64 tokens over 130 .. 8192 keys: 219 us with four, 231 with sixteen, 356 with
         // two; one token over 1025: 12.4 us with two tiles, 13.2 with one, 14.0 with four, 18.2
         // with eight; 96 blocks of 577 f32 keys: 39 with 128 keys, 45 with 64, 57 with 256).
-        // Prompts are split only where their blocks do not fill the GPU (12 sequences of 1 .. 512
-        // tokens, 376 blocks: 59 us with four per place, 78 with one; 1024 blocks of 8192 keys:
-        // 553 unsplit, 620 in two).
+        // Prompts are split only where there are fewer blocks than two per CU (12 sequences of
+        // 2 .. 304 tokens, 376 blocks: 54 us with twelve per CU, 56 with eight, 69 with four, 78
+        // unsplit; 512 blocks over 300 .. 1500 keys: 33.7 unsplit, 42 in two; 1024 blocks of
+        // 8192: 553 and 620).
         int64_t share = std::max<int64_t>({units * kv / ((int64_t)resident * 4), p.rows >= 128 ? 128 : 64,
                                            (kv + kMaxSplits - 1) / kMaxSplits});
-        if (p.rows >= 128 && units >= resident) share = kv;
+        if (p.rows >= 128 && units >= std::min(resident, 2 * num_cus())) share = kv;
         share = (share + 31) / 32 * 32;
         int64_t split = kv > share ? (kv + share - 1) / share : 1;
         const int64_t each = a.rows * (a.Dv * 4 + 8);

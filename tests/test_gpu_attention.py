@@ -188,6 +188,16 @@ def test_very_long_keys(hip, dtype, d):
     CacheProblem([(40, 5000)], 1, 1, d, 1, dtype, seed=2).check(hip)
 
 
+# Rows and splits for each join: up to 16, 32 and 64 splits of heads up to 64, 128 and 256, and more.
+@pytest.mark.parametrize("dtype", ("bfloat16", "float32"))
+@pytest.mark.parametrize("d,dv", [(64, 64), (64, 40), (128, 96), (128, 128), (256, 136), (256, 256)])
+@pytest.mark.parametrize("skv", [300, 2500])
+def test_joins_of_many_rows(hip, skv, d, dv, dtype):
+    DenseProblem(1, 16, 16, 300, skv, d, dtype, dv=dv, lengths=[skv - 40], seed=d).check(hip, heads=[0, 15])
+    seqs = [(200, skv), (1, 65), (0, 7), (100, 128)]
+    CacheProblem(seqs, 16, 4, d, 16, dtype, dv=dv, pad_rows=5, seed=dv).check(hip, heads=[0, 15])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_workspace(hip, dtype):
     """A workspace of any size: too small for a split, for some of them, and for all."""
