@@ -360,8 +360,8 @@ void qconv_block_forward(const Tensor* X, const QConvBlock* block, Tensor* Y, Co
  * scores, softmax statistics and sums in float32 or more, one rounding at the end.
  * The Gemm / Conv precision mode (tensor_ops_hip_set_exact) does not apply.  A key
  * that a query does not see adds nothing, whatever K and V hold there, and a row
- * that sees no key (or whose scores are all -inf) gives zeros.  Outputs overlap no
- * input.
+ * that sees no key (or whose scores are all -inf) gives zeros.  Outputs and workspaces
+ * overlap no input and not each other.
  *
  * Workspace (may be NULL): device memory of any type, 16-byte aligned, for the
  * partial results of calls that spread few rows over the GPU along the keys: per

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 namespace tohip {
 namespace {
@@ -23,6 +24,16 @@ bool good_scale(float s, const char* name) {
 constexpr int64_t kMaxKeys = 0x7FFFFFFF - 4096;      // key numbers past the last tile stay in 31 bits
 
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Y and Workspace share no memory with an input or with each other.
+bool apart(std::initializer_list<const Tensor*> inputs, const Tensor* Y, const Tensor* Workspace, const char* name) {
+    for (const Tensor* t : inputs) {
+        if (overlaps(t, Y)) { set_error("%s: Y overlaps an input", name); return false; }
+        if (overlaps(t, Workspace)) { set_error("%s: Workspace overlaps an input", name); return false; }
+    }
+    if (overlaps(Y, Workspace)) { set_error("%s: Workspace overlaps Y", name); return false; }
+    return true;
+}
 
 // Cuts the call into blocks and launches it.  kv: the most keys that a row may see, as far
 // as the host knows.
@@ -162,10 +173,6 @@ void attention_forward(const Tensor* Q, const Tensor* K, const Tensor* V, const 
         return;
     }
     if (a.Skv > kMaxKeys) { set_error("%s: K holds 2^31 keys or more per head", name); return; }
-    if (overlaps(Y, Q) || overlaps(Y, K) || overlaps(Y, V) || overlaps(Y, Mask)) {
-        set_error("%s: Y overlaps an input", name);
-        return;
-    }
     if (!good_scale(params->scale, name)) return;
     a.G = a.Hq / a.Hkv;
     a.fd_g = make_fastdiv((uint32_t)a.G);
@@ -213,6 +220,7 @@ void attention_forward(const Tensor* Q, const Tensor* K, const Tensor* V, const 
         if (!*tensor_ops_hip_last_error()) set_error("%s: Workspace must be a device tensor", name);
         return;
     }
+    if (!apart({Q, K, V, Mask, KVLen}, Y, Workspace, name)) return;
     if (!ensure_device()) return;
     if (!Y->size) return;
     DeviceScope scope;
@@ -282,14 +290,11 @@ void cache_attention_forward(const Tensor* Q, const Tensor* KCache, const Tensor
         set_error("%s: Pages hold 2^31 keys or more per sequence", name);
         return;
     }
-    if (overlaps(Y, Q) || overlaps(Y, KCache) || overlaps(Y, VCache)) {
-        set_error("%s: Y overlaps an input", name);
-        return;
-    }
     if (Workspace && (!tensor_sane(Workspace, name) || (Workspace->size && !is_dev(classify(Workspace->data))))) {
         if (!*tensor_ops_hip_last_error()) set_error("%s: Workspace must be a device tensor", name);
         return;
     }
+    if (!apart({Q, KCache, VCache, Pages, QStart, KVLen}, Y, Workspace, name)) return;
     if (!ensure_device()) return;
     if (!Y->size || !a.B) return;
     a.G = a.Hq / a.Hkv;

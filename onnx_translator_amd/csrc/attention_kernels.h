@@ -32,7 +32,10 @@ __device__ __forceinline__ double lane_value(double v, int lane) {
 // ---- one row per wave ---------------------------------------------------------------
 // Any head size, alignment and content.  Lanes take 64 keys at a time for the scores,
 // then 64 columns of V for the sums, in double: nothing overflows on the way to a
-// finite result, and a key that is not seen is never multiplied.
+// finite result, and a key that is not seen is never multiplied.  Bound by its double
+// products and one dependent pass after the other: what the matrix kernels do in 534 us
+// (4096 queries over 8192 keys, 32 heads of 128) takes it 0.29 s, so it takes what they do
+// not: odd head sizes, unaligned tensors, and single rows that they hand over.
 constexpr int kRowCols = 4;        // columns of V per lane and pass over the keys
 
 // Partial result of the keys [ks, ke) for query head h of token i: the maximum (of
@@ -800,7 +803,14 @@ template <int DT, int D, bool PAGED, int MR, int W> struct AttnLoads {
 };
 
 // Prompts: W waves of 32 rows share tiles of BN keys, two deep: while tile n is worked on, tile
-// n + 1 is on its way.
+// n + 1 is on its way.  S' = K Q' leaves a query's scores in one lane pair, in the order in
+// which O' += V' P' takes its weights, so they never leave the registers; 32 rows per wave are
+// what the products' largest form takes with the sums of 128 columns still in registers.
+// Bound by the matrix and vector units together (32 keys of 32 rows: 512 cycles of products at
+// 128 values per head, about as many for the 16 exponentials per lane and what surrounds them)
+// and, at full length, by power: 4096 queries over 8192 keys, 32 heads of 128 in bf16, 534 us or
+// 1.03 PFLOP/s; the last 4096 of 16384 keys in pages of 16, 980 us.  With 64 values per head the
+// exponentials weigh twice as much.
 template <int DT, int D, bool PAGED, bool MASK, int W, int BN>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D * kElem<DT> <= 128 && W == 4 && !MASK ? 3 : D * kElem<DT> <= 256 ? 2 : 1))) void k_attn_tiles(AttnArgs a) {
     typedef AttnWave<DT, D, PAGED, MASK, 32, (D <= 128)> Wave;      // (as far as registers go)
@@ -859,8 +869,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D * kEle
 
 // Few rows: a block is one wave, so nothing waits for another.  K and V have two buffers of
 // 32 keys each; K's is filled again as soon as its scores are made and V's as soon as it is
-// added, so three of the four are in flight while one is worked on (filled a whole tile at a
-// time, 64 tokens over 8192 keys took 261 us).
+// added, so three of the four are in flight while one is worked on.  Bound by memory: 64
+// tokens of 32 heads over 130 .. 8192 keys of 8 heads of 128 in bf16 take 220 us, 5.0 TB/s
+// (filled a whole tile at a time 261); one token over 1025 keys 12.1 us, of which 4 are the
+// join's launch and the rest a chain of loads: starts, length, pages, keys.
 template <int DT, int D, bool PAGED, bool MASK, int MR>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D * kElem<DT> <= 256 ? 2 : 1))) void k_attn_few(AttnArgs a) {
     typedef AttnWave<DT, D, PAGED, MASK, MR, (MR == 16 || D <= 128)> Wave;      // (as far as registers go)

@@ -328,6 +328,45 @@ def test_outputs_overlap_no_input(rec):
     assert b"must not overlap" in rec.lib.tensor_ops_hip_last_error()
 
 
+def test_indices_tables_and_workspaces_overlap_nothing(rec):
+    t, P = rec.tensor, O.PT()
+
+    def alias(x, shape, dt):
+        return rec.lib.tensor_wrap_device(x.contents.data, O._ints(shape), len(shape), dt)
+
+    def refused(fn, *a):
+        rec.lib.tensor_ops_hip_clear_error()
+        getattr(rec.lib, fn)(*a)
+        return b"overlap" in rec.lib.tensor_ops_hip_last_error()
+    q, k, v, y = (t((2, 2, 5, 64), O.F16) for _ in range(4))
+    p = ctypes.byref(Op.CAttentionParams(0, 0, 0.0, 0))
+    assert refused("attention_forward", q, k, v, P, alias(y, (2,), O.I32), y, p, P)
+    for x in (q, k, v, y):
+        assert refused("attention_forward", q, k, v, P, P, y, p, alias(x, (64,), O.U8))
+    assert not refused("attention_forward", q, k, v, P, P, y, p, t((64,), O.U8))
+    q, kc, vc, y = t((4, 2, 64), O.F16), t((3, 2, 4, 64), O.F16), t((3, 2, 4, 64), O.F16), t((4, 2, 64), O.F16)
+    ix = [t((1, 3), O.I32), t((2,), O.I32), t((1,), O.I32)]
+    p = ctypes.byref(Op.CCacheAttentionParams(0.0, 0, 0))
+    for i, shape in enumerate(((1, 3), (2,), (1,))):
+        on = list(ix)
+        on[i] = alias(y, shape, O.I32)
+        assert refused("cache_attention_forward", q, kc, vc, *on, y, p, P)
+    for x in (q, kc, vc, *ix, y):
+        assert refused("cache_attention_forward", q, kc, vc, *ix, y, p, alias(x, (4,), O.U8))
+    assert not refused("cache_attention_forward", q, kc, vc, *ix, y, p, t((64,), O.U8))
+    x, y, k, v = t((4, 6 * 64), O.F16), t((4, 2, 64), O.F16), t((4, 2, 64), O.F16), t((4, 2, 64), O.F16)
+    w, cos, sin, pos = t((64,), O.F16), t((9, 32), O.F16), t((9, 32), O.F16), t((4,), O.I32)
+    p = ctypes.byref(Op.CQKNormRotaryParams(2, 2, 0.0, 0))
+    assert not refused("qk_norm_rotary_forward", x, w, w, cos, sin, pos, P, y, k, v, p)
+    for out in (y, k, v):
+        for i, (shape, dt) in enumerate((((64,), O.F16), ((64,), O.F16), ((2, 32), O.F16), ((2, 32), O.F16), ((4,), O.I32))):
+            ins = [w, w, cos, sin, pos]
+            ins[i] = alias(out, shape, dt)
+            if i in (2, 3):                    # both tables of one shape
+                ins[5 - i] = t(shape, dt)
+            assert refused("qk_norm_rotary_forward", x, *ins, P, y, k, v, p)
+
+
 def test_too_many_keys(rec):
     big = (1, 1, (1 << 31) - 100, 8)
     launches, err = attn(rec, q=(1, 1, 1, 8), k=big, v=big)
