@@ -90,8 +90,8 @@ __device__ __forceinline__ int attn_hi(const AttnArgs& a, const AttnSeq& s, int 
     return a.causal && p < s.len ? p : s.len;
 }
 __device__ __forceinline__ int attn_lo(const AttnArgs& a, const AttnSeq& s, int i) {
-    const int p = s.first + i + 1 - a.window;
-    return a.window && p > 0 ? p : 0;
+    const int64_t p = (int64_t)s.first + i + 1 - a.window;       // (first may be as low as -n)
+    return a.window && p > 0 ? (int)p : 0;
 }
 
 // The page of key j of sequence b, or -1 where the table names none of the cache's.

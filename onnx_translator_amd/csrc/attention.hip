@@ -302,7 +302,7 @@ void cache_attention_forward(const Tensor* Q, const Tensor* KCache, const Tensor
     a.fd_ps = make_fastdiv((uint32_t)a.ps);
     a.scale = params->scale != 0.0f ? params->scale : (float)(1.0 / std::sqrt((double)a.Dk));
     a.causal = 1;
-    a.window = params->window;
+    a.window = params->window < (int64_t)a.max_pages * a.ps ? params->window : 0;     // (one that long closes nothing)
     a.qh = a.Dk;
     a.qt = (int64_t)a.Hq * a.Dk;
     a.yh = a.Dv;

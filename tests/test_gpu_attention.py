@@ -255,6 +255,17 @@ def test_cache_many_sequences(hip, count, hq, dtype):
     CacheProblem(seqs, hq, 1, 64, 4, dtype, pad_rows=3, seed=count).check(hip, heads=heads)
 
 
+@pytest.mark.parametrize("dtype", ("float16", "float32"))
+@pytest.mark.parametrize("d", [64, 20])
+@pytest.mark.parametrize("window", [95, 96, 97, 2 ** 31 - 1])
+def test_cache_windows_of_all_keys(hip, window, d, dtype):
+    """Windows about as long as what the table can name (96 keys), and the largest, with a length
+    that leaves the first tokens of a sequence without a key."""
+    p = CacheProblem([(90, 96), (40, 3), (1, 96)], 2, 1, d, 16, dtype, window=window, spare_columns=0, seed=7)
+    got = p.check(hip)
+    assert not got[90:127].any()
+
+
 @pytest.mark.parametrize("index", ["int32", "int64"])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_cache_ragged_batches(hip, dtype, index):
