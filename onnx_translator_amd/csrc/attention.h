@@ -133,7 +133,7 @@ class DeviceScope {
     bool moved_ = false;
 };
 
-constexpr int kMaxSplits = 128;    // of the keys, joined by one wave per row
+constexpr int kMaxSplits = 128;    // of the keys: two per lane of a joining wave
 
 struct AttnPlan {
     bool paged;
