@@ -134,11 +134,13 @@ class DeviceScope {
 };
 
 constexpr int kMaxSplits = 128;    // of the keys: two per lane of a joining wave
+constexpr int kTablePages = 64;    // page numbers that a wave holds, one per lane: a tile of keys names no more
+constexpr int kKeys256 = 128;      // keys of a tile under blocks of 256 rows (64 or 32 under the others)
 
 struct AttnPlan {
     bool paged;
     int d;                         // padded head size of the tile kernels; 0: a wave per row
-    int rows;                      // rows of a block: 16 or 32 (one wave), or 128 (four)
+    int rows;                      // rows of a block: 16 or 32 (one wave), 128 (four) or 256 (eight)
     unsigned blocks;
 };
 void launch_attention_f16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);

@@ -58,8 +58,11 @@ void run_attention(AttnArgs& a, int dt, bool paged, int64_t kv, const Tensor* ws
         // 256 rows per block where such blocks fill the GPU twice over (one fits a CU): K and V
         // pass through LDS half as often (1024 blocks of 128 rows over 8192 keys 591 us, 512 of
         // 256 540; of 64 values per head 120 and 100.  256 blocks over 300 .. 1500 keys: 35.6,
-        // twice as many of 128 rows 33.7).
-        if (p.rows == 128 && p.d * es <= 256 && es == 2 && units_of(256) >= 2 * num_cus()) p.rows = 256;
+        // twice as many of 128 rows 33.7).  Not where a tile of their keys may lie on more pages
+        // than a wave holds numbers of (pages of one key; tiles begin at multiples of 32).
+        if (p.rows == 128 && p.d * es <= 256 && es == 2 && (!paged || kKeys256 <= kTablePages * (int64_t)a.ps) &&
+            units_of(256) >= 2 * num_cus())
+            p.rows = 256;
         const int64_t units = units_of(p.rows), tiles = units / ((paged ? 1 : a.B) * (int64_t)a.Hkv);
         const int bn = p.rows == 128 && p.d * es <= 256 ? 64 : 32;
         const int lds = 4 * bn * p.d * es;

@@ -709,7 +709,9 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
 // instruction, the addresses of paged keys took longer than the loads themselves.  Rows past the last key
 // repeat it.  Pages whose size an instruction's rows do not divide are looked up row by row.
 // A wave holds 64 of the sequence's page numbers in a register: looked up in memory for each
-// tile, they were a second trip to it per tile (32 keys of one wave: 1.4 us).
+// tile, they were a second trip to it per tile (32 keys of one wave: 1.4 us).  A tile's pages are
+// all among them: a tile has at most 64 keys, or 128 that begin at an even one where pages have two
+// keys or more (the host sees to it).
 // Columns past the head size repeat the last chunk: Q is zero there, and where the product of
 // a value that is not finite is not either, the row is computed again.
 template <int DT, int D, bool PAGED, int MR, int W> struct AttnLoads {
@@ -744,6 +746,7 @@ template <int DT, int D, bool PAGED, int MR, int W> struct AttnLoads {
     TOHIP_INLINE __device__ int entry(const AttnArgs& a, int j) const { return __shfl(table, (int)a.fd_ps.div((uint32_t)j) - from); }
     // Looks up the pages of the tile of KEYS keys at j0, and where its instructions' rows begin.
     template <int KEYS> TOHIP_INLINE __device__ void find(const AttnArgs& a, int j0) {
+        static_assert(KEYS <= kTablePages || KEYS == kKeys256, "pages of a tile");
         const int end = min(j0 + KEYS - 1, last), j = min(j0 + lane * RPI, end);
         int pg = 0;
         if constexpr (PAGED) {
@@ -1075,7 +1078,7 @@ template <int DT, int D, bool PAGED, bool MASK> void launch_tiles_of(const AttnA
     if (p.rows == 16) hipLaunchKernelGGL((k_attn_few<DT, D, PAGED, MASK, 16>), dim3(p.blocks), dim3(64), 0, s, a);
     else if (p.rows == 32) hipLaunchKernelGGL((k_attn_few<DT, D, PAGED, MASK, 32>), dim3(p.blocks), dim3(64), 0, s, a);
     else if (p.rows == 128) hipLaunchKernelGGL((k_attn_tiles<DT, D, PAGED, MASK, 4, D * kElem<DT> <= 256 ? 64 : 32>), dim3(p.blocks), dim3(256), 0, s, a);
-    else if constexpr (D * kElem<DT> <= 256) hipLaunchKernelGGL((k_attn_tiles<DT, D, PAGED, MASK, 8, 128>), dim3(p.blocks), dim3(512), 0, s, a);
+    else if constexpr (D * kElem<DT> <= 256) hipLaunchKernelGGL((k_attn_tiles<DT, D, PAGED, MASK, 8, kKeys256>), dim3(p.blocks), dim3(512), 0, s, a);
 }
 template <int DT, int D> void launch_tiles_d(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
     if (p.paged) launch_tiles_of<DT, D, true, false>(a, p, s);

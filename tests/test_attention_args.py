@@ -243,6 +243,16 @@ def test_rows_of_a_block(rec, q, k, dt, rows):
     assert variant(r) == rows and (rows or names(r) == ["k_attn_rows"])
 
 
+@pytest.mark.parametrize("dt", [O.F16, O.BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("page,rows", [(1, 128), (2, 256), (3, 256), (16, 256)])
+def test_a_tile_of_keys_names_64_pages_at_most(rec, page, rows, d, dt):
+    """Blocks of 256 rows have tiles of 128 keys, and a wave holds 64 page numbers."""
+    caches = (16384 // page, 8, page, d)
+    r = cache(rec, q=(4096, 32, d), k=caches, v=caches, pages=(1, 16384 // page), start=(2,), length=(1,), dt=dt)
+    assert variant(r) == rows
+
+
 def test_keys_split_where_blocks_are_few(rec):
     few, many = ((1, 8, 1, 64), (1, 8, 1500, 64)), ((512, 8, 64, 64), (512, 8, 1500, 64))
     assert names(attn(rec, q=few[0], k=few[1], v=few[1])) == ["k_attn_few", "k_attn_join"]

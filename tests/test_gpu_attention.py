@@ -180,6 +180,15 @@ def test_cache_many_blocks(hip, page, window, dtype):
     CacheProblem(seqs, 64, 64, 128 if page == 16 else 64, page, dtype, window=window, seed=page, pad_rows=2).check(hip, heads=[0, 40, 63])
 
 
+@pytest.mark.parametrize("dtype", ("float16", "bfloat16"))
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("page,window", [(1, 0), (1, 150), (2, 0)])
+def test_cache_many_blocks_over_tiny_pages(hip, page, window, d, dtype):
+    """A tile of keys on more pages than a wave holds numbers of, or just as many."""
+    seqs = [(40, 90), (1, 700), (257, 257), (3, 3), (130, 400), (0, 9), (64, 65), (33, 128)]
+    CacheProblem(seqs, 64, 64, d, page, dtype, window=window, seed=d, pad_rows=2).check(hip, heads=[0, 40, 63])
+
+
 # More keys than a row has splits of two tiles, and than one register of page numbers.
 @pytest.mark.parametrize("dtype,d", [("float16", 64), ("float32", 64), ("bfloat16", 256), ("float32", 256)])
 def test_very_long_keys(hip, dtype, d):
