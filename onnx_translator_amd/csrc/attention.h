@@ -42,7 +42,7 @@ struct AttnArgs {
     // tiles: rows of tiles per batch (dense) or in all (paged), and the key splits of each
     int tiles, nsplit, share;      // share: keys of a split
     float* part_o;                 // [nsplit][rows][Dv]: normalised results of a split
-    float2* part_ml;               // [nsplit][rows]: (maximum in log2 units, sum)
+    float2* part_ml;               // [nsplit][rows]: (maximum of the scores, sum against it)
     int64_t rows;                  // rows of Y: tokens x query heads
 };
 

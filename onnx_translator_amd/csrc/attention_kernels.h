@@ -276,6 +276,7 @@ template <int DT, int CH, int MR> __device__ __forceinline__ int value_place(int
 // below 2^8 (and the float16 ones, raised by 2^6 out of its subnormal range, below 2^14).
 constexpr float kLazy = 8.0f;
 template <int DT> constexpr float kRaise = DT == kF16 ? 6.0f : 0.0f;
+template <int DT> constexpr float kLower = DT == kF16 ? 0x1p-6f : 1.0f;        // 2^-kRaise
 
 // ---- blocks, rows, keys -----------------------------------------------------------------
 // The sequence whose tiles hold slot t: the last b with floor(start_b * G / BM) + b <= t.
@@ -683,9 +684,10 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
                 }
             }
         }
-        // l is scaled by 2^(kRaise - m c): its exponent, in log2 units
+        // The maximum as a score: times log2 e it would overflow where scores are near float32's
+        // largest, and splits of other maxima would count as equal.  (1 / 2^kRaise is exact.)
         if (parts && live && h == 0)
-            a.part_ml[(int64_t)k.split * a.rows + w.out] = make_float2(m == -INFINITY ? -INFINITY : m * c - kRaise<DT>, l);
+            a.part_ml[(int64_t)k.split * a.rows + w.out] = make_float2(MASK || m == -INFINITY ? m : m * a.scale, l * kLower<DT>);
         unsigned long long rows = __ballot(bad && live);
         rows |= rows >> 32;
         if constexpr (GR == 4) rows |= rows >> 16;
@@ -697,7 +699,7 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
                 if (parts) a.part_o[((int64_t)k.split * a.rows + x.out) * a.Dv + d] = v;
                 else st_code<DT>(a.y, x.y + d, v);
             });
-            if (parts && (threadIdx.x & 63) == 0) a.part_ml[(int64_t)k.split * a.rows + x.out] = make_float2(rm * kLog2e, rl);
+            if (parts && (threadIdx.x & 63) == 0) a.part_ml[(int64_t)k.split * a.rows + x.out] = make_float2(rm, rl);
         }
     }
 };
@@ -940,7 +942,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D * kElem<DT
 }
 
 // ---- the splits of a row together -----------------------------------------------------
-// y = sum_s w_s o_s, w_s = l_s 2^(m_s - max) / sum: a wave per row.  Lanes hold the splits'
+// y = sum_s w_s o_s, w_s = l_s exp(m_s - max) / sum: a wave per row.  Lanes hold the splits'
 // weights, two each; then groups of Dv / 4 lanes add every group's share of the splits, four
 // columns per lane, kJoin splits at a time (one split after the other, by a thread per four
 // columns, took 38 us for 47 splits of 16 rows).
@@ -977,7 +979,7 @@ template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_join
         if (ahead) read(0);
         const float m = wave_allreduce(fmaxf(ml0.x, ml1.x), [](float x, float y) { return fmaxf(x, y); });
         auto weight = [&](float2 ml) {         // 0 for a split that saw no key
-            return ml.y == 0.0f ? 0.0f : ml.y * (ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m));
+            return ml.y == 0.0f ? 0.0f : ml.y * (ml.x == m ? 1.0f : __builtin_amdgcn_exp2f((ml.x - m) * kLog2e));
         };
         const float w0 = weight(ml0), w1 = weight(ml1);
         const float total = wave_allreduce(w0 + w1, [](float x, float y) { return x + y; });
@@ -1041,7 +1043,7 @@ template <int DT, bool PAGED, int L> __global__ __launch_bounds__(256) void k_at
     float m = ml.x;
 #pragma unroll
     for (int o = 1; o < L; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
-    const float w = ml.y == 0.0f ? 0.0f : ml.y * (ml.x == m ? 1.0f : __builtin_amdgcn_exp2f(ml.x - m));
+    const float w = ml.y == 0.0f ? 0.0f : ml.y * (ml.x == m ? 1.0f : __builtin_amdgcn_exp2f((ml.x - m) * kLog2e));
     float total = w;
 #pragma unroll
     for (int o = 1; o < L; o *= 2) total += __shfl_xor(total, o);

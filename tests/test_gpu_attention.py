@@ -230,6 +230,51 @@ def test_scores_past_log2_units(hip, dtype):
     check(got, np.broadcast_to(p.v64[:, :, 39:40], got.shape), np.zeros_like(got), dtype)
 
 
+# Queries, keys and heads: splits of few rows and of tiles, and the join of many rows.
+SPLIT = [(3, 1500, 1), (40, 1500, 1), (300, 300, 16)]
+
+
+@pytest.mark.parametrize("dtype", ("bfloat16", "float32"))
+@pytest.mark.parametrize("low,high", [(2.5e19, 2.9e19), (-2.9e19, -2.5e19)])
+@pytest.mark.parametrize("sq,skv,heads", SPLIT)
+def test_split_scores_past_log2_units(hip, sq, skv, heads, low, high, dtype):
+    """Scores near float32's largest in every split of the keys: the largest of all takes
+    everything (its weight is one and the others' zero, so the result is its value)."""
+    from tests.attention_ref import cast, check
+    p = DenseProblem(1, heads, heads, sq, skv, 64, dtype, scale=1.0, seed=5)
+    p.q64[:], p.k64[:] = 0.0, 0.0
+    p.q64[..., 0], p.k64[..., 0] = 1e19, low
+    at = skv - 70
+    p.k64[:, :, at, 0] = high
+    (p.q, p.q64), (p.k, p.k64) = cast(p.q64, dtype), cast(p.k64, dtype)
+    got = p.run(hip)
+    check(got, np.broadcast_to(p.v64[:, :, at:at + 1], got.shape), np.zeros_like(got), dtype)
+    # the same keys in the pages of a cache, for tokens that all see them
+    c = CacheProblem([(3, skv), (1, skv)], 2, 1, 64, 16, dtype, scale=1.0, seed=6)
+    c.q64[:], c.k64[:] = 0.0, 0.0
+    c.q64[..., 0], c.k64[..., 0] = 1e19, low
+    (c.q, c.q64) = cast(c.q64, dtype)
+    want = np.empty_like(c.q64)
+    for b, rows in enumerate((slice(0, 3), slice(3, 4))):
+        c.k64[c.pages[b, at // 16], :, at % 16, 0] = high
+        want[rows] = c.v64[c.pages[b, at // 16], 0, at % 16]
+    (c.k, c.k64) = cast(c.k64, dtype)
+    check(c.run(hip), want, np.zeros_like(want), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sq,skv,heads", SPLIT)
+def test_split_masks_near_the_lowest_value(hip, sq, skv, heads, dtype):
+    """A float32 mask far below every score in every split: the key it closes least takes
+    everything."""
+    from tests.attention_ref import check
+    mask = np.full((1, skv), -3.0e38)
+    mask[:, skv - 70] = -2.6e38
+    p = DenseProblem(1, heads, heads, sq, skv, 64, dtype, mask=mask, mask_dtype="float32", seed=7)
+    got = p.run(hip)
+    check(got, np.broadcast_to(p.v64[:, :, skv - 70:skv - 69], got.shape), np.zeros_like(got), dtype)
+
+
 # ------------------------------------------------------------------- cache -------
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", SIZES)
