@@ -98,6 +98,9 @@ def make_op(node: P.NodeProto, dtypes: Dict[str, str], shapes: Dict[str, Tuple[i
     if t == "DynamicQuantizeLinear":
         return Op.DynamicQuantizeLinear(ins, outs, version="17")
     if t == "Attention":
+        if node.domain not in ("", "ai.onnx"):
+            raise NotImplementedError(f"Attention (node {node.name!r}) of domain {node.domain!r} is not supported by "
+                                      "this build")
         # inputs: q, k, v, mask, past key, past value, lengths
         for i, what in ((4, "a past key"), (5, "a past value")):
             if len(ins) > i and ins[i]:

@@ -216,6 +216,24 @@ def test_onnx_attention_node():
             make_op(_node(ins, attrs, outs), {}, {})
 
 
+def test_onnx_attention_of_another_domain():
+    """The operator of that name in another domain has other inputs (packed weights, say)."""
+    from onnx_translator_amd.nn.ONNXImport import ONNXImport, make_op
+    from onnx_translator_amd.onnx import proto as P
+    node = _node(["x", "w", "b"], {"num_heads": 8})
+    node.domain = "com.microsoft"
+    with pytest.raises(NotImplementedError, match="com.microsoft"):
+        make_op(node, {}, {})
+    g = P.GraphProto(nodes=[node], name="g", inputs=[P.ValueInfoProto("x", P.FLOAT, [1, 4, 64])],
+                     outputs=[P.ValueInfoProto("y", P.FLOAT, [1, 4, 64])], initializers=[])
+    with pytest.raises(NotImplementedError, match="com.microsoft"):
+        ONNXImport(P.ModelProto.parse(P.ModelProto(graph=g).serialize()))
+    for domain in ("", "ai.onnx"):
+        node = _node(["q", "k", "v"], {})
+        node.domain = domain
+        assert isinstance(make_op(node, {}, {}), Op.Attention)
+
+
 # ------------------------------------------------------------------ dispatch -----
 def names(result):
     launches, err = result
