@@ -108,6 +108,9 @@ def make_op(node: P.NodeProto, dtypes: Dict[str, str], shapes: Dict[str, Tuple[i
         if float(node.attr("softcap", 0.0)) or len([o for o in outs if o]) > 1:
             raise NotImplementedError(f"Attention (node {node.name!r}) with a softcap or present outputs is not "
                                       "supported by this build")
+        if int(node.attr("softmax_precision", 1)) == 11:
+            raise NotImplementedError(f"Attention (node {node.name!r}) with a float64 softmax is not supported by this "
+                                      "build")
         if int(node.attr("is_causal", 0)) and len(ins) > 6 and ins[6]:
             raise NotImplementedError(f"Attention (node {node.name!r}), causal with lengths, is not supported by this "
                                       "build")

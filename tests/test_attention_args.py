@@ -234,6 +234,15 @@ def test_onnx_attention_of_another_domain():
         assert isinstance(make_op(node, {}, {}), Op.Attention)
 
 
+def test_onnx_attention_softmax_precision():
+    """The softmax is float32: float32 and less may be asked for, float64 (11) is refused."""
+    from onnx_translator_amd.nn.ONNXImport import make_op
+    for precision in (1, 10, 16):
+        assert isinstance(make_op(_node(["q", "k", "v"], {"softmax_precision": precision}), {}, {}), Op.Attention)
+    with pytest.raises(NotImplementedError, match="float64"):
+        make_op(_node(["q", "k", "v"], {"softmax_precision": 11}), {}, {})
+
+
 # ------------------------------------------------------------------ dispatch -----
 def names(result):
     launches, err = result
