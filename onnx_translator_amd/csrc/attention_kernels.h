@@ -237,11 +237,6 @@ template <int STEP> __device__ __forceinline__ void read_values(const uint32_t (
                  : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
                  : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(STEP) : "memory");
 }
-template <int STEP> __device__ __forceinline__ void read_values(const uint32_t (&at)[2], uint2 (&x)[2], uint2 (&y)[2]) {
-    asm volatile("ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %2, %4 offset:%6\n\t"
-                 "ds_read_b64_tr_b16 %1, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(y[0]), "=&v"(y[1]) : "v"(at[0]), "v"(at[1]), "n"(STEP) : "memory");
-}
 // Eight 32-bit values of one column: rows 0 .. 3 and G .. G + 3 of RB bytes each.
 template <int RB, int G> __device__ __forceinline__ void read_column8(uint32_t at, float (&v)[8]) {
     asm volatile("ds_read_b32 %0, %8\n\tds_read_b32 %1, %8 offset:%9\n\tds_read_b32 %2, %8 offset:%10\n\t"
@@ -1080,7 +1075,7 @@ template <int DT, int D, bool PAGED, bool MASK> void launch_tiles_of(const AttnA
     if (p.rows == 16) hipLaunchKernelGGL((k_attn_few<DT, D, PAGED, MASK, 16>), dim3(p.blocks), dim3(64), 0, s, a);
     else if (p.rows == 32) hipLaunchKernelGGL((k_attn_few<DT, D, PAGED, MASK, 32>), dim3(p.blocks), dim3(64), 0, s, a);
     else if (p.rows == 128) hipLaunchKernelGGL((k_attn_tiles<DT, D, PAGED, MASK, 4, D * kElem<DT> <= 256 ? 64 : 32>), dim3(p.blocks), dim3(256), 0, s, a);
-    else if constexpr (D * kElem<DT> <= 256) hipLaunchKernelGGL((k_attn_tiles<DT, D, PAGED, MASK, 8, kKeys256>), dim3(p.blocks), dim3(512), 0, s, a);
+    else if constexpr (kElem<DT> == 2 && D <= 128) hipLaunchKernelGGL((k_attn_tiles<DT, D, PAGED, MASK, 8, kKeys256>), dim3(p.blocks), dim3(512), 0, s, a);
 }
 template <int DT, int D> void launch_tiles_d(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
     if (p.paged) launch_tiles_of<DT, D, true, false>(a, p, s);

@@ -2,6 +2,9 @@
 device work, so each call here ends with its own message (a call that passes the checks ends
 with the missing device's, or launches under the recording runtime of tests/launches)."""
 import ctypes
+import itertools
+import re
+import subprocess
 
 import numpy as np
 import pytest
@@ -343,6 +346,27 @@ def test_rotary_kernels(rec):
     assert names(rotary(rec)) == ["k_rotary_chunks"]
     assert names(rotary(rec, cos=(100, 12), sin=(100, 12))) == ["k_rotary_any"]           # 24 rotated: no whole chunk pairs
     assert names(rotary(rec, x=(5, 8 * 20), wq=(20,), wk=(20,), cos=None, sin=None, pos=None, q=(5, 4, 20), k=(5, 2, 20), v=(5, 2, 20))) == ["k_rotary_any"]
+
+
+def test_every_instance_is_reached(rec):
+    """The attention kernels in the library are those that some call launches."""
+    from tests.launches import recorder
+    out = subprocess.run(["nm", "-C", recorder.OUT], capture_output=True, text=True, check=True).stdout
+    built = {m.replace(" ", "") for m in re.findall(r"__device_stub__(k_attn_\w+<[^>]*>)", out)}
+    launched = set()
+    for dt, d, n in itertools.product((O.F16, O.BF16, O.F32), (64, 128, 256), (1, 4, 5, 1000)):
+        # one row, up to 16 and 32, and tiles, each with keys to split and without; more heads fill the GPU
+        for hkv, skv in ((1, 1500), (2, 64), (128, 300), (16, 1024)):
+            q, kv, page = (1, 5 * hkv, n, d), (1, hkv, skv, d), (skv // 4, hkv, 4, d)
+            for r in (attn(rec, q=q, k=kv, v=kv, dt=dt), attn(rec, q=q, k=kv, v=kv, dt=dt, mask=(n, skv)),
+                      cache(rec, q=(n, 5 * hkv, d), k=page, v=page, pages=(1, skv // 4), start=(2,), length=(1,), dt=dt)):
+                assert not r[1]
+                launched |= {l.kernel.replace(" ", "") for l in r[0]}
+        # a wave per row
+        for r in (attn(rec, q=(1, 2, n, d), k=(1, 2, 9, d), v=(1, 2, 9, 33), dt=dt),
+                  cache(rec, q=(n, 2, d), k=(3, 2, 4, d), v=(3, 2, 4, 33), pages=(1, 3), start=(2,), length=(1,), dt=dt)):
+            launched |= {l.kernel.replace(" ", "") for l in r[0]}
+    assert built == launched, (sorted(built - launched), sorted(launched - built))
 
 
 def test_outputs_overlap_no_input(rec):
