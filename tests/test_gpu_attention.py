@@ -230,6 +230,28 @@ def test_scores_past_log2_units(hip, dtype):
     check(got, np.broadcast_to(p.v64[:, :, 39:40], got.shape), np.zeros_like(got), dtype)
 
 
+@pytest.mark.parametrize("dtype", ("float16", "bfloat16"))
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("b,hq,hkv,sq,skv", [(2, 4, 2, 1, 900), (2, 4, 2, 9, 900), (2, 4, 2, 70, 900), (8, 64, 64, 40, 90)],
+                         ids=["few", "32 rows", "tiles", "many blocks"])
+def test_mean_of_equal_values(hip, b, hq, hkv, sq, skv, d, dtype):
+    """Keys whose values are all the same: their mean is that value, whatever the weights are and
+    however they are rounded (what is added up is what is divided by).  Sums of n float32 terms
+    are off by (2 n + 4) 2^-24 < 2^-12 of the value: it is still the nearest of the type."""
+    from tests.attention_ref import cast
+    rng = np.random.default_rng(d)
+    for kw in (dict(), dict(mask=rng.random((b, 1, sq, skv)) < 0.8)):
+        p = DenseProblem(b, hq, hkv, sq, skv, d, dtype, scale=0.25 if d == 64 else 0.1, seed=sq, **kw)
+        p.v, p.v64 = cast(np.broadcast_to(rng.normal(0, 1, (b, hkv, 1, d)), p.v64.shape), dtype)
+        got = p.run(hip)
+        want = np.repeat(p.v64[:, :, :1], hq // hkv, axis=1)
+        assert (got == want).all(), (kw.keys(), int((got != want).sum()), got.size)
+    c = CacheProblem([(sq, skv), (1, 33)], hq, hkv, d, 16, dtype, scale=0.25, seed=sq)
+    value, value64 = cast(rng.normal(0, 1, (hkv, 1, d)), dtype)
+    c.v[:], c.v64[:] = value, value64
+    assert (c.run(hip) == np.repeat(value64[None, :, 0], hq // hkv, axis=1)).all()
+
+
 # Queries, keys and heads: splits of few rows and of tiles, and the join of many rows.
 SPLIT = [(3, 1500, 1), (40, 1500, 1), (300, 300, 16)]
 
