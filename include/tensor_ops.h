@@ -357,7 +357,10 @@ void qconv_block_forward(const Tensor* X, const QConvBlock* block, Tensor* Y, Co
 /* ---------------------------------------------------------------------------
  * Attention of a decoder layer, between its projection Gemms.  No counterpart in
  * the reference.  One element type per call (float16, bfloat16 or float32);
- * scores, softmax statistics and sums in float32 or more, one rounding at the end.
+ * scores, softmax statistics and sums in float32 or more.  In 16-bit types each
+ * softmax weight is rounded to the type for its product with V (the sum that they are
+ * divided by takes them as rounded), and the result once at the end.  A q.k that falls
+ * below float32's range before the scale counts as -inf.
  * The Gemm / Conv precision mode (tensor_ops_hip_set_exact) does not apply.  A key
  * that a query does not see adds nothing, whatever K and V hold there, and a row
  * that sees no key (or whose scores are all -inf) gives zeros.  Outputs and workspaces

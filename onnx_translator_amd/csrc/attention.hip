@@ -56,8 +56,8 @@ void run_attention(AttnArgs& a, int dt, bool paged, int64_t kv, const Tensor* ws
             return t * (paged ? 1 : a.B) * a.Hkv;
         };
         // 256 rows per block where such blocks fill the GPU twice over (one fits a CU): K and V
-        // pass through LDS half as often (1024 blocks of 128 rows over 8192 keys 591 us, 512 of
-        // 256 540; of 64 values per head 120 and 100.  256 blocks over 300 .. 1500 keys: 35.6,
+        // pass through LDS half as often (1024 blocks of 128 rows over 8192 keys 589 us, 512 of
+        // 256 538; of 64 values per head 120 and 100.  256 blocks over 300 .. 1500 keys: 35.6,
         // twice as many of 128 rows 33.7).  Not where a tile of their keys may lie on more pages
         // than a wave holds numbers of (pages of one key; tiles begin at multiples of 32).
         if (p.rows == 128 && p.d * es <= 256 && es == 2 && (!paged || kKeys256 <= kTablePages * (int64_t)a.ps) &&
@@ -76,7 +76,7 @@ void run_attention(AttnArgs& a, int dt, bool paged, int64_t kv, const Tensor* ws
         // Prompts are split only where there are fewer blocks than two per CU (12 sequences of
         // 2 .. 304 tokens, 376 blocks: 54 us with twelve per CU, 56 with eight, 69 with four, 78
         // unsplit; 512 blocks over 300 .. 1500 keys: 33.7 unsplit, 42 in two; 1024 blocks of
-        // 8192: 553 and 620).
+        // 128 rows over 8192: 589 and 634).
         int64_t share = std::max<int64_t>({units * kv / ((int64_t)resident * 4), p.rows >= 128 ? 128 : 64,
                                            (kv + kMaxSplits - 1) / kMaxSplits});
         if (p.rows >= 128 && units >= std::min(resident, 2 * num_cus())) share = kv;

@@ -5,7 +5,8 @@
 //
 // over the keys a query sees.  One pass over the keys: a running maximum and sum,
 // the output rescaled where the maximum grows.  Scores, statistics and sums are
-// held in 32 bits or more; the result is rounded once.
+// held in 32 bits or more.  Two roundings to a 16-bit type: each weight p_j for its
+// product with V (and for the sum of the weights: AttnWave::pack), and the result.
 //
 // Keys that are not seen (past the length, later than the query, outside the
 // window, closed by the mask, or on a page that the cache does not have) add
@@ -33,7 +34,7 @@ __device__ __forceinline__ double lane_value(double v, int lane) {
 // Any head size, alignment and content.  Lanes take 64 keys at a time for the scores,
 // then 64 columns of V for the sums, in double: nothing overflows on the way to a
 // finite result, and a key that is not seen is never multiplied.  Bound by its double
-// products and one dependent pass after the other: what the matrix kernels do in 534 us
+// products and one dependent pass after the other: what the matrix kernels do in 540 us
 // (4096 queries over 8192 keys, 32 heads of 128) takes it 0.29 s, so it takes what they do
 // not: odd head sizes, unaligned tensors, and single rows that they hand over.
 constexpr int kRowCols = 4;        // columns of V per lane and pass over the keys
@@ -156,7 +157,8 @@ template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_rows
 // What a closed key holds does not matter as long as it is finite: its weight is zero.
 // Where a result comes out infinite or NaN (a closed key's value was, or values near the
 // type's largest overflowed a sum on the way), or a page of the sequence is missing, the
-// row is computed again by attn_row above, which looks at open keys only.
+// row is computed again by attn_row above, which looks at open keys only.  A q.k that falls
+// below float32's range before the scale is -inf, a key of no weight.
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
@@ -590,8 +592,9 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
     // mean between the values but never scales it, and a weight that takes nearly everything has
     // none.  (With the sum of the unrounded ones the error of one float16 token over 1500 keys was up
     // to 2.1 times that of float32 weights, in 10000 draws, now 1.7; bfloat16 over 1025 keys 2.0 and
-    // 1.45; on average 1.25 either way.  It costs 33.5 -> 35.6 us for 448 queries over 300 .. 1500
-    // keys of 16 heads of 64, eight batches; nothing measurable where heads are longer or rows few.)
+    // 1.45; on average 1.25 either way.  It costs 34.0 -> 36.2 us for 448 queries over 300 .. 1500
+    // keys of 16 heads of 64, eight batches; nothing measurable over pages, where heads are longer
+    // or rows few.)
     static constexpr int NPV = DT == kF32 ? NP : 1, NKK = DT == kF32 ? 1 : NP / 8;
     struct Weights {
         uint4 h[NKK];
@@ -834,8 +837,9 @@ template <int DT, int D, bool PAGED, int MR, int W> struct AttnLoads {
 // what the products' largest form takes with the sums of 128 columns still in registers.
 // Bound by the matrix and vector units together (32 keys of 32 rows: 512 cycles of products at
 // 128 values per head, about as many for the 16 exponentials per lane and what surrounds them)
-// and, at full length, by power: 4096 queries over 8192 keys, 32 heads of 128 in bf16, 534 us or
-// 1.03 PFLOP/s; the last 4096 of 16384 keys in pages of 16, 980 us.  With 64 values per head the
+// and, at full length, by power: 4096 queries over 8192 keys, 32 heads of 128 in bf16, 538 .. 557 us
+// by card or 1.0 PFLOP/s; the last 4096 of 16384 keys in pages of 16, 980 .. 1020 us (630 and
+// 1080 in the first hundred calls of an idle card, whose clock rises meanwhile).  With 64 values per head the
 // exponentials weigh twice as much.
 template <int DT, int D, bool PAGED, bool MASK, int W, int BN>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D * kElem<DT> <= 128 && W == 4 && !MASK ? 3 : D * kElem<DT> <= 256 ? 2 : 1))) void k_attn_tiles(AttnArgs a) {
@@ -897,8 +901,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D * kEle
 // 32 keys each; K's is filled again as soon as its scores are made and V's as soon as it is
 // added, so three of the four are in flight while one is worked on.  Bound by memory: 64
 // tokens of 32 heads over 130 .. 8192 keys of 8 heads of 128 in bf16 take 220 us, 5.0 TB/s
-// (filled a whole tile at a time 261); one token over 1025 keys 12.1 us, of which 4 are the
-// join's launch and the rest a chain of loads: starts, length, pages, keys.
+// (filled a whole tile at a time 261); one token over 1025 keys 12.3 us, of which 4 are the
+// join's launch and the rest a chain of loads: starts, length, pages, keys.  float32 heads of more
+// than 64 values take 64 or 128 KB of LDS per wave and, for 256 values and 32 rows, more than 512
+// registers, so two waves or one run on a CU: 16 tokens of 16 heads over 130 .. 4096 keys of 4
+// heads reach 2.0 TB/s with 64 values, 2.2 with 128, 1.5 with 256.
 template <int DT, int D, bool PAGED, bool MASK, int MR>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D * kElem<DT> <= 256 ? 2 : 1))) void k_attn_few(AttnArgs a) {
     typedef AttnWave<DT, D, PAGED, MASK, MR, (MR == 16 || D <= 128)> Wave;      // (as far as registers go)
