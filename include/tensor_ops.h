@@ -425,6 +425,78 @@ void qk_norm_rotary_forward(const Tensor* QKV, const Tensor* QWeight, const Tens
                             const Tensor* Sin, const Tensor* Positions, const Tensor* Slots, Tensor* Q, Tensor* K,
                             Tensor* V, const QKNormRotaryParams* params);
 
+/* ---------------------------------------------------------------------------
+ * The steps of a decoding loop around the attention.  No counterpart in the reference.
+ * Device tensors only; under graph capture as any other call.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    int page_size;
+} CachePlanParams;
+/* What a step's requests need of a paged cache, from their lengths.  Request b has Past[b]
+ * tokens in the cache and brings New[b] >= 0 more, or has ended (New[b] < 0).  Pages [requests,
+ * pages per request] names each request's pages in order (written in place), Free [n] is a ring
+ * of free page numbers and State (int64 [3]: pages ever taken from the ring, pages ever given
+ * back to it, requests refused) its ends: place State[0] % n is the next to be taken, place
+ * State[1] % n the next to be given back to.  A ring that has held every page of the cache once
+ * (Free = 0 .. n - 1, State = 0, n, 0) holds them for good.
+ *   First the pages of ended requests go back to the ring; then the others take, in order,
+ * what their new tokens need.  A request is refused, and takes nothing, if the needs up to and
+ * with its own are more than the ring holds, if its row of Pages is too short or if its tokens
+ * go past the rows of Positions; one that needs no page is not refused for want of pages.
+ *   QStart [requests + 1] (sums of New; refused requests keep their rows) and KVLen [requests]
+ * (Past + New, Past if refused, 0 if ended) are those of cache_attention_forward; Positions and
+ * Slots [tokens] those of qk_norm_rotary_forward: the token's place in its request plus Offset
+ * (one number, NULL: 0; a shared prefix, say) and page * page_size + place in the page, both -1
+ * for a refused request's tokens and for rows behind the last request.  A position or slot that its type does not hold
+ * is -1.  NextState receives the state after the step, with the requests refused in it.  KVLen may be Past
+ * and NextState State (the same memory and type); nothing else may overlap.  int32 or int64
+ * each, State and NextState int64. */
+void cache_plan_forward(const Tensor* New, const Tensor* Past, const Tensor* Offset, const Tensor* State,
+                        Tensor* Pages, Tensor* Free, Tensor* QStart, Tensor* KVLen, Tensor* Positions,
+                        Tensor* Slots, Tensor* NextState, const CachePlanParams* params);
+typedef struct {
+    float scale;      /* factor of q.k; 0: 1 / sqrt(size of a key) */
+    int max_prefix;   /* what the caller knows of PrefixLen and of the longest KVLen (0: nothing): */
+    int max_kv;       /* they shape the launches, never the result */
+} PrefixAttentionParams;
+/* cache_attention_forward for sequences that share a prefix: every token sees the first
+ * PrefixLen (one number) keys on the pages PrefixPages [n], in order, and of its sequence's own
+ * keys (Pages, KVLen: without the prefix) those up to its own.  The result is that of one
+ * softmax over both.  The prefix is read once for all sequences.  Types, shapes, QStart, rows
+ * behind the last sequence, pages that the cache does not have, numerics and Workspace as for
+ * cache_attention_forward, except that a call captured into a graph needs a workspace of two
+ * splits at least (two times 4 * Dv + 8 bytes for every query head of every token). */
+void prefix_cache_attention_forward(const Tensor* Q, const Tensor* KCache, const Tensor* VCache,
+                                    const Tensor* PrefixPages, const Tensor* PrefixLen, const Tensor* Pages,
+                                    const Tensor* QStart, const Tensor* KVLen, Tensor* Y,
+                                    const PrefixAttentionParams* params, Tensor* Workspace);
+typedef struct {
+    int vocab;        /* the columns of Logits that are tokens, from the first on; 0: all */
+} SampleParams;
+/* A token per row of Logits [rows, columns] (float16, bfloat16 or float32) from a given random
+ * number.  With x a row, t = Temperature[row], weights w_i = exp((x_i - max x) / t):
+ *   TopK     k > 0: the k largest x are kept (0 or less: all);
+ *   TopP     of those, in falling order, the ones whose larger ones weigh less than p of all
+ *            those (the largest always; p >= 1 or NaN: all);
+ *   MinP     of those, the ones with w_i >= m (m > 1 counts as 1, NaN as 0);
+ * each [rows], NULL: not applied; equal x rank by index, the lower first.  Token[row] is the
+ * first kept index whose weight with those of the kept indices before it is more than
+ * Uniform[row] (in [0, 1), float32 or float64) times the weight of all kept.  A temperature of 0
+ * or less (or NaN) takes the largest x, the first of equal ones; Temperature NULL: 1.  NaN
+ * among the logits count as -inf, which is never drawn; a row of nothing else gives -1.
+ * Temperature, TopP and MinP are float32, TopK int32 or int64, Token int32 or int64.  LogProb
+ * (float32 [rows], may be NULL) receives the logarithm of the probability with which the token
+ * was drawn (0 for a greedy row, -inf for Token -1).  Sums of weights are kept in 64-bit fixed
+ * point, at least 2^-44 of the largest weight for up to 2^18 columns, in which their order does
+ * not matter: the same call gives the same token.
+ *   Workspace (may be NULL): device memory of any type, 16-byte aligned, that lets a call spread
+ * a row over the GPU: sample_workspace_bytes(rows, columns) bytes.  Without one an eager call takes them from the
+ * library's pool; a call captured into a graph keeps each row on one compute unit, which is
+ * slower where rows are few and long.  Calls that may overlap must not share one. */
+void sample_forward(const Tensor* Logits, const Tensor* Uniform, const Tensor* Temperature, const Tensor* TopK,
+                    const Tensor* TopP, const Tensor* MinP, Tensor* Token, Tensor* LogProb,
+                    const SampleParams* params, Tensor* Workspace);
+
 #ifdef __cplusplus
 }
 #endif

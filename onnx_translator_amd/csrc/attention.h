@@ -33,6 +33,9 @@ struct AttnArgs {
     int mask_dt;                   // kU8 / kI8: 0 closes a key; else added to the score
     IndexVec len;                  // keys in use per batch (dense: p may be null) or sequence
     IndexVec pages, qstart;        // paged only
+    int64_t qstep;                 // entries of qstart from one sequence's to the next one's
+    IndexVec prefix, plen;         // the rows' kernel of a shared prefix: its pages, its keys
+    int prefix_pages;
     int B, Hq, Hkv, G, Sq, Skv, Dk, Dv;
     int T;                         // paged: tokens of Q
     int ps, max_pages, npages;     // page size, pages per sequence, pages of the cache
@@ -41,6 +44,7 @@ struct AttnArgs {
     int causal, window;
     // tiles: rows of tiles per batch (dense) or in all (paged), and the key splits of each
     int tiles, nsplit, share;      // share: keys of a split
+    bool parts;                    // partial results (also of one split) instead of Y
     float* part_o;                 // [nsplit][rows][Dv]: normalised results of a split
     float2* part_ml;               // [nsplit][rows]: (maximum of the scores, sum against it)
     int64_t rows;                  // rows of Y: tokens x query heads
@@ -68,7 +72,7 @@ __device__ __forceinline__ AttnSeq attn_seq_at(const AttnArgs& a, int b, int64_t
 }
 template <bool PAGED> __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int b) {
     if constexpr (PAGED) {
-        return attn_seq_at(a, b, a.qstart[b], a.qstart[b + 1]);
+        return attn_seq_at(a, b, a.qstart[b * a.qstep], a.qstart[(b + 1) * a.qstep]);
     } else {
         AttnSeq s;
         s.b = b;
@@ -94,9 +98,20 @@ __device__ __forceinline__ int attn_lo(const AttnArgs& a, const AttnSeq& s, int 
     return a.window && p > 0 ? (int)p : 0;
 }
 
-// The page of key j of sequence b, or -1 where the table names none of the cache's.
-__device__ __forceinline__ int attn_page(const AttnArgs& a, int b, int j) {
-    const int64_t p = a.pages[(int64_t)b * a.max_pages + (int)a.fd_ps.div((uint32_t)j)];
+// Keys at fixed strides, in pages, or in pages behind those of a prefix that all sequences share.
+constexpr int kDense = 0, kPaged = 1, kPrefixed = 2;
+
+// Keys of the prefix.
+__device__ __forceinline__ int attn_shared(const AttnArgs& a) {
+    const int64_t l = a.plen[0], cap = (int64_t)a.prefix_pages * a.ps;
+    return (int)(l < 0 ? 0 : l > cap ? cap : l);
+}
+// The page of key j of sequence b, or -1 where the table names none of the cache's.  (With a
+// prefix keys 0 .. shared - 1 are the prefix's.)
+template <int KEYS> __device__ __forceinline__ int attn_page(const AttnArgs& a, int b, int j, int shared) {
+    int64_t p;
+    if (KEYS == kPrefixed && j < shared) p = a.prefix[(int)a.fd_ps.div((uint32_t)j)];
+    else p = a.pages[(int64_t)b * a.max_pages + (int)a.fd_ps.div((uint32_t)(j - shared))];
     return p >= 0 && p < a.npages ? (int)p : -1;
 }
 
@@ -138,10 +153,11 @@ constexpr int kTablePages = 64;    // page numbers that a wave holds, one per la
 constexpr int kKeys256 = 128;      // keys of a tile under blocks of 256 rows (64 or 32 under the others)
 
 struct AttnPlan {
-    bool paged;
+    int keys;                      // kDense, kPaged; kPrefixed (a wave per row only)
     int d;                         // padded head size of the tile kernels; 0: a wave per row
     int rows;                      // rows of a block: 16 or 32 (one wave), 128 (four) or 256 (eight)
-    unsigned blocks;
+    unsigned blocks;               // 0: the join alone
+    bool join;                     // the splits, if there are several, follow
 };
 void launch_attention_f16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);
 void launch_attention_bf16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);

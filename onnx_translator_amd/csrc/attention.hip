@@ -1,5 +1,6 @@
-// attention.hip — attention_forward (dense keys and values, masks, lengths) and
-// cache_attention_forward (new tokens over a paged cache): argument checks and launches.
+// attention.hip — attention_forward (dense keys and values, masks, lengths),
+// cache_attention_forward (new tokens over a paged cache) and prefix_cache_attention_forward
+// (the same behind a shared prefix): argument checks and launches.
 // The kernels are in attention_kernels.h.
 #include "attention.h"
 
@@ -35,52 +36,159 @@ bool apart(std::initializer_list<const Tensor*> inputs, const Tensor* Y, const T
     return true;
 }
 
+bool good_workspace(const Tensor* ws, const char* name) {
+    if (!ws || (tensor_sane(ws, name) && (!ws->size || is_dev(classify(ws->data))))) return true;
+    if (!*tensor_ops_hip_last_error()) set_error("%s: Workspace must be a device tensor", name);
+    return false;
+}
+
+// What the calls over a paged cache have in common.
+bool cache_args(AttnArgs& a, const Tensor* Q, const Tensor* KCache, const Tensor* VCache, const Tensor* Pages,
+                const Tensor* QStart, const Tensor* KVLen, const Tensor* Y, float scale, const char* name) {
+    const Tensor* all[] = {Q, KCache, VCache, Pages, QStart, KVLen, Y};
+    for (const Tensor* t : all) {
+        if (!tensor_sane(t, name)) return false;
+        if (t->size && !is_dev(classify(t->data))) { set_error("%s: every tensor must be device-resident", name); return false; }
+    }
+    if (!float_type(Q) || Q->dtype != KCache->dtype || Q->dtype != VCache->dtype || Q->dtype != Y->dtype) {
+        set_error("%s: Q, the caches and Y must have one type: float16, bfloat16 or float32", name);
+        return false;
+    }
+    if (Q->ndim != 3 || KCache->ndim != 4 || VCache->ndim != 4 || Y->ndim != 3) {
+        set_error("%s: Q and Y must be [tokens, heads, size], the caches [pages, heads, page size, size]", name);
+        return false;
+    }
+    a.T = Q->shape[0];
+    a.Hq = Q->shape[1];
+    a.Dk = Q->shape[2];
+    a.npages = KCache->shape[0];
+    a.Hkv = KCache->shape[1];
+    a.ps = KCache->shape[2];
+    a.Dv = VCache->shape[3];
+    if (a.npages < 1 || a.ps < 1 || a.Dk < 1 || a.Dv < 1 || KCache->shape[3] != a.Dk || VCache->shape[0] != a.npages ||
+        VCache->shape[1] != a.Hkv || VCache->shape[2] != a.ps) {
+        set_error("%s: the shapes of Q and the caches do not belong together", name);
+        return false;
+    }
+    if (a.Hq < 1 || a.Hkv < 1 || a.Hq % a.Hkv) {
+        set_error("%s: the query heads must be a multiple of the key heads, got %d and %d", name, a.Hq, a.Hkv);
+        return false;
+    }
+    if (Y->shape[0] != a.T || Y->shape[1] != a.Hq || Y->shape[2] != a.Dv) {
+        set_error("%s: Y must have Q's shape with the values' head size", name);
+        return false;
+    }
+    if (!index_type(Pages) || !index_type(QStart) || !index_type(KVLen) || Pages->ndim != 2 || QStart->ndim != 1 ||
+        KVLen->ndim != 1 || KVLen->shape[0] != Pages->shape[0] || QStart->shape[0] != Pages->shape[0] + 1) {
+        set_error("%s: Pages must be [sequences, pages], KVLen [sequences] and QStart [sequences + 1], int32 or int64", name);
+        return false;
+    }
+    if (!good_scale(scale, name)) return false;
+    a.B = Pages->shape[0];
+    a.max_pages = Pages->shape[1];
+    if ((int64_t)a.max_pages * a.ps > kMaxKeys) {
+        set_error("%s: Pages hold 2^31 keys or more per sequence", name);
+        return false;
+    }
+    a.G = a.Hq / a.Hkv;
+    a.fd_g = make_fastdiv((uint32_t)a.G);
+    a.fd_ps = make_fastdiv((uint32_t)a.ps);
+    a.scale = scale != 0.0f ? scale : (float)(1.0 / std::sqrt((double)a.Dk));
+    a.causal = 1;
+    a.qstep = 1;
+    a.qh = a.Dk;
+    a.qt = (int64_t)a.Hq * a.Dk;
+    a.yh = a.Dv;
+    a.yt = (int64_t)a.Hq * a.Dv;
+    a.kt = a.Dk;
+    a.kh = (int64_t)a.ps * a.Dk;
+    a.kb = a.kh * a.Hkv;
+    a.vt = a.Dv;
+    a.vh = (int64_t)a.ps * a.Dv;
+    a.vb = a.vh * a.Hkv;
+    a.q = Q->data;
+    a.k = KCache->data;
+    a.v = VCache->data;
+    a.y = Y->data;
+    a.pages = {Pages->data, (int)Pages->dtype == kI64};
+    a.qstart = {QStart->data, (int)QStart->dtype == kI64};
+    a.len = {KVLen->data, (int)KVLen->dtype == kI64};
+    return true;
+}
+
+// The blocks that a call's rows make.
+struct AttnBlocks {
+    int64_t units, tiles;              // blocks of one split; row tiles of a batch (dense) or in all (paged)
+    int resident;                      // blocks on the GPU at once
+};
+
+// Whether the matrix kernels take the call; its block shape in p.
+bool attention_blocks(const AttnArgs& a, int es, bool paged, AttnPlan& p, AttnBlocks& k) {
+    const int vec = 16 / es, dm = a.Dk > a.Dv ? a.Dk : a.Dv;
+    const int64_t per = paged ? (int64_t)a.T : (int64_t)a.Sq;      // tokens of a sequence at most
+    if (!(dm <= 256 && a.Dk % vec == 0 && a.Dv % vec == 0 && per * a.G < 0x7FFFFF00 && a.kt * es < (1 << 26) &&
+          a.vt * es < (1 << 26) && aligned(a.q) && aligned(a.k) && aligned(a.v) && aligned(a.y)))
+        return false;
+    p.d = dm <= 64 ? 64 : dm <= 128 ? 128 : 256;
+    const int64_t mean = paged ? ((int64_t)a.T * a.G + a.B - 1) / a.B : per * a.G;      // rows of a sequence
+    p.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 128;
+    auto units_of = [&](int rows) {
+        const int64_t t = paged ? (int64_t)a.T * a.G / rows + a.B : (per * a.G + rows - 1) / rows;
+        return t * (paged ? 1 : a.B) * a.Hkv;
+    };
+    // 256 rows per block where such blocks fill the GPU twice over (one fits a CU): K and V
+    // pass through LDS half as often (1024 blocks of 128 rows over 8192 keys 589 us, 512 of
+    // 256 538; of 64 values per head 120 and 100.  256 blocks over 300 .. 1500 keys: 35.6,
+    // twice as many of 128 rows 33.7).  Not where a tile of their keys may lie on more pages
+    // than a wave holds numbers of (pages of one key; tiles begin at multiples of 32).
+    if (p.rows == 128 && p.d * es <= 256 && es == 2 && (!paged || kKeys256 <= kTablePages * (int64_t)a.ps) &&
+        units_of(256) >= 2 * num_cus())
+        p.rows = 256;
+    k.units = units_of(p.rows);
+    k.tiles = k.units / ((paged ? 1 : a.B) * (int64_t)a.Hkv);
+    const int bn = p.rows == 128 && p.d * es <= 256 ? 64 : 32;
+    const int lds = 4 * bn * p.d * es;
+    // blocks on a CU at once (by registers: three of four waves for 64 values of 16 bits)
+    const int most = p.rows == 128 ? (p.d * es <= 128 && !a.mask ? 3 : 2) : 8;
+    k.resident = num_cus() * (p.rows == 256 ? 1 : std::min(160 * 1024 / lds, most));
+    return true;
+}
+
+// Keys per split: four blocks for every place on the GPU, as lengths differ, and two tiles
+// at least (64 tokens over 130 .. 8192 keys: 219 us with four, 231 with sixteen, 356 with
+// two; one token over 1025: 12.4 us with two tiles, 13.2 with one, 14.0 with four, 18.2
+// with eight; 96 blocks of 577 f32 keys: 39 with 128 keys, 45 with 64, 57 with 256).
+// Prompts are split only where there are fewer blocks than two per CU (12 sequences of
+// 2 .. 304 tokens, 376 blocks: 54 us with twelve per CU, 56 with eight, 69 with four, 78
+// unsplit; 512 blocks over 300 .. 1500 keys: 33.7 unsplit, 42 in two; 1024 blocks of
+// 128 rows over 8192: 589 and 634).
+int64_t attention_share(const AttnPlan& p, const AttnBlocks& k, int64_t kv, int splits) {
+    int64_t share = std::max<int64_t>({k.units * kv / ((int64_t)k.resident * 4), p.rows >= 128 ? 128 : 64,
+                                       (kv + splits - 1) / splits});
+    if (p.rows >= 128 && k.units >= std::min(k.resident, 2 * num_cus())) share = kv;
+    return (share + 31) / 32 * 32;
+}
+
+// Whether the blocks of a launch stay within the runtime's work-items.
+bool launchable(const AttnPlan& p, const AttnBlocks& k, int64_t split) {
+    const int threads = p.rows >= 128 ? 2 * p.rows : 64;
+    return k.tiles <= 0x7FFFFFFF && k.units * split * threads < (int64_t(1) << 32);
+}
+
+void launch(const AttnArgs& a, const AttnPlan& p, int dt) {
+    (dt == kF16 ? launch_attention_f16 : dt == kBF16 ? launch_attention_bf16 : launch_attention_f32)(a, p, stream());
+}
+
 // Cuts the call into blocks and launches it.  kv: the most keys that a row may see, as far
 // as the host knows.
 void run_attention(AttnArgs& a, int dt, bool paged, int64_t kv, const Tensor* ws, const char* name) {
-    const int es = dt == kF32 ? 4 : 2, vec = 16 / es, dm = a.Dk > a.Dv ? a.Dk : a.Dv;
-    const int64_t tokens = paged ? (int64_t)a.T : (int64_t)a.B * a.Sq;
-    a.rows = tokens * a.Hq;
+    a.rows = (paged ? (int64_t)a.T : (int64_t)a.B * a.Sq) * a.Hq;
     a.nsplit = 1;
-    AttnPlan p = {paged, 0, 0, 0};
+    AttnPlan p = {paged ? kPaged : kDense, 0, 0, 0, true};
+    AttnBlocks k;
     void* part = nullptr;
-    const int64_t per = paged ? (int64_t)a.T : (int64_t)a.Sq;      // tokens of a sequence at most
-    if (dm <= 256 && a.Dk % vec == 0 && a.Dv % vec == 0 && per * a.G < 0x7FFFFF00 && a.kt * es < (1 << 26) &&
-        a.vt * es < (1 << 26) && aligned(a.q) && aligned(a.k) &&
-        aligned(a.v) && aligned(a.y)) {
-        p.d = dm <= 64 ? 64 : dm <= 128 ? 128 : 256;
-        const int64_t mean = paged ? ((int64_t)a.T * a.G + a.B - 1) / a.B : per * a.G;      // rows of a sequence
-        p.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 128;
-        auto units_of = [&](int rows) {
-            const int64_t t = paged ? (int64_t)a.T * a.G / rows + a.B : (per * a.G + rows - 1) / rows;
-            return t * (paged ? 1 : a.B) * a.Hkv;
-        };
-        // 256 rows per block where such blocks fill the GPU twice over (one fits a CU): K and V
-        // pass through LDS half as often (1024 blocks of 128 rows over 8192 keys 589 us, 512 of
-        // 256 538; of 64 values per head 120 and 100.  256 blocks over 300 .. 1500 keys: 35.6,
-        // twice as many of 128 rows 33.7).  Not where a tile of their keys may lie on more pages
-        // than a wave holds numbers of (pages of one key; tiles begin at multiples of 32).
-        if (p.rows == 128 && p.d * es <= 256 && es == 2 && (!paged || kKeys256 <= kTablePages * (int64_t)a.ps) &&
-            units_of(256) >= 2 * num_cus())
-            p.rows = 256;
-        const int64_t units = units_of(p.rows), tiles = units / ((paged ? 1 : a.B) * (int64_t)a.Hkv);
-        const int bn = p.rows == 128 && p.d * es <= 256 ? 64 : 32;
-        const int lds = 4 * bn * p.d * es;
-        // blocks on a CU at once (by registers: three of four waves for 64 values of 16 bits)
-        const int most = p.rows == 128 ? (p.d * es <= 128 && !a.mask ? 3 : 2) : 8;
-        const int resident = num_cus() * (p.rows == 256 ? 1 : std::min(160 * 1024 / lds, most));
-        // Keys per split: four blocks for every place on the GPU, as lengths differ, and two tiles
-        // at least (64 tokens over 130 .. 8192 keys: 219 us with four, 231 with sixteen, 356 with
-        // two; one token over 1025: 12.4 us with two tiles, 13.2 with one, 14.0 with four, 18.2
-        // with eight; 96 blocks of 577 f32 keys: 39 with 128 keys, 45 with 64, 57 with 256).
-        // Prompts are split only where there are fewer blocks than two per CU (12 sequences of
-        // 2 .. 304 tokens, 376 blocks: 54 us with twelve per CU, 56 with eight, 69 with four, 78
-        // unsplit; 512 blocks over 300 .. 1500 keys: 33.7 unsplit, 42 in two; 1024 blocks of
-        // 128 rows over 8192: 589 and 634).
-        int64_t share = std::max<int64_t>({units * kv / ((int64_t)resident * 4), p.rows >= 128 ? 128 : 64,
-                                           (kv + kMaxSplits - 1) / kMaxSplits});
-        if (p.rows >= 128 && units >= std::min(resident, 2 * num_cus())) share = kv;
-        share = (share + 31) / 32 * 32;
+    if (attention_blocks(a, dt == kF32 ? 4 : 2, paged, p, k)) {
+        int64_t share = attention_share(p, k, kv, kMaxSplits);
         int64_t split = kv > share ? (kv + share - 1) / share : 1;
         const int64_t each = a.rows * (a.Dv * 4 + 8);
         if (split > 1 && ws) {
@@ -95,21 +203,101 @@ void run_attention(AttnArgs& a, int dt, bool paged, int64_t kv, const Tensor* ws
         if (split > 1) {
             a.nsplit = (int)split;
             a.share = (int)share;
+            a.parts = true;
             a.part_o = (float*)part;
             a.part_ml = (float2*)(a.part_o + split * a.rows * a.Dv);
         }
-        const int64_t blocks = units * a.nsplit;
-        const int threads = p.rows >= 128 ? 2 * p.rows : 64;
-        if (tiles > 0x7FFFFFFF || blocks * threads >= (int64_t(1) << 32)) {
+        if (!launchable(p, k, a.nsplit)) {
             p.d = 0;                                   // past the runtime's work-items per launch
             a.nsplit = 1;
         }
-        a.tiles = (int)tiles;
-        p.blocks = (unsigned)blocks;
+        a.tiles = (int)k.tiles;
+        p.blocks = (unsigned)(k.units * a.nsplit);
     }
-    (dt == kF16 ? launch_attention_f16 : dt == kBF16 ? launch_attention_bf16 : launch_attention_f32)(a, p, stream());
+    launch(a, p, dt);
     check_launch(name);
     if (part && !ws) pool_free(part);
+}
+
+// A batch behind a shared prefix: the prefix's keys as those of one long sequence whose new
+// tokens are all of the batch's (so a tile of rows is filled by many sequences, and the keys
+// are read once per tile and not once per sequence), each sequence's own keys as ever, both as
+// partial results, and one join.  own_kv, prefix_kv: the most keys, as far as the host knows.
+void run_prefixed(AttnArgs& own, int dt, int64_t own_kv, int64_t prefix_kv, const Tensor* ws, const char* name) {
+    const int es = dt == kF32 ? 4 : 2;
+    own.rows = (int64_t)own.T * own.Hq;
+    own.nsplit = 1;
+    AttnArgs pre = own;
+    pre.qstep = own.B;
+    pre.B = 1;
+    pre.pages = own.prefix;
+    pre.len = own.plen;
+    pre.max_pages = own.prefix_pages;
+    pre.causal = 0;
+    AttnPlan p0 = {kPaged, 0, 0, 0, false}, p1 = p0;
+    AttnBlocks k0, k1;
+    if (attention_blocks(pre, es, true, p0, k0) && attention_blocks(own, es, true, p1, k1)) {
+        int64_t share0 = attention_share(p0, k0, prefix_kv, kMaxSplits - 32), share1 = attention_share(p1, k1, own_kv, 32);
+        if (p0.rows >= 128) {
+            // two blocks for every CU's place: each split writes and reads a partial row of Dv
+            // float32 for what it saves in time
+            const int64_t split = std::max<int64_t>(1, 2 * num_cus() / (((int64_t)own.T * own.G + p0.rows - 1) / p0.rows * own.Hkv));
+            share0 = std::max<int64_t>((prefix_kv + split - 1) / split, 128);
+            share0 = std::max(share0, (prefix_kv + kMaxSplits - 33) / (kMaxSplits - 32));
+            share0 = (share0 + 31) / 32 * 32;
+        }
+        auto splits = [](int64_t kv, int64_t share) { return kv > share ? (kv + share - 1) / share : 1; };
+        const int64_t each = own.rows * (own.Dv * 4 + 8);
+        int64_t n0 = splits(prefix_kv, share0), n1 = splits(own_kv, share1);
+        void* part = nullptr;
+        if (ws && aligned(ws->data) && (int64_t)tensor_bytes(ws) / each >= 2) {
+            const int64_t room = (int64_t)tensor_bytes(ws) / each;
+            if (n0 + n1 > room) {                      // fewer of both
+                n1 = std::max<int64_t>(1, n1 * room / (n0 + n1));
+                n0 = std::max<int64_t>(1, room - n1);
+                share0 = ((prefix_kv + n0 - 1) / n0 + 31) / 32 * 32;
+                share1 = ((own_kv + n1 - 1) / n1 + 31) / 32 * 32;
+            }
+            part = ws->data;
+        } else {
+            ws = nullptr;
+            if (stream_capturing(stream())) {
+                set_error("%s: a captured call needs a workspace of two splits at least (%lld bytes, 16-byte aligned)", name,
+                          (long long)(2 * each));
+                return;
+            }
+            part = pool_alloc((size_t)((n0 + n1) * each), true);
+        }
+        if (part && launchable(p0, k0, n0) && launchable(p1, k1, n1)) {
+            AttnArgs all = own;
+            all.nsplit = (int)(n0 + n1);
+            all.parts = true;
+            all.part_o = (float*)part;
+            all.part_ml = (float2*)(all.part_o + all.nsplit * own.rows * own.Dv);
+            auto run = [&](AttnArgs& a, AttnPlan& p, const AttnBlocks& k, int64_t n, int64_t share, int64_t at) {
+                a.nsplit = (int)n;
+                a.share = (int)share;
+                a.parts = true;
+                a.tiles = (int)k.tiles;
+                a.part_o = all.part_o + at * own.rows * own.Dv;
+                a.part_ml = all.part_ml + at * own.rows;
+                p.blocks = (unsigned)(k.units * n);
+                launch(a, p, dt);
+            };
+            run(pre, p0, k0, n0, share0, 0);
+            run(own, p1, k1, n1, share1, n0);
+            p1.blocks = 0;
+            p1.join = true;
+            launch(all, p1, dt);
+            check_launch(name);
+            if (!ws) pool_free(part);
+            return;
+        }
+        if (part && !ws) pool_free(part);
+    }
+    AttnPlan rows = {kPrefixed, 0, 0, 0, false};       // other sizes, and calls without memory
+    launch(own, rows, dt);
+    check_launch(name);
 }
 
 }  // namespace
@@ -219,10 +407,7 @@ void attention_forward(const Tensor* Q, const Tensor* K, const Tensor* V, const 
             return;
         }
     }
-    if (Workspace && (!tensor_sane(Workspace, name) || (Workspace->size && !is_dev(classify(Workspace->data))))) {
-        if (!*tensor_ops_hip_last_error()) set_error("%s: Workspace must be a device tensor", name);
-        return;
-    }
+    if (!good_workspace(Workspace, name)) return;
     if (!apart({Q, K, V, Mask, KVLen}, Y, Workspace, name)) return;
     if (!ensure_device()) return;
     if (!Y->size) return;
@@ -246,86 +431,52 @@ void cache_attention_forward(const Tensor* Q, const Tensor* KCache, const Tensor
     const char* name = "cache_attention_forward";
     tensor_ops_hip_clear_error();
     if (!params) { set_error("%s: NULL params", name); return; }
-    const Tensor* all[] = {Q, KCache, VCache, Pages, QStart, KVLen, Y};
-    for (const Tensor* t : all) {
-        if (!tensor_sane(t, name)) return;
-        if (t->size && !is_dev(classify(t->data))) { set_error("%s: every tensor must be device-resident", name); return; }
-    }
-    if (!float_type(Q) || Q->dtype != KCache->dtype || Q->dtype != VCache->dtype || Q->dtype != Y->dtype) {
-        set_error("%s: Q, the caches and Y must have one type: float16, bfloat16 or float32", name);
-        return;
-    }
-    if (Q->ndim != 3 || KCache->ndim != 4 || VCache->ndim != 4 || Y->ndim != 3) {
-        set_error("%s: Q and Y must be [tokens, heads, size], the caches [pages, heads, page size, size]", name);
-        return;
-    }
     AttnArgs a = {};
-    a.T = Q->shape[0];
-    a.Hq = Q->shape[1];
-    a.Dk = Q->shape[2];
-    a.npages = KCache->shape[0];
-    a.Hkv = KCache->shape[1];
-    a.ps = KCache->shape[2];
-    a.Dv = VCache->shape[3];
-    if (a.npages < 1 || a.ps < 1 || a.Dk < 1 || a.Dv < 1 || KCache->shape[3] != a.Dk || VCache->shape[0] != a.npages ||
-        VCache->shape[1] != a.Hkv || VCache->shape[2] != a.ps) {
-        set_error("%s: the shapes of Q and the caches do not belong together", name);
-        return;
-    }
-    if (a.Hq < 1 || a.Hkv < 1 || a.Hq % a.Hkv) {
-        set_error("%s: the query heads must be a multiple of the key heads, got %d and %d", name, a.Hq, a.Hkv);
-        return;
-    }
-    if (Y->shape[0] != a.T || Y->shape[1] != a.Hq || Y->shape[2] != a.Dv) {
-        set_error("%s: Y must have Q's shape with the values' head size", name);
-        return;
-    }
-    if (!index_type(Pages) || !index_type(QStart) || !index_type(KVLen) || Pages->ndim != 2 || QStart->ndim != 1 ||
-        KVLen->ndim != 1 || KVLen->shape[0] != Pages->shape[0] || QStart->shape[0] != Pages->shape[0] + 1) {
-        set_error("%s: Pages must be [sequences, pages], KVLen [sequences] and QStart [sequences + 1], int32 or int64", name);
-        return;
-    }
-    if (!good_scale(params->scale, name)) return;
+    if (!cache_args(a, Q, KCache, VCache, Pages, QStart, KVLen, Y, params->scale, name)) return;
     if (params->window < 0 || params->max_kv < 0) { set_error("%s: window and max_kv must not be negative", name); return; }
-    a.B = Pages->shape[0];
-    a.max_pages = Pages->shape[1];
-    if ((int64_t)a.max_pages * a.ps > kMaxKeys) {
-        set_error("%s: Pages hold 2^31 keys or more per sequence", name);
-        return;
-    }
-    if (Workspace && (!tensor_sane(Workspace, name) || (Workspace->size && !is_dev(classify(Workspace->data))))) {
-        if (!*tensor_ops_hip_last_error()) set_error("%s: Workspace must be a device tensor", name);
-        return;
-    }
+    if (!good_workspace(Workspace, name)) return;
     if (!apart({Q, KCache, VCache, Pages, QStart, KVLen}, Y, Workspace, name)) return;
     if (!ensure_device()) return;
     if (!Y->size || !a.B) return;
-    a.G = a.Hq / a.Hkv;
-    a.fd_g = make_fastdiv((uint32_t)a.G);
-    a.fd_ps = make_fastdiv((uint32_t)a.ps);
-    a.scale = params->scale != 0.0f ? params->scale : (float)(1.0 / std::sqrt((double)a.Dk));
-    a.causal = 1;
-    a.window = params->window < (int64_t)a.max_pages * a.ps ? params->window : 0;     // (one that long closes nothing)
-    a.qh = a.Dk;
-    a.qt = (int64_t)a.Hq * a.Dk;
-    a.yh = a.Dv;
-    a.yt = (int64_t)a.Hq * a.Dv;
-    a.kt = a.Dk;
-    a.kh = (int64_t)a.ps * a.Dk;
-    a.kb = a.kh * a.Hkv;
-    a.vt = a.Dv;
-    a.vh = (int64_t)a.ps * a.Dv;
-    a.vb = a.vh * a.Hkv;
-    a.q = Q->data;
-    a.k = KCache->data;
-    a.v = VCache->data;
-    a.y = Y->data;
-    a.pages = {Pages->data, (int)Pages->dtype == kI64};
-    a.qstart = {QStart->data, (int)QStart->dtype == kI64};
-    a.len = {KVLen->data, (int)KVLen->dtype == kI64};
-    DeviceScope scope;
     const int64_t cap = (int64_t)a.max_pages * a.ps;
+    a.window = params->window < cap ? params->window : 0;     // (one that long closes nothing)
+    DeviceScope scope;
     run_attention(a, (int)Q->dtype, true, params->max_kv ? std::min<int64_t>(params->max_kv, cap) : cap, Workspace, name);
+}
+
+void prefix_cache_attention_forward(const Tensor* Q, const Tensor* KCache, const Tensor* VCache,
+                                    const Tensor* PrefixPages, const Tensor* PrefixLen, const Tensor* Pages,
+                                    const Tensor* QStart, const Tensor* KVLen, Tensor* Y,
+                                    const PrefixAttentionParams* params, Tensor* Workspace) {
+    const char* name = "prefix_cache_attention_forward";
+    tensor_ops_hip_clear_error();
+    if (!params) { set_error("%s: NULL params", name); return; }
+    AttnArgs a = {};
+    if (!cache_args(a, Q, KCache, VCache, Pages, QStart, KVLen, Y, params->scale, name)) return;
+    for (const Tensor* t : {PrefixPages, PrefixLen}) {
+        if (!tensor_sane(t, name)) return;
+        if (t->size && !is_dev(classify(t->data))) { set_error("%s: every tensor must be device-resident", name); return; }
+    }
+    if (!index_type(PrefixPages) || !index_type(PrefixLen) || PrefixPages->ndim != 1 || PrefixLen->size != 1) {
+        set_error("%s: PrefixPages must be [pages] and PrefixLen one number, int32 or int64", name);
+        return;
+    }
+    if (params->max_prefix < 0 || params->max_kv < 0) { set_error("%s: max_prefix and max_kv must not be negative", name); return; }
+    a.prefix_pages = PrefixPages->shape[0];
+    const int64_t cap = (int64_t)a.max_pages * a.ps, prefix_cap = (int64_t)a.prefix_pages * a.ps;
+    if (prefix_cap > kMaxKeys || cap + prefix_cap > kMaxKeys) {
+        set_error("%s: PrefixPages and Pages hold 2^31 keys or more per sequence", name);
+        return;
+    }
+    if (!good_workspace(Workspace, name)) return;
+    if (!apart({Q, KCache, VCache, PrefixPages, PrefixLen, Pages, QStart, KVLen}, Y, Workspace, name)) return;
+    if (!ensure_device()) return;
+    if (!Y->size || !a.B) return;
+    a.prefix = {PrefixPages->data, (int)PrefixPages->dtype == kI64};
+    a.plen = {PrefixLen->data, (int)PrefixLen->dtype == kI64};
+    DeviceScope scope;
+    auto known = [](int most, int64_t cap) { return most ? std::min<int64_t>(most, cap) : cap; };
+    run_prefixed(a, (int)Q->dtype, known(params->max_kv, cap), known(params->max_prefix, prefix_cap), Workspace, name);
 }
 
 }  // extern "C"

@@ -41,11 +41,13 @@ constexpr int kRowCols = 4;        // columns of V per lane and pass over the ke
 
 // Partial result of the keys [ks, ke) for query head h of token i: the maximum (of
 // scaled scores), the sum and, by store(d, value), the normalised output.
-template <int DT, bool PAGED, class ST>
+template <int DT, int KEYS, class ST>
 __device__ __forceinline__ void attn_row(const AttnArgs& a, const AttnSeq& s, int h, int i, int ks, int ke, float& m_out,
                                          float& l_out, ST store) {
+    constexpr bool PAGED = KEYS != kDense;
     const int lane = (int)(threadIdx.x & 63), hk = (int)a.fd_g.div((uint32_t)h);
-    const int lo = max(ks, attn_lo(a, s, i)), hi = min(ke, attn_hi(a, s, i));
+    const int shared = KEYS == kPrefixed ? attn_shared(a) : 0;      // all of them are seen
+    const int lo = max(ks, attn_lo(a, s, i)), hi = min(ke, shared + (shared ? max(attn_hi(a, s, i), 0) : attn_hi(a, s, i)));
     const int64_t qo = PAGED ? (s.tok0 + i) * a.qt + h * a.qh : s.b * a.qb + i * a.qt + h * a.qh;
     const int64_t mo = s.b * a.mb + h * a.mh + i * a.mq;
     for (int d0 = 0; d0 < a.Dv; d0 += 64 * kRowCols) {
@@ -54,12 +56,12 @@ __device__ __forceinline__ void attn_row(const AttnArgs& a, const AttnSeq& s, in
         for (int j0 = lo; j0 < hi; j0 += 64) {
             const int j = j0 + lane;
             bool seen = j < hi;
-            const int page = PAGED && seen ? attn_page(a, s.b, j) : 0;
+            const int page = PAGED && seen ? attn_page<KEYS>(a, s.b, j, shared) : 0;
             seen = seen && page >= 0;
             float t = -INFINITY;
             KeyRow row = {0, 0};
             if (seen) {
-                row = attn_key_row<PAGED>(a, s.b, page, j);
+                row = attn_key_row<PAGED>(a, s.b, page, j < shared ? j : j - shared);
                 float bias = 0.0f;
                 if (a.mask) {
                     const int64_t o = mo + (int64_t)j * a.mk;
@@ -110,7 +112,8 @@ __device__ __forceinline__ void attn_row(const AttnArgs& a, const AttnSeq& s, in
     }
 }
 
-template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a, int64_t rows) {
+template <int DT, int KEYS> __device__ __forceinline__ void attn_rows(const AttnArgs& a, int64_t rows) {
+    constexpr bool PAGED = KEYS != kDense;
     const int64_t step = (int64_t)gridDim.x * 4;
     for (int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); r < rows; r += step) {
         const int64_t t = r / a.Hq;
@@ -135,8 +138,16 @@ template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_rows
         i = (int)at;
         const int64_t yo = PAGED ? t * a.yt + h * a.yh : b * a.yb + i * a.yt + h * a.yh;
         float m, l;
-        attn_row<DT, PAGED>(a, s, h, i, 0, s.len, m, l, [&](int d, float v) { st_code<DT>(a.y, yo + d, v); });
+        attn_row<DT, KEYS>(a, s, h, i, 0, KEYS == kPrefixed ? 0x7FFFFFFF : s.len, m, l, [&](int d, float v) { st_code<DT>(a.y, yo + d, v); });
     }
+}
+
+template <int DT, bool PAGED> __global__ __launch_bounds__(256) void k_attn_rows(AttnArgs a, int64_t rows) {
+    attn_rows<DT, PAGED ? kPaged : kDense>(a, rows);
+}
+// Behind a shared prefix, in one pass over both.
+template <int DT> __global__ __launch_bounds__(256) void k_prefix_rows(AttnArgs a, int64_t rows) {
+    attn_rows<DT, kPrefixed>(a, rows);
 }
 
 // ---- tiles on the matrix cores ------------------------------------------------------
@@ -292,7 +303,7 @@ template <int DT> constexpr float kLower = DT == kF16 ? 0x1p-6f : 1.0f;        /
 // (The slots of a sequence, one more than its whole tiles may need, follow from the starts
 // alone, so no list of tiles has to be made.)  64 sequences are tried at a time.
 template <int BM> __device__ __forceinline__ int64_t slot_base(const AttnArgs& a, int b) {
-    int64_t t0 = a.qstart[b];
+    int64_t t0 = a.qstart[b * a.qstep];
     t0 = t0 < 0 ? 0 : t0 > a.T ? a.T : t0;
     return t0 * a.G / BM + b;
 }
@@ -300,7 +311,7 @@ template <int BM> __device__ __forceinline__ AttnSeq slot_sequence(const AttnArg
     int lo = 0, n = a.B;                       // the answer is in [lo, lo + n)
     const int lane = (int)(threadIdx.x & 63);
     if (n < 64) {                              // all starts in one load
-        const int64_t v = a.qstart[min(lane, n)];
+        const int64_t v = a.qstart[min(lane, n) * a.qstep];
         const int start = (int)(v < 0 ? 0 : v > a.T ? a.T : v);
         const bool le = lane < n && (int64_t)start * a.G / BM + lane <= t;
         const int b = max(0, (int)__popcll(__ballot(le)) - 1);
@@ -683,7 +694,7 @@ template <int DT, int D, bool PAGED, bool MASK, int MR, bool EARLY> struct AttnW
         permlane_pair<32>(l, la, lb);
         l = la + lb;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const bool parts = a.nsplit > 1;
+        const bool parts = a.parts;
         // (no weight although a key was seen: the scores are past what float32 holds in log2 units)
         bool bad = again || (l == 0.0f && m > -INFINITY);
 #pragma unroll
@@ -1111,21 +1122,24 @@ template <int DT, int D, bool PAGED, bool MASK> void launch_tiles_of(const AttnA
     else if constexpr (kElem<DT> == 2 && D <= 128) hipLaunchKernelGGL((k_attn_tiles<DT, D, PAGED, MASK, 8, kKeys256>), dim3(p.blocks), dim3(512), 0, s, a);
 }
 template <int DT, int D> void launch_tiles_d(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
-    if (p.paged) launch_tiles_of<DT, D, true, false>(a, p, s);
+    if (p.keys == kPaged) launch_tiles_of<DT, D, true, false>(a, p, s);
     else if (a.mask) launch_tiles_of<DT, D, false, true>(a, p, s);
     else launch_tiles_of<DT, D, false, false>(a, p, s);
 }
 template <int DT> void launch_attention(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
+    const bool paged = p.keys != kDense;
     if (!p.d) {
         const unsigned grid = grid_for((size_t)a.rows, 4, 1u << 20);
-        if (p.paged) hipLaunchKernelGGL((k_attn_rows<DT, true>), dim3(grid), dim3(256), 0, s, a, a.rows);
+        if (p.keys == kPrefixed) hipLaunchKernelGGL((k_prefix_rows<DT>), dim3(grid), dim3(256), 0, s, a, a.rows);
+        else if (paged) hipLaunchKernelGGL((k_attn_rows<DT, true>), dim3(grid), dim3(256), 0, s, a, a.rows);
         else hipLaunchKernelGGL((k_attn_rows<DT, false>), dim3(grid), dim3(256), 0, s, a, a.rows);
         return;
     }
-    if (p.d == 64) launch_tiles_d<DT, 64>(a, p, s);
+    if (!p.blocks) {}
+    else if (p.d == 64) launch_tiles_d<DT, 64>(a, p, s);
     else if (p.d == 128) launch_tiles_d<DT, 128>(a, p, s);
     else launch_tiles_d<DT, 256>(a, p, s);
-    if (a.nsplit > 1) {
+    if (p.join && a.nsplit > 1) {
         const int lanes = a.Dv <= 64 ? 16 : a.Dv <= 128 ? 32 : 64;
         if (a.rows > 4096 && a.rows <= (1 << 24) && a.nsplit <= lanes) {
             const dim3 grid((unsigned)((a.rows + 256 / lanes - 1) / (256 / lanes)));
@@ -1135,12 +1149,12 @@ template <int DT> void launch_attention(const AttnArgs& a, const AttnPlan& p, hi
                 else if (lanes == 32) hipLaunchKernelGGL((k_attn_join_rows<DT, P, 32>), grid, dim3(256), 0, s, a);
                 else hipLaunchKernelGGL((k_attn_join_rows<DT, P, 64>), grid, dim3(256), 0, s, a);
             };
-            if (p.paged) join(std::true_type());
+            if (paged) join(std::true_type());
             else join(std::false_type());
             return;
         }
         const unsigned grid = grid_for((size_t)a.rows, 4, 1u << 20);
-        if (p.paged) hipLaunchKernelGGL((k_attn_join<DT, true>), dim3(grid), dim3(256), 0, s, a);
+        if (paged) hipLaunchKernelGGL((k_attn_join<DT, true>), dim3(grid), dim3(256), 0, s, a);
         else hipLaunchKernelGGL((k_attn_join<DT, false>), dim3(grid), dim3(256), 0, s, a);
     }
 }

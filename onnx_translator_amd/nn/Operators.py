@@ -26,7 +26,8 @@ from . import DTYPE_MAP, DTYPE_TO_NUMPY, DeviceArray, Ops, Tensor, Tensor_, PT
 __all__ = ["CConvParams", "CPoolParams", "CReduceParams", "RELU", "COS", "ABS", "ADD", "SUB", "MUL", "DIV",
            "QuantizeLinear", "DequantizeLinear", "Conv", "MaxPool", "Gemm", "Softmax", "Flatten", "Reshape",
            "GlobalAveragePool", "DynamicQuantizeLinear", "ElementwiseChain", "CChainStep", "CAttentionParams",
-           "CCacheAttentionParams", "CQKNormRotaryParams", "Attention", "CacheAttention", "QKNormRotary"]
+           "CCacheAttentionParams", "CQKNormRotaryParams", "Attention", "CacheAttention", "QKNormRotary",
+           "CPrefixAttentionParams", "CCachePlanParams", "CSampleParams", "PrefixCacheAttention", "CachePlan", "Sample"]
 
 
 class CConvParams(ctypes.Structure):
@@ -905,6 +906,21 @@ class CQKNormRotaryParams(ctypes.Structure):
                 ("interleaved", ctypes.c_int)]
 
 
+class CPrefixAttentionParams(ctypes.Structure):
+    """``PrefixAttentionParams`` of include/tensor_ops.h."""
+    _fields_ = [("scale", ctypes.c_float), ("max_prefix", ctypes.c_int), ("max_kv", ctypes.c_int)]
+
+
+class CCachePlanParams(ctypes.Structure):
+    """``CachePlanParams`` of include/tensor_ops.h."""
+    _fields_ = [("page_size", ctypes.c_int)]
+
+
+class CSampleParams(ctypes.Structure):
+    """``SampleParams`` of include/tensor_ops.h."""
+    _fields_ = [("vocab", ctypes.c_int)]
+
+
 class Attention(Ops):
     """softmax(scale Q K' + mask) V per head (``attention_forward``): the ONNX Attention
     operator without a past, for keys and values of any length (an encoder's states, say).
@@ -1045,3 +1061,104 @@ class QKNormRotary(Ops):
         if slots is not None:
             shapes[1:] = [tuple(key_cache.size), tuple(value_cache.size)]
         return _values(self, [Tensor_(*s, dtype=dt) for s in shapes])
+
+
+class PrefixCacheAttention(Ops):
+    """:class:`CacheAttention` for sequences that share a prefix, read once for all of them
+    (``prefix_cache_attention_forward``).
+
+    ``forward(q, key_cache, value_cache, prefix_pages, prefix_len, pages, q_start, kv_len)``:
+    prefix_pages [n] names the prefix's pages in order, prefix_len (one number) its keys; pages and
+    kv_len are the sequences' own, without the prefix.  A token sees the whole prefix and its
+    sequence's keys up to its own.  ``max_prefix`` and ``max_kv`` tell the launches the longest that
+    the caller expects.  Device tensors only."""
+
+    def __init__(self, inputs, outputs, scale=None, max_prefix=0, max_kv=0, dtype=None, version="1"):
+        super().__init__(inputs, outputs)
+        self.scale, self.max_prefix, self.max_kv = scale, int(max_prefix), int(max_kv)
+        self.dtype = dtype
+        self.version = version
+
+    def forward(self, q: Tensor, key_cache: Tensor, value_cache: Tensor, prefix_pages: Tensor, prefix_len: Tensor,
+                pages: Tensor, q_start: Tensor, kv_len: Tensor, workspace: Tensor = None):
+        _on_device("PrefixCacheAttention", q=q, key_cache=key_cache, value_cache=value_cache,
+                   prefix_pages=prefix_pages, prefix_len=prefix_len, pages=pages, q_start=q_start, kv_len=kv_len,
+                   workspace=workspace)
+        p = CPrefixAttentionParams(_scale(self.scale), self.max_prefix, self.max_kv)
+
+        def arrange(ins, out):
+            return (*ins[:8], out, ctypes.byref(p), ins[8])
+        t = self._run("prefix_cache_attention_forward",
+                      [q, key_cache, value_cache, prefix_pages, prefix_len, pages, q_start, kv_len, workspace],
+                      tuple(q.size[:2]) + (value_cache.size[3],), self.dtype or q.dtype, arrange=arrange)
+        return _values(self, t)
+
+    def forward_(self, q: Tensor_, key_cache: Tensor_, value_cache: Tensor_, *rest):
+        return _values(self, Tensor_(*(tuple(q.size[:2]) + (value_cache.size[3],)), dtype=self.dtype or q.dtype))
+
+
+class CachePlan(Ops):
+    """What a step's requests need of a paged cache, from their lengths (``cache_plan_forward``).
+
+    ``forward(new, past, state, pages, free, tokens, offset)``: request b has past[b] tokens in the
+    cache and brings new[b] more, or has ended (new[b] < 0); pages [requests, n] is the table, free
+    a ring of free page numbers and state (int64 [3]: pages ever taken, ever given back, requests
+    refused) its ends.  Table, ring and state are updated in place.  Gives [q_start, kv_len,
+    positions, slots] of ``dtype``, the last two for ``tokens`` rows (-1 behind the last request
+    and for refused ones): what :class:`QKNormRotary` and :class:`CacheAttention` take.  Positions
+    begin at ``offset`` (one number; a shared prefix).  Device tensors only."""
+
+    def __init__(self, inputs, outputs, page_size, dtype="int32", version="1"):
+        super().__init__(inputs, outputs)
+        self.page_size = int(page_size)
+        self.dtype = dtype
+        self.version = version
+
+    def _shapes(self, new, tokens):
+        return [(new.size[0] + 1,), (new.size[0],), (int(tokens),), (int(tokens),)]
+
+    def forward(self, new: Tensor, past: Tensor, state: Tensor, pages: Tensor, free: Tensor, tokens,
+                offset: Tensor = None):
+        _on_device("CachePlan", new=new, past=past, state=state, pages=pages, free=free, offset=offset)
+        outs = [Tensor(*s, dtype=self.dtype, data=DeviceArray(self.lib, s, self.dtype, zero=False))
+                for s in self._shapes(new, tokens)]
+        p = CCachePlanParams(self.page_size)
+        ins = [t.data.ptr if t is not None else PT() for t in (new, past, offset, state, pages, free)]
+        self._call("cache_plan_forward", *ins, *[t.data.ptr for t in outs], state.data.ptr, ctypes.byref(p))
+        return _values(self, outs)
+
+    def forward_(self, new: Tensor_, past=None, state=None, pages=None, free=None, tokens=0, offset=None):
+        return _values(self, [Tensor_(*s, dtype=self.dtype) for s in self._shapes(new, tokens)])
+
+
+class Sample(Ops):
+    """A token per row of logits from given random numbers (``sample_forward``).
+
+    ``forward(logits, uniform, temperature, top_k, top_p, min_p)``: logits [rows, columns], uniform
+    [rows] in [0, 1), the settings [rows] each or None (temperature 1, no filter); a temperature of
+    0 takes the largest logit.  The k largest logits are kept, of those the ones whose larger ones
+    weigh less than p of all those, and of these the ones of at least min_p times the largest
+    weight; equal logits rank by index.  Gives [token (``dtype``), logprob (float32)], both [rows].
+    ``vocab`` restricts the draw to the first columns.  Device tensors only."""
+
+    def __init__(self, inputs, outputs, vocab=0, dtype="int32", version="1"):
+        super().__init__(inputs, outputs)
+        self.vocab = int(vocab)
+        self.dtype = dtype
+        self.version = version
+
+    def forward(self, logits: Tensor, uniform: Tensor, temperature: Tensor = None, top_k: Tensor = None,
+                top_p: Tensor = None, min_p: Tensor = None, workspace: Tensor = None):
+        _on_device("Sample", logits=logits, uniform=uniform, temperature=temperature, top_k=top_k, top_p=top_p,
+                   min_p=min_p, workspace=workspace)
+        rows = (logits.size[0],)
+        outs = [Tensor(*rows, dtype=dt, data=DeviceArray(self.lib, rows, dt, zero=False))
+                for dt in (self.dtype, "float32")]
+        p = CSampleParams(self.vocab)
+        ins = [t.data.ptr if t is not None else PT() for t in (logits, uniform, temperature, top_k, top_p, min_p)]
+        self._call("sample_forward", *ins, *[t.data.ptr for t in outs], ctypes.byref(p),
+                   workspace.data.ptr if workspace is not None else PT())
+        return _values(self, outs)
+
+    def forward_(self, logits: Tensor_, *rest):
+        return _values(self, [Tensor_(logits.size[0], dtype=dt) for dt in (self.dtype, "float32")])

@@ -232,6 +232,9 @@ class Ops:
                     _sig(lib, "attention_forward", None, [P] * 6 + [V, P])
                     _sig(lib, "cache_attention_forward", None, [P] * 7 + [V, P])
                     _sig(lib, "qk_norm_rotary_forward", None, [P] * 10 + [V])
+                    _sig(lib, "prefix_cache_attention_forward", None, [P] * 9 + [V, P])
+                    _sig(lib, "cache_plan_forward", None, [P] * 11 + [V])
+                    _sig(lib, "sample_forward", None, [P] * 8 + [V, P])
                     lib.init_cos_lut()
                     cls._lib = lib
                     cls._lib_initialized = True

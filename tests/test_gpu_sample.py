@@ -1,0 +1,218 @@
+"""sample_forward on the GPU against a float64 restatement (tests/decode_ref.py)."""
+import math
+
+import numpy as np
+import pytest
+
+from tests.decode_ref import SampleProblem
+
+pytestmark = pytest.mark.gpu
+
+TYPES = ("float16", "bfloat16", "float32")
+FILTERS = {"none": {}, "k": dict(k=20), "k1": dict(k=1), "p": dict(p=0.8), "m": dict(m=0.05), "kp": dict(k=40, p=0.9),
+           "kpm": dict(k=50, p=0.95, m=0.02), "pm": dict(p=0.7, m=0.1)}
+
+
+def logits(rows, v, seed=0, std=2.0, tall=8):
+    """A bulk, and a few that stand out."""
+    rng = np.random.default_rng(seed)
+    x = rng.normal(0, std, (rows, v))
+    for r in range(rows):
+        at = rng.integers(0, v, min(tall, v))
+        x[r, at] += rng.uniform(0, 12, len(at))
+    return x, rng.random(rows).astype(np.float32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("filters", list(FILTERS))
+@pytest.mark.parametrize("v", [1, 2, 7, 100, 1000, 8191, 8192, 8193, 32003])
+def test_filters(hip, v, filters, dtype):
+    x, u = logits(5, v, seed=v)
+    SampleProblem(x, u, dtype, t=[1.0, 0.7, 1.3, 0.3, 2.0], **FILTERS[filters]).check(hip)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("filters", ["none", "p", "kp"])
+@pytest.mark.parametrize("v", [50021, 131072, 262144])
+def test_large_vocabularies(hip, v, filters, dtype):
+    x, u = logits(3, v, seed=v)
+    SampleProblem(x, u, dtype, t=[1.0, 0.6, 1.5], **FILTERS[filters]).check(hip)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_flat_rows(hip, dtype):
+    """Nothing stands out: top-p keeps tens of thousands, top-k thousands."""
+    x, u = logits(6, 40000, tall=0, std=0.5)
+    SampleProblem(x, u, dtype, p=[0.5, 0.9, 0.99, 0.999, 0.2, 0.01], t=1.0).check(hip)
+    SampleProblem(x, u, dtype, k=[4000, 4096, 4097, 5000, 20000, 39999]).check(hip)
+    SampleProblem(x, u, dtype, k=[4000, 20000, 30000, 39999, 40000, 50000], p=[0.9, 0.95, 0.5, 0.99, 0.3, 0.999]).check(hip)
+    SampleProblem(x, u, dtype, m=[0.001, 0.01, 0.1, 0.2, 0.3, 0.9]).check(hip)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [10, 5000, 20011])
+def test_equal_logits(hip, v, dtype):
+    """Ties rank by index, at the top-k and the top-p border alike."""
+    rng = np.random.default_rng(v)
+    x = rng.integers(-2, 3, (8, v)).astype(np.float64)
+    x[0] = 1.0
+    u = rng.random(8).astype(np.float32)
+    SampleProblem(x, u, dtype, k=[3, 3, 1, 2, v // 2, v // 3, v - 1, v]).check(hip)
+    SampleProblem(x, u, dtype, p=[0.313, 0.771, 0.2077, 0.55, 0.931, 0.1017, 0.0501, 0.99]).check(hip)
+    SampleProblem(x, u, dtype, k=[5, 9, v // 2, v // 2, v // 4, v // 4, v - 1, v], p=[0.313, 0.771, 0.2077, 0.55, 0.931, 0.1017, 0.6001, 0.97]).check(hip)
+
+
+def test_both_zeros_are_equal(hip):
+    x = np.array([[-1.0, -0.0, 0.0, -0.0, 0.0]])
+    for k, may in ((1, {1}), (2, {1, 2}), (3, {1, 2, 3})):
+        seen = set()
+        for u in np.linspace(0, 0.999, 13):
+            tokens, _ = SampleProblem(x, [u], k=k).check(hip)
+            seen.add(int(tokens[0]))
+        assert seen == may
+    assert SampleProblem(x, [0.5], t=0.0).check(hip)[0][0] == 1
+
+
+@pytest.mark.parametrize("t", [0.0, -1.0, math.nan])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_greedy(hip, dtype, t):
+    x, u = logits(6, 9000, seed=3)
+    x[1, [70, 8500]] = 40.0                          # equal: the first
+    x[2, 8999] = 50.0
+    x[3, 0] = 50.0
+    tokens, lps = SampleProblem(x, u, dtype, t=t, k=5, p=0.5, m=0.1).check(hip)
+    assert tokens[1:4].tolist() == [70, 8999, 0] and not lps.any()
+
+
+@pytest.mark.parametrize("t", [1e-30, 1e-3, 50.0, 1e30, math.inf])
+def test_temperatures(hip, t):
+    x, u = logits(4, 3001, seed=4)
+    SampleProblem(x, u, t=t).check(hip)
+    SampleProblem(x, u, t=t, k=17).check(hip)
+    SampleProblem(x, u, t=t, p=0.8317).check(hip)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("filters", list(FILTERS))
+def test_masked_logits(hip, dtype, filters):
+    """-inf and NaN are never drawn; a row of nothing else gives -1."""
+    x, u = logits(6, 5003, seed=5)
+    rng = np.random.default_rng(6)
+    x[0, rng.random(5003) < 0.9] = -np.inf
+    x[1] = -np.inf
+    x[2] = np.nan
+    x[3] = -np.inf
+    x[3, 4321] = -3.0                                # one left
+    x[4, rng.random(5003) < 0.5] = np.nan
+    x[5, :5000] = -np.inf
+    u[:] = [0.999, 0.5, 0.5, 0.9, 0.99, 0.9]
+    tokens, lps = SampleProblem(x, u, dtype, t=[1.0, 1.0, 0.0, 0.7, 1.0, 1.0], **FILTERS[filters]).check(hip)
+    assert tokens[1] == tokens[2] == -1 and lps[1] == lps[2] == -np.inf and tokens[3] == 4321 and tokens[5] >= 5000
+    assert SampleProblem(x, u, dtype, t=0.0).check(hip)[0][[1, 2, 3]].tolist() == [-1, -1, 4321]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_infinite_logits(hip, dtype):
+    """+inf takes everything, several share alike."""
+    x, u = logits(4, 2000, seed=7)
+    x[:, [17, 900, 1500]] = np.inf
+    for u0, want in ((0.0, 17), (0.4, 900), (0.9, 1500)):
+        u[:] = u0
+        for f in ({}, dict(p=0.99), dict(m=0.3), dict(k=3)):
+            assert (SampleProblem(x, u, dtype, **f).check(hip)[0] == want).all()
+        assert (SampleProblem(x, u, dtype, k=1).check(hip)[0] == 17).all()
+    low = np.full((2, 50), float(np.finfo(np.float16).min) if dtype == "float16" else -3e38)
+    SampleProblem(low, [0.3, 0.9], dtype, p=[1.0, 0.517]).check(hip)
+
+
+@pytest.mark.parametrize("u_type", ["float32", "float64"])
+def test_uniform_numbers_outside(hip, u_type):
+    """Below 0 (or NaN) the first kept token, 1 or more the last."""
+    x, _ = logits(1, 500, seed=8)
+    kept = np.sort(np.argsort(-x[0])[:10])
+    for u, want in ((0.0, kept[0]), (-1.0, kept[0]), (-math.inf, kept[0]), (math.nan, kept[0]), (1.0, kept[-1]), (7.0, kept[-1]), (math.inf, kept[-1])):
+        got = SampleProblem(x, [u], k=10, t=5.0, u_type=u_type).run(hip)[0]
+        assert got[0] == want, u
+
+
+def test_settings_out_of_range(hip):
+    """k below 1: all; p of 0 or less: the largest alone; p of 1 and more, NaN: all; m above 1: the largest."""
+    x, u = logits(6, 3000, seed=9)
+    SampleProblem(x, u, k=[0, -5, 3000, 3001, 1 << 30, 2]).check(hip)
+    tokens, _ = SampleProblem(x, u, p=[0.0, -1.0, -math.inf, 1.0, 3.0, math.nan]).check(hip)
+    assert (tokens[:3] == x[:3].argmax(1)).all()
+    tokens, _ = SampleProblem(x, u, m=[1.0, 2.0, math.inf, 0.0, -1.0, math.nan]).check(hip)
+    assert (tokens[:3] == x[:3].argmax(1)).all()
+    SampleProblem(x, u, k=np.full(6, 1 << 40)).check(hip, index="int64")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("columns,vocab", [(100, 99), (1001, 1), (9000, 8191), (8200, 8199)])
+def test_part_of_the_columns(hip, dtype, columns, vocab):
+    """Columns behind the vocabulary are no tokens, whatever they hold."""
+    x, u = logits(4, columns, seed=columns)
+    x[:, vocab:] = [[np.nan], [np.inf], [1e4], [-np.inf]]
+    for f in ({}, dict(k=3), dict(p=0.5), dict(t=0.0)):
+        SampleProblem(x, u, dtype, vocab=vocab, **f).check(hip)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 255, 256, 257, 600])
+def test_rows(hip, rows):
+    x, u = logits(rows, 701, seed=rows)
+    rng = np.random.default_rng(rows)
+    SampleProblem(x, u, "float16", t=rng.uniform(0.3, 1.5, rows) * (rng.random(rows) < 0.9), k=rng.integers(0, 60, rows),
+                  p=rng.uniform(0.3, 1.2, rows), m=rng.uniform(0, 0.1, rows)).check(hip)
+
+
+def test_types_and_absent_results(hip):
+    x, u = logits(4, 900, seed=11)
+    p = SampleProblem(x, u, k=[3, 0, 9, 1], u_type="float64")
+    a = p.check(hip, token="int64", index="int64")
+    b = p.check(hip, logprob=False)
+    assert (a[0] == b[0]).all()
+
+
+def test_logits_off_their_alignment(hip):
+    """Rows that begin in the middle of a 16-byte chunk, and a tensor that does."""
+    import ctypes
+    import torch
+    from oracle import oracle as O
+    from onnx_translator_amd.nn.Operators import CSampleParams
+    from tests.decode_ref import Dev
+    for dtype, code in ((torch.float16, O.F16), (torch.bfloat16, O.BF16), (torch.float32, O.F32)):
+        name = str(dtype).replace("torch.", "")
+        for v, skip in ((997, 0), (997, 1), (8193, 3), (20001, 5)):
+            x, u = logits(3, v, seed=v + skip)
+            p = SampleProblem(x, u, name, k=[0, 30, 7], p=[0.9, 1.0, 0.8])
+            flat = torch.full((skip + 3 * v,), float("inf"), dtype=dtype, device="cuda")
+            flat[skip:] = p.x.cuda().reshape(-1)
+            torch.cuda.synchronize()
+            with Dev(hip) as dev:
+                xt = hip.lib.tensor_wrap_device(ctypes.c_void_p(flat.data_ptr() + skip * flat.element_size()), (ctypes.c_int * 2)(3, v), 2, code)
+                out = dev.put(np.zeros(3, np.int32))
+                dev.call("sample_forward", xt, dev.put(p.u), O.PT(), dev.put(p.k), dev.put(p.p), O.PT(), out, O.PT(),
+                         ctypes.byref(CSampleParams(0)), O.PT())
+                got = hip.dev_read(out, O.I32)
+                dev.held.append(xt)
+            assert (got == p.run(hip)[0]).all(), (name, v, skip)
+            p.check(hip)
+
+
+def test_the_distribution(hip):
+    """Evenly spaced numbers draw each token as often as its probability says (within one)."""
+    n = 4000
+    x = np.broadcast_to(np.log([0.5, 0.2, 0.05, 0.15, 0.1]), (n, 5)).copy()
+    u = ((np.arange(n) + 0.5) / n).astype(np.float32)
+    for f, p in (({}, [0.5, 0.2, 0.05, 0.15, 0.1]), (dict(k=3), np.array([0.5, 0.2, 0, 0.15, 0]) / 0.85),
+                 (dict(p=0.6), np.array([0.5, 0.2, 0, 0, 0]) / 0.7), (dict(m=0.25), np.array([0.5, 0.2, 0, 0.15, 0]) / 0.85)):
+        tokens, _ = SampleProblem(x, u, **f).run(hip)
+        assert np.abs(np.bincount(tokens, minlength=5) - n * np.array(p)).max() <= 1
+
+
+def test_repeatable(hip):
+    x, u = logits(64, 50000, seed=12, tall=2)
+    p = SampleProblem(x, u, "float16", p=0.97)
+    a = p.run(hip)
+    for _ in range(5):
+        b = p.run(hip)
+        assert (a[0] == b[0]).all() and (a[1] == b[1]).all()
