@@ -489,10 +489,12 @@ typedef struct {
  * was drawn (0 for a greedy row, -inf for Token -1).  Sums of weights are kept in 64-bit fixed
  * point, at least 2^-44 of the largest weight for up to 2^18 columns, in which their order does
  * not matter: the same call gives the same token.
- *   Workspace (may be NULL): device memory of any type, 16-byte aligned, that lets a call spread
- * a row over the GPU: sample_workspace_bytes(rows, columns) bytes.  Without one an eager call takes them from the
- * library's pool; a call captured into a graph keeps each row on one compute unit, which is
- * slower where rows are few and long.  Calls that may overlap must not share one. */
+ *   Workspace (may be NULL): device memory of any type, 16-byte aligned, with which a call
+ * spreads long rows over the GPU: sample_workspace_bytes(rows, tokens) bytes, 0 where a call of
+ * that size needs none.  Without one an eager call takes them from the library's pool; a call
+ * captured into a graph keeps each row on one compute unit, which is slower.  Calls that may
+ * overlap must not share one. */
+size_t sample_workspace_bytes(int rows, int columns);
 void sample_forward(const Tensor* Logits, const Tensor* Uniform, const Tensor* Temperature, const Tensor* TopK,
                     const Tensor* TopP, const Tensor* MinP, Tensor* Token, Tensor* LogProb,
                     const SampleParams* params, Tensor* Workspace);

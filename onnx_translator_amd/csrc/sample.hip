@@ -15,7 +15,9 @@
 #include "attention.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 namespace tohip {
 namespace {
@@ -34,237 +36,535 @@ struct SampleArgs {
 typedef unsigned long long u64;
 
 // ---- one weight ------------------------------------------------------------------------
-// Order-preserving key of a logit: NaN as -inf, -0 as +0.
+// Order-preserving key of a logit that is no NaN: -0 as +0.
 __device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t b = f2u(x + 0.0f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return u2f(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
+// Value and index as one number: larger for larger values, and of equal ones for lower indices.
+__device__ __forceinline__ u64 rank_of(float x, int i) { return ((u64)key_of(x) << 32) | (uint32_t)~i; }
+__device__ __forceinline__ int index_of(u64 rank) { return (int)~(uint32_t)rank; }
+__device__ __forceinline__ float value_of(u64 rank) { return of_key((uint32_t)(rank >> 32)); }
 
-// log2 of x's weight against the row's largest value (x <= top; equal infinities weigh 1).
-__device__ __forceinline__ double log2_weight(float x, float top, double per) {
-    return x == top ? 0.0 : x == -INFINITY || top == INFINITY ? -INFINITY : ((double)x - (double)top) * per;
-}
-// 2^y for y <= 0: 2^f by its Taylor series, |f| <= 1/2 (12 terms: 2^-52 of the result).
-__device__ __forceinline__ double pow2(double y) {
-    const double n = __builtin_rint(y), f = y - n;
-    double p = 2.5678435993488206e-11;                // ln2^12 / 12!, ...
-    p = __builtin_fma(p, f, 4.4455382718708116e-10);
-    p = __builtin_fma(p, f, 7.054911620801123e-09);
-    p = __builtin_fma(p, f, 1.01780860092397e-07);
-    p = __builtin_fma(p, f, 1.321548679014431e-06);
-    p = __builtin_fma(p, f, 1.5252733804059841e-05);
-    p = __builtin_fma(p, f, 0.0001540353039338161);
-    p = __builtin_fma(p, f, 0.0013333558146428443);
-    p = __builtin_fma(p, f, 0.009618129107628477);
-    p = __builtin_fma(p, f, 0.05550410866482158);
-    p = __builtin_fma(p, f, 0.24022650695910072);
-    p = __builtin_fma(p, f, 0.6931471805599453);
-    p = __builtin_fma(p, f, 1.0);
-    return __builtin_ldexp(p, (int)n);
-}
-// The weight 2^y in whole numbers of 2^-shift (shift <= 51), rounded to the nearest: the low bits
-// of the sum with 2^52.
-__device__ __forceinline__ u64 fixed_weight(double y, int shift) {
-    if (!(y >= -54.0)) return 0;
-    const double v = __builtin_ldexp(pow2(y), shift) + 0x1p52;
-    return __builtin_bit_cast(u64, v) & 0xFFFFFFFFFFFFFull;
-}
+// A logit as a number whose differences are numbers too: +inf as one beyond all others.
+__device__ __forceinline__ double finite(float x) { return __builtin_fmin((double)x, 1e300); }
 
-// ---- a block's sums ---------------------------------------------------------------------
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kEach = 8;                               // logits of a thread in a tile, in index order
-constexpr int kTile = kThreads * kEach;
-constexpr int kBins = 2048, kMaxTiles = 2048;          // (16 M columns)
+// Against the largest of some logits: weights 2^((x - top) per).
+struct Weights {
+    double top, per;
+    int shift;                         // in whole numbers of 2^-shift, at most 51
 
-__device__ __forceinline__ u64 shfl_up64(u64 v, int o) { return (u64)__shfl_up((long long)v, o); }
-
-// Sums of all threads before this one, and of all.
-__device__ __forceinline__ u64 scan_before(u64 v, u64* waves, u64& total) {
-    const int lane = (int)threadIdx.x & 63, w = (int)threadIdx.x >> 6;
-    u64 s = v;
+    // log2 of the weight, -100 for what weighs nothing in 64 bits (-inf among it)
+    __device__ __forceinline__ double log2_of(float x) const { return __builtin_fmax((finite(x) - top) * per, -100.0); }
+    // 2^y for -100 <= y <= 0, as the bits of 2^52 + the weight rounded to the nearest whole number:
+    // the polynomial through 2^f at the eleven Chebyshev points of |f| <= 1/2 (off by 2^-51.6 of
+    // itself), with whole part and shift put into its exponent.  Without a branch, and the factors
+    // as scalars: else each costs two moves, more than the product.
+    __device__ __forceinline__ u64 bits(double y) const {
+        constexpr double kC[11] = {1.0, 0.69314718055995, 0.24022650695910097, 0.05550410866444772, 0.009618129107606888,
+                                   0.0013333558230164974, 0.0001540353044173605, 1.5252657260200837e-05,
+                                   1.321544258792169e-06, 1.0208690299958306e-07, 7.072585949269223e-09};
+        const double n = y + 0x1.8p52, f = y - (n - 0x1.8p52);      // (n's low bits: the whole part)
+        double v = kC[10];
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const u64 x = shfl_up64(s, o);
-        if (lane >= o) s += x;
-    }
-    __syncthreads();                                   // (the last call's are read)
-    if (lane == 63) waves[w] = s;
-    __syncthreads();
-    u64 before = 0;
-    total = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; i++) {
-        const u64 x = waves[i];
-        before += i < w ? x : 0;
-        total += x;
-    }
-    return before + s - v;
-}
-
-struct SampleShared {
-    u64 waves[kWaves];
-    u64 bins[kBins];
-    u64 tile_mass[kMaxTiles];
-    uint32_t tile_ties[kMaxTiles];
-    u64 found[3];
-};
-
-// The bin, from the highest down, in which the sums pass `want` (1 <= want <= the sum of all): the
-// bin and the sum of the bins above it.
-__device__ __forceinline__ void pick_bin(SampleShared& s, u64 want, int& bin, u64& above) {
-    const int hi = kBins - 1 - 2 * (int)threadIdx.x;
-    const u64 a = s.bins[hi], b = s.bins[hi - 1];
-    u64 total;
-    const u64 before = scan_before(a + b, s.waves, total);
-    if (before < want && want <= before + a) { s.found[0] = (u64)hi; s.found[1] = before; }
-    else if (before + a < want && want <= before + a + b) { s.found[0] = (u64)hi - 1; s.found[1] = before + a; }
-    __syncthreads();
-    bin = (int)s.found[0];
-    above = s.found[1];
-}
-
-// ---- a row ---------------------------------------------------------------------------------
-// Tiles begin at the 16-byte chunk that holds the row's first logit; places outside the row give
-// -inf.
-template <int DT> struct SampleRow {
-    static constexpr int ES = DT == kF32 ? 4 : 2, VEC = 16 / ES;
-    const char* base;
-    int first, V, tiles;
-
-    __device__ __forceinline__ SampleRow(const SampleArgs& a, int64_t row) {
-        const uintptr_t p = (uintptr_t)a.x + (uintptr_t)(row * a.ld * ES);
-        base = (const char*)(p & ~(uintptr_t)15);
-        first = (int)((p & 15) / ES);
-        V = a.V;
-        tiles = (first + V + kTile - 1) / kTile;
-    }
-    __device__ __forceinline__ int index(int tile) const { return tile * kTile + (int)threadIdx.x * kEach - first; }
-    __device__ __forceinline__ void load(int tile, float (&x)[kEach]) const {
-        const int i0 = index(tile);
-#pragma unroll
-        for (int c = 0; c < kEach; c += VEC) {
-            const int i = i0 + c;
-            const char* p = base + (int64_t)(i + first) * ES;
-            if (i >= 0 && i + VEC <= V) {
-                const uint4 q = *reinterpret_cast<const uint4*>(p);
-                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if constexpr (DT == kF32) {
-                        x[c + e] = u2f(w[e]);
-                    } else if constexpr (DT == kBF16) {
-                        x[c + 2 * e] = u2f(w[e] << 16);
-                        x[c + 2 * e + 1] = u2f(w[e] & 0xFFFF0000u);
-                    } else {
-                        x[c + 2 * e] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
-                        x[c + 2 * e + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    x[c + e] = i + e >= 0 && i + e < V ? (float)ld_d<DT>(p, e) : -INFINITY;
-            }
+        for (int i = 9; i >= 0; i--) {
+            double c = kC[i];
+            asm("" : "+s"(c));
+            v = __builtin_fma(v, f, c);
         }
+        const u64 b = __builtin_bit_cast(u64, v);
+        const uint32_t hi = (uint32_t)(b >> 32) + (((uint32_t)__builtin_bit_cast(u64, n) + (uint32_t)shift) << 20);
+        return __builtin_bit_cast(u64, __builtin_bit_cast(double, ((u64)hi << 32) | (uint32_t)b) + 0x1p52);
+    }
+    static constexpr u64 kBias = 0x4330000000000000ull;              // 2^52's bits
+    __device__ __forceinline__ u64 of_log2(double y) const { return bits(y) - kBias; }
+    __device__ __forceinline__ u64 of(float x) const { return of_log2(log2_of(x)); }
+    template <int N> __device__ __forceinline__ u64 sum(const float (&x)[N]) const {
+        u64 s = 0;
 #pragma unroll
-        for (int e = 0; e < kEach; e++) x[e] = x[e] != x[e] ? -INFINITY : x[e];
+        for (int e = 0; e < N; e++) s += bits(log2_of(x[e]));
+        return s - (u64)N * kBias;
     }
 };
 
+// ---- sums ---------------------------------------------------------------------------------
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 lanes_before(u64 v) {      // (0 where there is none)
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xF, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xF, false);
+    return ((u64)hi << 32) | lo;
+}
+// Sums of the wave's lanes up to and with each.
+__device__ __forceinline__ u64 wave_scan(u64 v) {
+    v += lanes_before<0x111, 0xF>(v);                  // row_shr 1, 2, 4, 8: in rows of 16 lanes
+    v += lanes_before<0x112, 0xF>(v);
+    v += lanes_before<0x114, 0xF>(v);
+    v += lanes_before<0x118, 0xF>(v);
+    v += lanes_before<0x142, 0xA>(v);                  // lane 15 of the row before to rows 1 and 3
+    v += lanes_before<0x143, 0xC>(v);                  // lane 31 to rows 2 and 3
+    return v;
+}
+struct Add {
+    template <class T> __device__ __forceinline__ T operator()(T x, T y) const { return x + y; }
+};
+struct Max {
+    __device__ __forceinline__ float operator()(float x, float y) const { return fmaxf(x, y); }
+};
+struct Min {
+    __device__ __forceinline__ int operator()(int x, int y) const { return x < y ? x : y; }
+    __device__ __forceinline__ float operator()(float x, float y) const { return fminf(x, y); }
+};
+
+// Sums over a block of NT threads.  to: LDS of a number per wave.
+template <int NT> struct Block {
+    static constexpr int kWaves = NT / 64;
+    // Of all threads before this one, and of all.
+    static __device__ __forceinline__ u64 before(u64 v, u64* to, u64& total) {
+        const int lane = (int)threadIdx.x & 63, w = (int)threadIdx.x >> 6;
+        const u64 s = wave_scan(v);
+        __syncthreads();                               // (the last call's are read)
+        if (lane == 63) to[w] = s;
+        __syncthreads();
+        u64 b = 0;
+        total = 0;
+#pragma unroll
+        for (int i = 0; i < kWaves; i++) {
+            const u64 x = to[i];
+            b += i < w ? x : 0;
+            total += x;
+        }
+        return b + s - v;
+    }
+    template <class T, class OP> static __device__ __forceinline__ T reduce(T v, u64* waves, OP op) {
+        T* to = reinterpret_cast<T*>(waves);
+        v = wave_allreduce(v, op);
+        __syncthreads();
+        if (((int)threadIdx.x & 63) == 0) to[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = to[0];
+#pragma unroll
+        for (int i = 1; i < kWaves; i++) v = op(v, to[i]);
+        return v;
+    }
+};
+
+// ---- a row's settings ------------------------------------------------------------------------
+struct Settings {
+    double per, t, p, m;               // log2 e / t; m in [0, 1]
+    int64_t k;
+    bool greedy, by_k, by_p;
+
+    __device__ __forceinline__ Settings(const SampleArgs& a, int64_t row) {
+        t = a.temperature ? (double)a.temperature[row] : 1.0;
+        p = a.top_p ? (double)a.top_p[row] : 1.0;
+        const double low = a.min_p ? (double)a.min_p[row] : 0.0;
+        m = low >= 1.0 ? 1.0 : low > 0.0 ? low : 0.0;  // (NaN: 0)
+        k = a.top_k.p ? a.top_k[row] : 0;
+        greedy = !(t > 0.0);
+        by_k = k > 0 && k < a.V;
+        by_p = p < 1.0;
+        per = __builtin_fmax(1.4426950408889634 / t, 1e-60);      // (not 0: an infinite logit is beyond all others)
+    }
+    __device__ __forceinline__ bool filters() const { return by_k || by_p || m > 0.0; }
+    // The whole number that the weights before a kept value stay below, of `total`.
+    __device__ __forceinline__ u64 want(u64 total) const {
+        const double w = __builtin_ceil(p * (double)total);
+        return !(w >= 1.0) ? 1 : w >= (double)total ? total : (u64)w;
+    }
+    // 2^y (of a weight) against min-p, in double.
+    __device__ __forceinline__ bool passes(double y) const { return !(m > 0.0) || exp2(y) >= m; }
+    // A value that no logit passing min-p is below.
+    __device__ __forceinline__ float least(float top) const {
+        if (top == INFINITY) return top;
+        const double x = (double)top + t * log(m);
+        const float f = (float)(x - 1e-6 * __builtin_fabs(x) - 1e-30);
+        return f == f ? f : -INFINITY;
+    }
+};
+// The number below which the first of the kept weights, added up, are drawn.
+__device__ __forceinline__ u64 draw_target(const SampleArgs& a, int64_t row, u64 all) {
+    const double u = a.u64 ? ((const double*)a.u)[row] : (double)((const float*)a.u)[row];
+    const double at = u * (double)all;
+    const u64 target = !(at > 0.0) ? 0 : at >= (double)all ? all - 1 : (u64)at;
+    return target < all ? target : all - 1;
+}
 __device__ __forceinline__ void put_token(const SampleArgs& a, int64_t row, int64_t token, float logprob) {
     if (a.token64) ((int64_t*)a.token)[row] = token;
     else ((int32_t*)a.token)[row] = (int32_t)token;
     if (a.logprob) a.logprob[row] = logprob;
 }
+__device__ __forceinline__ void put_drawn(const SampleArgs& a, int64_t row, int token, double y, u64 all) {
+    put_token(a, row, token, (float)((y + (double)a.shift) * 0.6931471805599453 - log((double)all)));
+}
 
-// A block per row, any filters, any logits.
-template <int DT> __global__ __launch_bounds__(kThreads) void k_sample_row(SampleArgs a) {
-    __shared__ SampleShared s;
-    constexpr int kRounds = DT == kF32 ? 3 : 2;        // digits of 11, 11 and 10 bits; 16-bit logits differ in the first two
-    const int64_t row = blockIdx.x;
-    const int tid = (int)threadIdx.x;
-    const SampleRow<DT> r(a, row);
-    const double t = a.temperature ? (double)a.temperature[row] : 1.0;
-    const double p = a.top_p ? (double)a.top_p[row] : 1.0, m = a.min_p ? (double)a.min_p[row] : 0.0;
-    const int64_t k = a.top_k.p ? a.top_k[row] : 0;
+// ---- logits ----------------------------------------------------------------------------------
+// The logits of a row by 16-byte chunks from the one that holds its first on; -inf outside the row
+// and for NaN.
+template <int DT> struct RowChunks {
+    static constexpr int ES = DT == kF32 ? 4 : 2, VEC = 16 / ES;
+    const char* base;
+    int first, V;                                      // index 0 is place `first` of the chunk at base
 
-    // ---- the largest value, and where it is first: (key, ~index) as one number
-    u64 best = 0;
-    for (int tile = 0; tile < r.tiles; tile++) {
-        float x[kEach];
-        r.load(tile, x);
-        const int i = r.index(tile);
+    __device__ __forceinline__ RowChunks(const SampleArgs& a, int64_t row) {
+        const char* p = (const char*)a.x + row * a.ld * ES;
+        first = (int)((uintptr_t)p & 15) / ES;
+        base = p - first * ES;
+        V = a.V;
+    }
+    __device__ __forceinline__ uint4 whole(int i) const { return *reinterpret_cast<const uint4*>(base + (int64_t)(i + first) * ES); }
+    __device__ __forceinline__ uint4 part(int i) const {
+        const char* p = base + (int64_t)(i + first) * ES;
+        uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < kEach; e++) {
-            const u64 v = ((u64)key_of(x[e]) << 32) | (uint32_t)~(i + e);
-            best = x[e] > -INFINITY && v > best ? v : best;
+        for (int e = 0; e < 4; e++) {
+            if constexpr (DT == kF32) {
+                w[e] = i + e >= 0 && i + e < V ? ((const uint32_t*)p)[e] : 0xFF800000u;
+            } else {
+                constexpr uint32_t none = DT == kBF16 ? 0xFF80u : 0xFC00u;
+                const uint32_t lo = i + 2 * e >= 0 && i + 2 * e < V ? ((const uint16_t*)p)[2 * e] : none;
+                const uint32_t hi = i + 2 * e + 1 >= 0 && i + 2 * e + 1 < V ? ((const uint16_t*)p)[2 * e + 1] : none;
+                w[e] = lo | (hi << 16);
+            }
+        }
+        return uint4{w[0], w[1], w[2], w[3]};
+    }
+    // N chunks at at(0), at(1), ..., all of them between the indices lo and hi of a wave's (so that
+    // inside a row the loads go out together).
+    template <int N, class AT> __device__ __forceinline__ void chunks(int lo, int hi, AT at, uint4 (&q)[N]) const {
+        if (lo >= 0 && hi <= V) {
+#pragma unroll
+            for (int c = 0; c < N; c++) q[c] = whole(at(c));
+        } else {
+#pragma unroll
+            for (int c = 0; c < N; c++) q[c] = part(at(c));
         }
     }
+    static __device__ __forceinline__ void open(uint4 q, float* x) {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const u64 v = (u64)__shfl_xor((long long)best, o);
-        best = v > best ? v : best;
-    }
-    if ((tid & 63) == 0) s.waves[tid >> 6] = best;
-    __syncthreads();
-    best = 0;
+        for (int e = 0; e < 4; e++) {
+            if constexpr (DT == kF32) {
+                x[e] = u2f(w[e]);
+            } else if constexpr (DT == kBF16) {
+                x[2 * e] = u2f(w[e] << 16);
+                x[2 * e + 1] = u2f(w[e] & 0xFFFF0000u);
+            } else {
+                x[2 * e] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
+                x[2 * e + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
+            }
+        }
 #pragma unroll
-    for (int i = 0; i < kWaves; i++) best = s.waves[i] > best ? s.waves[i] : best;
-    if (best == 0) {
-        if (tid == 0) put_token(a, row, -1, -INFINITY);
-        return;
+        for (int e = 0; e < VEC; e++) x[e] = x[e] != x[e] ? -INFINITY : x[e];
     }
-    if (!(t > 0.0)) {
-        if (tid == 0) put_token(a, row, (int)~(uint32_t)best, 0.0f);
-        return;
-    }
-    const float top = of_key((uint32_t)(best >> 32));
-    const double per = 1.4426950408889634 / t;
-    auto weight = [&](float x) { return fixed_weight(log2_weight(x, top, per), a.shift); };
+};
 
-    // ---- the border: kept are keys above `border`, and the first `ties` equal to it
+// ---- few candidates --------------------------------------------------------------------------
+// Where the kept tokens are known to be among at most kMost candidates, these are ranked by value for
+// the filters and by index for the draw: up to kFew by counting the larger ones, which takes no
+// barrier between its reads (120 candidates: 2.4 us where a sort takes 5), more by sorting.
+constexpr int kMost = 2048, kFew = 256;
+
+template <int NT> struct Candidates {
+    u64 waves[Block<NT>::kWaves];
+    u64 rank[kMost], mass[kMost], order[kMost];
+    unsigned count;
+};
+
+// Adds the logits of a wave's lanes that are at least `least` to a list of at most `most` (every lane
+// calls); count goes on past it.
+__device__ __forceinline__ void add_candidate(u64* list, unsigned* count, unsigned most, bool in, float x, int i) {
+    const unsigned long long who = __ballot(in);
+    if (!who) return;
+    const int lane = (int)threadIdx.x & 63;
+    unsigned at = 0;
+    if (lane == __builtin_ctzll(who)) at = atomicAdd(count, (unsigned)__popcll(who));
+    at = (unsigned)__builtin_amdgcn_readlane((int)at, __builtin_ctzll(who)) + (unsigned)__popcll(who & ((1ull << lane) - 1));
+    if (in && at < most) list[at] = rank_of(x, i);
+}
+
+// n numbers in LDS, n a power of two, in falling order.
+template <int NT> __device__ __forceinline__ void sort_falling(u64* v, int n) {
+    for (int size = 2; size <= n; size *= 2) {
+        for (int step = size / 2; step > 0; step /= 2) {
+            __syncthreads();
+            for (int t = (int)threadIdx.x; t < n / 2; t += NT) {
+                const int i = 2 * t - (t & (step - 1)), j = i + step;
+                const u64 x = v[i], y = v[j];
+                if ((x < y) == ((i & size) == 0)) {
+                    v[i] = y;
+                    v[j] = x;
+                }
+            }
+        }
+    }
+    __syncthreads();
+}
+
+// Draws from the c.count <= kMost candidates of top-k or of min-p alone (they hold all that those keep).
+template <int NT> __device__ __forceinline__ void draw_candidates(const SampleArgs& a, int64_t row, const Settings& g, const Weights& w,
+                                                                  Candidates<NT>& c) {
+    const int tid = (int)threadIdx.x;
+    __syncthreads();
+    const int count = (int)c.count, most = g.by_k && g.k < count ? (int)g.k : count;
+    if (count <= kFew) {
+        // a candidate per thread; the larger ones and their weights, then the kept ones before it
+        const u64 mine = tid < count ? c.rank[tid] : 0;
+        const double y = mine ? w.log2_of(value_of(mine)) : -100.0;
+        const u64 own = mine ? w.of_log2(y) : 0;
+        if (tid < count) c.mass[tid] = own;
+        __syncthreads();
+        int larger = 0;
+        u64 above = 0;
+        if (tid < (count + 63) / 64 * 64) {
+#pragma unroll 4
+            for (int j = 0; j < count; j++) {
+                const bool l = c.rank[j] > mine;
+                larger += l;
+                above += l ? c.mass[j] : 0;
+            }
+        }
+        const bool ranked = mine && larger < most;
+        u64 total = 0;
+        if (g.by_p) total = Block<NT>::reduce(ranked ? own : 0, c.waves, Add());
+        const bool keep = ranked && (!g.by_p || above < g.want(total)) && g.passes(y);
+        if (tid < count) c.order[tid] = keep ? own : 0;
+        const u64 all = Block<NT>::reduce(keep ? own : 0, c.waves, Add());
+        const u64 target = draw_target(a, row, all);
+        u64 before = 0;
+        if (keep) {
+#pragma unroll 4
+            for (int j = 0; j < count; j++) before += (uint32_t)c.rank[j] > (uint32_t)mine ? c.order[j] : 0;      // (~index)
+            if (before <= target && target < before + own) put_drawn(a, row, index_of(mine), y, all);
+        }
+        return;
+    }
+    int n = 2 * kFew;
+    while (n < count) n *= 2;
+    for (int i = count + tid; i < n; i += NT) c.rank[i] = 0;
+    sort_falling<NT>(c.rank, n);
+    // neighbouring ranks in a thread
+    constexpr int E = kMost / NT;
+    u64 v[E], sum = 0, total, kept_here = 0;
+    double y[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int i = E * tid + e;
+        y[e] = i < most ? w.log2_of(value_of(c.rank[i])) : -100.0;
+        v[e] = i < most ? w.of_log2(y[e]) : 0;
+        sum += v[e];
+    }
+    u64 before = Block<NT>::before(sum, c.waves, total);
+    const u64 want = g.by_p ? g.want(total) : ~0ull;
+    bool keep[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        keep[e] = E * tid + e < most && before < want && g.passes(y[e]);
+        before += v[e];
+        kept_here += keep[e];
+    }
+    // (ranks are kept up to some rank, so their numbers are the kept ones')
+    const int kept = (int)Block<NT>::reduce(kept_here, c.waves, Add());
+    n = 64;
+    while (n < kept) n *= 2;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int i = E * tid + e;
+        if (i >= n) continue;
+        c.order[i] = keep[e] ? ((u64)(uint32_t)c.rank[i] << 32) | (unsigned)i : 0;      // (~index: falling order is rising index)
+        c.mass[i] = keep[e] ? v[e] : 0;
+    }
+    sort_falling<NT>(c.order, n);
+    int who[E];
+    sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int i = E * tid + e;
+        who[e] = i < kept ? (int)(uint32_t)c.order[i] : -1;
+        v[e] = who[e] >= 0 ? c.mass[who[e]] : 0;
+        sum += v[e];
+    }
+    before = Block<NT>::before(sum, c.waves, total);
+    const u64 target = draw_target(a, row, total);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        if (before <= target && target < before + v[e])
+            put_drawn(a, row, index_of(c.rank[who[e]]), w.log2_of(value_of(c.rank[who[e]])), total);
+        before += v[e];
+    }
+}
+
+// ---- any number of candidates, in one block ---------------------------------------------------
+constexpr int kEach = 8;                               // logits of a thread in a tile, in index order
+constexpr int kHeld = 4;                               // tiles that a block holds in registers
+constexpr int kBins = 2048;
+constexpr int kMaxTiles = 2048, kRowThreads = 1024, kShortThreads = 256;      // (16 M columns)
+
+template <int NT> struct Histograms {
+    u64 waves[Block<NT>::kWaves];
+    u64 bins[kBins];
+    u64 tile_mass[kMaxTiles];
+    uint32_t tile_ties[kMaxTiles];
+    u64 found[2];
+};
+template <int NT> union SampleShared {
+    Histograms<NT> h;
+    Candidates<NT> c;
+};
+
+// The first of n sums (thread t has those from n / NT t on, by at(i)) up to and with which they reach
+// `want` (from 1 on): its number and the sum before it; -1: they do not.  found: LDS of two.
+template <int NT, int N, class AT> __device__ __forceinline__ int reach(AT at, u64 want, u64* waves, u64* found, u64& before, u64& total) {
+    u64 v[N], sum = 0;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        v[e] = at(N * (int)threadIdx.x + e);
+        sum += v[e];
+    }
+    if (threadIdx.x == 0) found[0] = ~0ull;
+    u64 b = Block<NT>::before(sum, waves, total);
+    if (b < want && want <= b + sum) {
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            if (b < want && want <= b + v[e]) {
+                found[0] = (u64)(N * (int)threadIdx.x + e);
+                found[1] = b;
+            }
+            b += v[e];
+        }
+    }
+    __syncthreads();
+    before = found[1];
+    return (int)found[0];
+}
+
+// A row in tiles, from its first chunk on; HELD: all of them (at most kHeld) stay in registers.
+template <int DT, int NT, bool HELD> struct SampleRow : RowChunks<DT> {
+    typedef RowChunks<DT> Chunks;
+    static constexpr int PER = kEach / Chunks::VEC;    // chunks of a thread in a tile
+    static constexpr int kTile = NT * kEach;
+    int tiles;
+    uint4 held[HELD ? kHeld : 1][PER];
+
+    __device__ __forceinline__ SampleRow(const SampleArgs& a, int64_t row) : Chunks(a, row) {
+        tiles = (this->first + this->V + kTile - 1) / kTile;
+        if constexpr (HELD) {
+#pragma unroll
+            for (int i = 0; i < kHeld; i++) raw(i, held[i]);
+        }
+    }
+    __device__ __forceinline__ int index(int tile) const { return tile * kTile + (int)threadIdx.x * kEach - this->first; }
+    __device__ __forceinline__ void raw(int tile, uint4 (&q)[PER]) const {
+        const int lo = tile * kTile + __builtin_amdgcn_readfirstlane((int)threadIdx.x & ~63) * kEach - this->first;
+        this->chunks(lo, lo + 64 * kEach, [&](int c) { return index(tile) + c * Chunks::VEC; }, q);
+    }
+    __device__ __forceinline__ void load(int tile, float (&x)[kEach]) const {
+        uint4 q[PER];
+        raw(tile, q);
+#pragma unroll
+        for (int c = 0; c < PER; c++) Chunks::open(q[c], x + c * Chunks::VEC);
+    }
+    // f(tile, logits) for every tile in index order
+    template <class F> __device__ __forceinline__ void each(F f) const {
+        if constexpr (HELD) {
+#pragma unroll
+            for (int tile = 0; tile < kHeld; tile++) {
+                if (tile >= tiles) break;
+                float x[kEach];
+#pragma unroll
+                for (int c = 0; c < PER; c++) {
+                    uint4 q = held[tile][c];           // (opened anew each time: kept open, they take twice the registers)
+                    asm volatile("" : "+v"(q.x), "+v"(q.y), "+v"(q.z), "+v"(q.w));
+                    Chunks::open(q, x + c * Chunks::VEC);
+                }
+                f(tile, x);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            uint4 next[PER];
+            raw(0, next);
+            for (int tile = 0; tile < tiles; tile++) {
+                float x[kEach];
+#pragma unroll
+                for (int c = 0; c < PER; c++) Chunks::open(next[c], x + c * Chunks::VEC);
+                if (tile + 1 < tiles) raw(tile + 1, next);
+                f(tile, x);
+            }
+        }
+    }
+};
+
+// Draws among the logits whose rank is at least `border` and that pass min-p, from the tiles' weights.
+template <int DT, int NT, class ROW> __device__ __forceinline__ void draw_tile(const SampleArgs& a, int64_t row, const ROW& r, const Settings& g, const Weights& w,
+                                                               u64 border, float least, Histograms<NT>& s) {
+    u64 all = 0, total;
+    for (int i = 0; i < r.tiles; i++) all += s.tile_mass[i];
+    u64 target = draw_target(a, row, all);
+    int tile = 0;
+    for (; tile + 1 < r.tiles && target >= s.tile_mass[tile]; tile++) target -= s.tile_mass[tile];
+    float x[kEach];
+    u64 v[kEach], mine = 0;
+    r.load(tile, x);
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+        const double y = w.log2_of(x[e]);
+        v[e] = x[e] >= least && rank_of(x[e], r.index(tile) + e) >= border && g.passes(y) ? w.of_log2(y) : 0;
+        mine += v[e];
+    }
+    u64 from = Block<NT>::before(mine, s.waves, total);
+    if (from <= target && target < from + mine) {
+#pragma unroll
+        for (int e = 0; e < kEach; e++) {
+            if (from <= target && target < from + v[e]) put_drawn(a, row, r.index(tile) + e, w.log2_of(x[e]), all);
+            from += v[e];
+        }
+    }
+}
+
+// Kept are the values above some border value and the first few equal to it.  The border is found
+// digit by digit from the highest values down, in histograms of counts (top-k) or weights (top-p).
+template <int DT, int NT, class ROW> __device__ __forceinline__ void draw_any(const SampleArgs& a, int64_t row, const ROW& r, const Settings& g, const Weights& wt,
+                                                              Histograms<NT>& s) {
+    constexpr int kRounds = DT == kF32 ? 3 : 2;        // digits of 11, 11 and 10 bits; 16-bit logits differ in the first two
+    const int tid = (int)threadIdx.x;
     uint32_t border = 0;                               // (no key: everything is kept)
     u64 ties = 0, equal = 0;                           // equal: keys that are the border's, of those ranked at all
-    // A digit search from the highest key down: the value at which the sums of amount(x) over the
-    // keys >= least pass want.  less: what to take off the sum of least's own bin.
+    // The value at which the sums of amount(x) over the keys >= least pass want_of(their total), and
+    // the sum above it; false: they do not.  less: what to take off the sum of least's own bin.
     auto search = [&](auto amount, uint32_t least, u64 less, auto want_of, u64& above) {
         uint32_t prefix = 0;
         u64 want = 0, within = 0;
         above = 0;
         for (int round = 0; round < kRounds; round++) {
             const int low = round == 0 ? 21 : round == 1 ? 10 : 0, width = round == 2 ? 10 : 11;
-            for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
             __syncthreads();
-            for (int tile = 0; tile < r.tiles; tile++) {
-                float x[kEach];
-                r.load(tile, x);
+            for (int i = tid; i < kBins; i += NT) s.bins[i] = 0;
+            __syncthreads();
+            r.each([&](int, const float (&x)[kEach]) {
 #pragma unroll
                 for (int e = 0; e < kEach; e++) {
                     const uint32_t key = key_of(x[e]);
                     if (x[e] == -INFINITY || key < least) continue;
                     if (round && (key >> (low + width)) != prefix) continue;
                     const u64 v = amount(x[e]);
-                    if (v) atomicAdd(&s.bins[(key >> low) & (kBins - 1) & ((1u << width) - 1)], v);
+                    if (v) atomicAdd(&s.bins[(key >> low) & ((1u << width) - 1)], v);
                 }
-            }
+            });
             __syncthreads();
             if (less && tid == 0 && (!round || (least >> (low + width)) == prefix))
                 s.bins[(least >> low) & ((1u << width) - 1)] -= less;
             __syncthreads();
             if (round == 0) {
-                u64 total;
-                (void)scan_before(s.bins[2 * tid] + s.bins[2 * tid + 1], s.waves, total);
+                u64 sum = 0;
+                for (int i = tid; i < kBins; i += NT) sum += s.bins[i];
+                const u64 total = Block<NT>::reduce(sum, s.waves, Add());
                 want = want_of(total);
-                if (!want || want > total) return false;               // all of them
+                if (!want || want > total) return false;
             }
-            int bin;
-            u64 over;
-            pick_bin(s, want - above, bin, over);
+            u64 over, total;
+            const int bin = kBins - 1 - reach<NT, kBins / NT>([&](int i) { return s.bins[kBins - 1 - i]; }, want - above, s.waves, s.found, over, total);
             above += over;
             within = s.bins[bin];
             prefix = (prefix << width) | (uint32_t)bin;
-            __syncthreads();
         }
         if (kRounds == 2) prefix = prefix & (1u << 21) ? prefix << 10 : (prefix << 10) | 0x3FF;      // the digits all values share
         border = prefix;
@@ -272,47 +572,37 @@ template <int DT> __global__ __launch_bounds__(kThreads) void k_sample_row(Sampl
         return true;
     };
 
-    if (k > 0 && k < a.V) {
+    if (g.by_k) {
         u64 above;
-        if (search([](float) { return (u64)1; }, 0u, 0, [&](u64) { return (u64)k; }, above)) ties = (u64)k - above;
+        if (search([](float) { return (u64)1; }, 0u, 0, [&](u64) { return (u64)g.k; }, above)) ties = (u64)g.k - above;
     }
-    if (p < 1.0) {
+    if (g.by_p) {
         // of border's equals only `ties` are there
         const uint32_t least = border;
-        const u64 own = least ? weight(of_key(least)) : 0, gone = least ? (equal - ties) * own : 0, had = ties;
+        const u64 own = least ? wt.of(of_key(least)) : 0, gone = least ? (equal - ties) * own : 0;
         u64 above, want = 0;
-        const bool some = search(weight, least, gone, [&](u64 total) {
-            const double w = __builtin_ceil(p * (double)total);
-            want = !(w >= 1.0) ? 1 : w >= (double)total ? total : (u64)w;
-            return want;
-        }, above);
+        const bool some = search([&](float x) { return wt.of(x); }, least, gone, [&](u64 total) { return want = g.want(total); }, above);
         if (some) {
-            const u64 each = weight(of_key(border)), n = equal / each;            // (each > 0: the sums pass want here)
+            const u64 each = wt.of(of_key(border)), n = equal / each;            // (each > 0: the sums pass want here)
             ties = (want - above + each - 1) / each;
             ties = ties < 1 ? 1 : ties > n ? n : ties;
             equal = border == least ? n + (gone / (own ? own : 1)) : n;
-        } else {
-            ties = had;
         }
     }
-    const double least_weight = m >= 1.0 ? 1.0 : m > 0.0 ? m : 0.0;
     const bool some_ties = border && ties < equal;     // the ties are told apart by index
 
     // ---- the kept weights, tile by tile in index order
     // Weights of this thread's logits; before: equals of the border in the tiles and threads before.
-    auto weigh = [&](const float (&x)[kEach], u64 before, u64 (&w)[kEach]) {
+    auto weigh = [&](const float (&x)[kEach], u64 before, u64 (&v)[kEach]) {
         u64 sum = 0;
 #pragma unroll
         for (int e = 0; e < kEach; e++) {
             const uint32_t key = key_of(x[e]);
             bool keep = x[e] > -INFINITY && key >= border;
             if (some_ties && key == border) keep = keep && before++ < ties;
-            w[e] = 0;
-            if (keep) {
-                const double y = log2_weight(x[e], top, per);
-                if (!(least_weight > 0.0) || pow2(y < -1000.0 ? -1000.0 : y) >= least_weight) w[e] = fixed_weight(y, a.shift);
-            }
-            sum += w[e];
+            const double y = wt.log2_of(x[e]);
+            v[e] = keep && g.passes(y) ? wt.of_log2(y) : 0;
+            sum += v[e];
         }
         return sum;
     };
@@ -323,42 +613,577 @@ template <int DT> __global__ __launch_bounds__(kThreads) void k_sample_row(Sampl
         return n;
     };
     u64 all = 0, met = 0;
-    for (int tile = 0; tile < r.tiles; tile++) {
-        float x[kEach];
-        u64 w[kEach], before = 0, total;
-        r.load(tile, x);
+    __syncthreads();
+    r.each([&](int tile, const float (&x)[kEach]) {
+        u64 v[kEach], before = 0, total;
         if (tid == 0) s.tile_ties[tile] = (uint32_t)met;
         if (some_ties) {
-            before = met + scan_before(count_ties(x), s.waves, total);
+            before = met + Block<NT>::before(count_ties(x), s.waves, total);
             met += total;
         }
-        (void)scan_before(weigh(x, before, w), s.waves, total);
+        total = Block<NT>::reduce(weigh(x, before, v), s.waves, Add());
         if (tid == 0) s.tile_mass[tile] = total;
         all += total;
-    }
+    });
     __syncthreads();
 
     // ---- the draw
-    const double u = a.u64 ? ((const double*)a.u)[row] : (double)((const float*)a.u)[row];
-    const double at = u * (double)all;
-    u64 target = !(at > 0.0) ? 0 : at >= (double)all ? all - 1 : (u64)at;
-    if (target >= all) target = all - 1;
+    u64 target = draw_target(a, row, all);
     int tile = 0;
     for (; tile + 1 < r.tiles && target >= s.tile_mass[tile]; tile++) target -= s.tile_mass[tile];
     float x[kEach];
-    u64 w[kEach], before = 0, total;
+    u64 v[kEach], before = 0, total;
     r.load(tile, x);
-    if (some_ties) before = s.tile_ties[tile] + scan_before(count_ties(x), s.waves, total);
-    const u64 mine = weigh(x, before, w);
-    u64 from = scan_before(mine, s.waves, total);
+    if (some_ties) before = s.tile_ties[tile] + Block<NT>::before(count_ties(x), s.waves, total);
+    const u64 mine = weigh(x, before, v);
+    u64 from = Block<NT>::before(mine, s.waves, total);
     if (from <= target && target < from + mine) {
 #pragma unroll
         for (int e = 0; e < kEach; e++) {
-            if (from <= target && target < from + w[e])
-                put_token(a, row, r.index(tile) + e,
-                          (float)(log2_weight(x[e], top, per) * 0.6931471805599453 + (double)a.shift * 0.6931471805599453 - log((double)all)));
-            from += w[e];
+            if (from <= target && target < from + v[e]) put_drawn(a, row, r.index(tile) + e, wt.log2_of(x[e]), all);
+            from += v[e];
         }
+    }
+}
+
+// A value that at least k logits are no less than, from the largest logits of some groups of them
+// (visit(f) calls f with the thread's): counted in bins between the least and the largest of these,
+// lo and top.  -inf: there are fewer groups.
+template <int NT, class V> __device__ __forceinline__ float kth_bound(V visit, u64 k, float lo, float top, Histograms<NT>& s) {
+    const float scale = (float)(kBins - 1) / (top - lo);
+    __syncthreads();
+    for (int i = (int)threadIdx.x; i < kBins; i += NT) s.bins[i] = 0;
+    __syncthreads();
+    visit([&](float x) {
+        if (x == -INFINITY) return;
+        const float f = (top - x) * scale;             // (NaN of equal or infinite ones: bin 0)
+        atomicAdd(&s.bins[f > 0.0f ? (int)fminf(f, kBins - 1) : 0], (u64)1);
+    });
+    __syncthreads();
+    u64 before, total;
+    const int bin = reach<NT, kBins / NT>([&](int i) { return s.bins[i]; }, k, s.waves, s.found, before, total);
+    if (bin < 0) return -INFINITY;
+    const float edge = top - (float)(bin + 1) / scale;                 // (rounded: down by more than its own errors)
+    const float least = edge - 1e-5f * (__builtin_fabsf(top) + __builtin_fabsf(lo));
+    return least == least && top < INFINITY ? least : -INFINITY;
+}
+
+// Among the `count` ranks of the border's bin (weights above it: `above`) the last that top-p keeps;
+// kept(rank, weight) for those that min-p lets pass too.
+template <int NT, class F> __device__ __forceinline__ u64 border_in(u64* list, int count, u64 above, u64 want, const Settings& g, const Weights& w, u64* waves,
+                                                     u64* found, F kept) {
+    int n = 64;
+    while (n < count) n *= 2;
+    for (int i = count + (int)threadIdx.x; i < n; i += NT) list[i] = 0;
+    sort_falling<NT>(list, n);
+    constexpr int E = kMost / NT;
+    u64 v[E], sum = 0, total;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int i = E * (int)threadIdx.x + e;
+        v[e] = i < count ? w.of(value_of(list[i])) : 0;
+        sum += v[e];
+    }
+    if (threadIdx.x == 0) found[0] = ~0ull;
+    u64 before = above + Block<NT>::before(sum, waves, total);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int i = E * (int)threadIdx.x + e;
+        if (i < count && before < want) {
+            atomicMin(&found[0], list[i]);
+            if (g.passes(w.log2_of(value_of(list[i])))) kept(list[i], v[e]);
+        }
+        before += v[e];
+    }
+    __syncthreads();
+    const u64 border = found[0];
+    __syncthreads();
+    return border;
+}
+
+// Bins of a weight's logarithm from the largest down.
+__device__ __forceinline__ int log_bin(double y) { return min((int)(y * -51.0), kBins - 1); }      // (51 to a factor of two: 40 of them)
+
+// A block per row.  HELD: the row is read once, into registers.
+template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sample_row(SampleArgs a) {
+    __shared__ SampleShared<NT> s;
+    typedef Block<NT> B;
+    const int64_t row = blockIdx.x;
+    const int tid = (int)threadIdx.x;
+    const SampleRow<DT, NT, HELD> r(a, row);
+    const Settings g(a, row);
+
+    // ---- the largest value
+    float most = -INFINITY;
+    r.each([&](int, const float (&x)[kEach]) {
+#pragma unroll
+        for (int e = 0; e < kEach; e++) most = fmaxf(most, x[e]);
+    });
+    const float top = B::reduce(most, s.h.waves, Max());
+    if (top == -INFINITY) {
+        if (tid == 0) put_token(a, row, -1, -INFINITY);
+        return;
+    }
+    if (g.greedy) {                                    // and where it is first
+        int at = 0x7FFFFFFF;
+        r.each([&](int tile, const float (&x)[kEach]) {
+#pragma unroll
+            for (int e = kEach - 1; e >= 0; e--) at = x[e] == top ? min(at, r.index(tile) + e) : at;
+        });
+        at = B::reduce(at, s.h.waves, Min());
+        if (tid == 0) put_token(a, row, at, 0.0f);
+        return;
+    }
+    const Weights w = {finite(top), g.per, a.shift};
+
+    // ---- top-k, or min-p alone: few candidates, where few are above what none kept is below
+    if (g.by_k || (!g.by_p && g.m > 0.0)) {
+        float least = -INFINITY;
+        if (g.by_k) {
+            const float lo = B::reduce(most > -INFINITY ? most : top, s.h.waves, Min());
+            least = kth_bound<NT>([&](auto f) { f(most); }, (u64)g.k, lo, top, s.h);
+        }
+        if (g.m > 0.0 && !g.by_p) least = fmaxf(least, g.least(top));
+        __syncthreads();
+        if (tid == 0) s.c.count = 0;
+        __syncthreads();
+        r.each([&](int tile, const float (&x)[kEach]) {
+#pragma unroll
+            for (int e = 0; e < kEach; e++)
+                add_candidate(s.c.rank, &s.c.count, kMost, x[e] >= least && x[e] > -INFINITY, x[e], r.index(tile) + e);
+        });
+        __syncthreads();
+        if (s.c.count <= kMost) {
+            draw_candidates<NT>(a, row, g, w, s.c);
+            return;
+        }
+        __syncthreads();
+        draw_any<DT, NT>(a, row, r, g, w, s.h);
+        return;
+    }
+    // ---- no filter, or top-p: the weights by their logarithm, then those above the border's bin by
+    // tile, and the bin's own one by one
+    Histograms<NT>& h = s.h;
+    u64 border = 0;
+    int bin = kBins;
+    u64 above = 0, want = 0;
+    if (g.by_p) {
+        __syncthreads();
+        for (int i = tid; i < kBins; i += NT) h.bins[i] = 0;
+        __syncthreads();
+        r.each([&](int, const float (&x)[kEach]) {
+#pragma unroll
+            for (int e = 0; e < kEach; e++) {
+                const double y = w.log2_of(x[e]);
+                const u64 v = w.of_log2(y);
+                if (v) atomicAdd(&h.bins[log_bin(y)], v);
+            }
+        });
+        __syncthreads();
+        u64 sum = 0, total;
+        for (int i = tid; i < kBins; i += NT) sum += h.bins[i];
+        sum = B::reduce(sum, h.waves, Add());
+        want = g.want(sum);
+        bin = reach<NT, kBins / NT>([&](int i) { return h.bins[i]; }, want, h.waves, h.found, above, total);
+        if (bin == kBins - 1) {                        // (among weights below 2^-40)
+            draw_any<DT, NT>(a, row, r, g, w, h);
+            return;
+        }
+        __syncthreads();
+        if (tid == 0) h.tile_ties[0] = 0;              // the bin's count; its ranks go where the bins were
+        __syncthreads();
+    }
+    u64 mass[HELD ? kHeld : 1];
+    r.each([&](int tile, const float (&x)[kEach]) {
+        u64 sum = 0;
+        if (!g.by_p) {
+            sum = w.sum(x);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kEach; e++) {
+                const double y = w.log2_of(x[e]);
+                const int b = log_bin(y);
+                if (b < bin && g.passes(y)) sum += w.of_log2(y);
+                add_candidate(h.bins, &h.tile_ties[0], kBins, b == bin, x[e], r.index(tile) + e);
+            }
+        }
+        if constexpr (HELD) {
+            mass[tile] = sum;
+        } else {
+            sum = B::reduce(sum, h.waves, Add());
+            if (tid == 0) h.tile_mass[tile] = sum;
+        }
+    });
+    if constexpr (HELD) {
+#pragma unroll
+        for (int tile = 0; tile < kHeld; tile++) {
+            if (tile >= r.tiles) break;
+            const u64 sum = B::reduce(mass[tile], h.waves, Add());
+            if (tid == 0) h.tile_mass[tile] = sum;
+        }
+    }
+    __syncthreads();
+    if (g.by_p) {
+        const int count = (int)h.tile_ties[0];
+        if (count > kBins) {                           // (many equal ones)
+            draw_any<DT, NT>(a, row, r, g, w, h);
+            return;
+        }
+        border = border_in<NT>(h.bins, count, above, want, g, w, h.waves, h.found,
+                               [&](u64 rank, u64 v) { atomicAdd(&h.tile_mass[(index_of(rank) + r.first) / r.kTile], v); });
+    }
+    draw_tile<DT, NT>(a, row, r, g, w, border, -FLT_MAX, h);
+}
+
+// ---- a row spread over blocks -----------------------------------------------------------------
+// Few long rows would leave most of the GPU idle, and many are read more often than need be by a
+// block each.  So one launch reads all logits once and leaves, of every 4096 of a row (a span), the
+// largest value, the sum of the weights against it, and, where top-p or min-p may need them, these sums
+// by the weights' logarithm; of every 16 the largest value.  A block per row goes on from those:
+// with top-k the few logits that can be kept, else the span that the draw falls into, and for a
+// border the logits whose logarithm is the border's.
+constexpr int kSpanThreads = 256, kSpan = 16 * kSpanThreads;
+constexpr int kSpans = 512;                            // of a row at most
+constexpr int kLogBins = 128;                          // four to a factor of two, from a span's largest down
+constexpr int kNear = 12288;                           // logits of the border's bins
+
+struct Spread {
+    float *largest, *group;            // of each span, and of each 16 logits
+    u64 *mass, *bins;                  // of each span
+    int spans;                         // of a row
+};
+
+// A logit's logarithm in bins, downwards, from that of 0 on: the same for all spans and launches.
+__device__ __forceinline__ double grid_of(float x, double per) { return -__builtin_floor(finite(x) * (per * 4.0)); }
+
+// Chunk i of a lane's 16 logits of a span: its first index.
+template <int DT> __device__ __forceinline__ int span_index(const RowChunks<DT>& r, int span, int group, int i) {
+    return span * kSpan + (group >> 6) * 1024 + i * 64 * RowChunks<DT>::VEC + (group & 63) * RowChunks<DT>::VEC - r.first;
+}
+
+template <int DT> __global__ __launch_bounds__(kSpanThreads) void k_sample_spans(SampleArgs a, Spread w) {
+    __shared__ u64 bins[kLogBins], waves[kSpanThreads / 64];
+    typedef Block<kSpanThreads> B;
+    constexpr int N = 16 / RowChunks<DT>::VEC;
+    const int64_t row = blockIdx.x / (unsigned)w.spans;
+    const int span = (int)(blockIdx.x % (unsigned)w.spans), tid = (int)threadIdx.x;
+    const RowChunks<DT> r(a, row);
+    uint4 q[N];
+    const int lo = span * kSpan + __builtin_amdgcn_readfirstlane(tid >> 6) * 1024 - r.first;
+    r.chunks(lo, lo + 1024, [&](int i) { return span_index<DT>(r, span, tid, i); }, q);
+    const Settings g(a, row);
+    const bool logs = !g.greedy && !g.by_k && g.filters(), sums = !g.greedy && !g.by_k && (g.by_p || !logs);
+    if (logs && tid < kLogBins) bins[tid] = 0;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < N; i++) RowChunks<DT>::open(q[i], x + i * RowChunks<DT>::VEC);
+    float most = x[0];
+#pragma unroll
+    for (int e = 1; e < 16; e++) most = fmaxf(most, x[e]);
+    const int64_t at = row * w.spans + span;
+    if (g.by_k) w.group[at * kSpanThreads + tid] = most;
+    const float top = B::reduce(most, waves, Max());
+    if (tid == 0) w.largest[at] = top;
+    if (!logs && !sums) return;
+    u64 sum = 0;
+    if (top > -INFINITY) {
+        const Weights wt = {finite(top), g.per, a.shift};
+        if (!logs) {
+            sum = wt.sum(x);
+        } else {
+            const double from = grid_of(top, g.per);
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const u64 v = wt.of(x[e]);
+                const double b = __builtin_fmin(grid_of(x[e], g.per) - from, kLogBins - 1);
+                if (v) atomicAdd(&bins[(int)b], v);
+                sum += v;
+            }
+        }
+    }
+    sum = B::reduce(sum, waves, Add());                // (and the bins are filled)
+    if (tid == 0) w.mass[at] = sum;
+    if (logs && tid < kLogBins) w.bins[at * kLogBins + tid] = bins[tid];
+}
+
+// The span in which the sums of mass(span) pass the target, and the target within it.
+template <class M> __device__ __forceinline__ int pick_span(const SampleArgs& a, int64_t row, int spans, u64* waves, u64* found, M mass, u64& target, u64& all) {
+    const int i = 2 * (int)threadIdx.x;                // (at most 2 kRowThreads)
+    const u64 p = i < spans ? mass(i) : 0, q = i + 1 < spans ? mass(i + 1) : 0;
+    const u64 before = Block<kRowThreads>::before(p + q, waves, all);
+    target = draw_target(a, row, all);
+    if (before <= target && target < before + p) { found[0] = (u64)i; found[1] = target - before; }
+    else if (before + p <= target && target < before + p + q) { found[0] = (u64)i + 1; found[1] = target - before - p; }
+    __syncthreads();
+    target = found[1];
+    return (int)found[0];
+}
+
+struct PickShared {
+    union {
+        SampleShared<kRowThreads> s;
+        struct {
+            u64 waves[kRowThreads / 64], fine[kBins], row_bins[kLogBins];
+            u64 near[kNear];
+        };
+    };
+    u64 kept[kSpans], found[2];
+    unsigned count, count2;
+};
+static_assert(kSpan == 4 * kRowThreads, "logits of a thread in the drawn span");
+
+template <int DT> __global__ __launch_bounds__(kRowThreads) void k_sample_pick(SampleArgs a, Spread w) {
+    __shared__ PickShared s;
+    typedef Block<kRowThreads> B;
+    constexpr int NT = kRowThreads, VEC = RowChunks<DT>::VEC;
+    const int64_t row = blockIdx.x;
+    const int tid = (int)threadIdx.x, lane = tid & 63;
+    const float* largest = w.largest + row * w.spans;
+    const u64* mass = w.mass + row * w.spans;
+    const Settings g(a, row);
+    float top = -INFINITY;
+    for (int i = tid; i < w.spans; i += NT) top = fmaxf(top, largest[i]);
+    top = B::reduce(top, s.waves, Max());
+    if (top == -INFINITY) {
+        if (tid == 0) put_token(a, row, -1, -INFINITY);
+        return;
+    }
+    const RowChunks<DT> r(a, row);
+    // A thread's four neighbouring logits of a span, and the first one's index.
+    auto logits = [&](int span, float (&x)[4]) {
+        const int i = span * kSpan + 4 * tid - r.first;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float v = i + e >= 0 && i + e < a.V ? (float)ld_d<DT>(a.x, row * a.ld + i + e) : -INFINITY;
+            x[e] = v != v ? -INFINITY : v;
+        }
+        return i;
+    };
+    if (g.greedy) {
+        int at = 0x7FFFFFFF;
+        for (int i = tid; i < w.spans; i += NT) at = largest[i] == top ? min(at, i) : at;
+        float x[4];
+        const int i = logits(B::reduce(at, s.waves, Min()), x);
+        at = 0x7FFFFFFF;
+#pragma unroll
+        for (int e = 3; e >= 0; e--) at = x[e] == top ? i + e : at;
+        at = B::reduce(at, s.waves, Min());
+        if (tid == 0) put_token(a, row, at, 0.0f);
+        return;
+    }
+    const Weights wt = {finite(top), g.per, a.shift};
+    // A sum of weights against a span's largest value (y: log2 of this one's weight), against the row's.
+    // (Nothing where the largest itself weighs nothing: no draw could end there.)
+    auto factor_of = [&](double y) { return y >= -(double)a.shift ? exp2(y) : 0.0; };
+    auto against_top = [&](u64 v, double factor) { return (u64)__builtin_rint((double)v * factor); };
+    // Draws in a span among what keep(x, index, log2 of the weight) says.
+    auto draw_span = [&](int span, u64 target, u64 all, auto keep) {
+        float x[4];
+        u64 v[4], mine = 0, total;
+        const int i = logits(span, x);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const double y = wt.log2_of(x[e]);
+            v[e] = x[e] > -INFINITY && keep(x[e], i + e, y) ? wt.of_log2(y) : 0;
+            mine += v[e];
+        }
+        u64 before = B::before(mine, s.waves, total);
+        if (target >= total) target = total - 1;       // (its sum against its own largest value was rounded once more)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (before <= target && target < before + v[e]) put_drawn(a, row, i + e, wt.log2_of(x[e]), all);
+            before += v[e];
+        }
+    };
+    if (!g.filters()) {
+        u64 target, all;
+        const int span = pick_span(a, row, w.spans, s.waves, s.found,
+                                   [&](int i) { return against_top(mass[i], factor_of(wt.log2_of(largest[i]))); }, target, all);
+        draw_span(span, target, all, [](float, int, double) { return true; });
+        return;
+    }
+    const SampleRow<DT, NT, false> whole(a, row);
+    if (g.by_k) {
+        // ---- the few logits that can be among the k largest
+        const float* group = w.group + row * w.spans * kSpanThreads;
+        const int groups = w.spans * kSpanThreads;
+        float lo = top;
+        for (int i = tid; i < groups; i += NT) lo = group[i] > -INFINITY ? fminf(lo, group[i]) : lo;
+        lo = B::reduce(lo, s.waves, Min());
+        float least = kth_bound<NT>([&](auto f) {
+            for (int i = tid; i < groups; i += NT) f(group[i]);
+        }, (u64)g.k, lo, top, s.s.h);
+        if (g.m > 0.0 && !g.by_p) least = fmaxf(least, g.least(top));
+        __syncthreads();
+        if (tid == 0) s.s.c.count = 0;
+        __syncthreads();
+        for (int i0 = 0; i0 < groups && s.s.c.count <= kMost; i0 += NT) {
+            const int i = i0 + tid;
+            const bool in = i < groups && group[i] >= least && group[i] > -INFINITY;
+            if (!__ballot(in)) continue;
+#pragma unroll
+            for (int c = 0; c < 16 / VEC; c++) {
+                float x[VEC];
+                const int at = span_index<DT>(r, i / kSpanThreads, i % kSpanThreads, c);
+                RowChunks<DT>::open(in ? r.part(at) : uint4{0, 0, 0, 0}, x);
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    add_candidate(s.s.c.rank, &s.s.c.count, kMost, in && x[e] >= least && x[e] > -INFINITY, x[e], at + e);
+            }
+        }
+        __syncthreads();
+        if (s.s.c.count <= kMost) {
+            draw_candidates<NT>(a, row, g, wt, s.s.c);
+            return;
+        }
+        __syncthreads();
+        draw_any<DT, NT>(a, row, whole, g, wt, s.s.h);
+        return;
+    }
+
+    // ---- top-p, min-p: the row's weights by their logarithm
+    const double from = grid_of(top, g.per);
+    __syncthreads();
+    if (tid < kLogBins) s.row_bins[tid] = 0;
+    if (tid == 0) s.count = s.count2 = 0;
+    __syncthreads();
+    auto each_bin = [&](auto f) {                      // f(span, bin of the row, weight): a wave per span
+        for (int i = tid >> 6; i < w.spans; i += B::kWaves) {
+            const double y = wt.log2_of(largest[i]), below = grid_of(largest[i], g.per) - from;
+            const double factor = factor_of(y);
+            if (!(factor > 0.0 && below < kLogBins)) continue;
+            const u64* b = w.bins + (row * w.spans + i) * kLogBins;
+            f(i, (int)below + lane, against_top(b[lane], factor), (int)below + 64 + lane, against_top(b[lane + 64], factor));
+        }
+    };
+    u64 weights = 0;
+    each_bin([&](int, int i, u64 p, int j, u64 q) {
+        // (the last bin of a span holds all that is below: no less than the row's last)
+        if (p) atomicAdd(&s.row_bins[min(i, kLogBins - 1)], p);
+        if (q) atomicAdd(&s.row_bins[min(j, kLogBins - 1)], q);
+        weights += p + q;
+    });
+    weights = B::reduce(weights, s.waves, Add());
+    const u64 want = g.by_p ? g.want(weights) : ~0ull;
+    u64 above = 0, total;
+    int first = kLogBins, last = -1;                   // bins that a border may lie in
+    if (g.by_p) {
+        first = reach<NT, 1>([&](int i) { return i < kLogBins ? s.row_bins[i] : 0; }, want, s.waves, s.found, above, total);
+        if (first < 0) first = kLogBins - 1;
+        last = first;
+    }
+    if (g.m > 0.0) {
+        const double b = __builtin_fmin(-__builtin_floor(wt.top * (g.per * 4.0) + 4.0 * log2(g.m)) - from, kLogBins);
+        if ((int)b - 1 <= last || !g.by_p) first = min(first, max((int)b - 1, 0));
+        if (!g.by_p || (int)b - 1 <= last) last = max((int)b + 1, first);      // (min-p's, unless top-p's is well above)
+        if (g.by_p && (int)b - 1 > first) last = first;
+        // weights above the first bin
+        u64 sum = tid < kLogBins && tid < first ? s.row_bins[tid] : 0;
+        above = B::reduce(sum, s.waves, Add());
+    }
+    if (last >= kLogBins - 1) {                        // (among weights below 2^-31 of the largest)
+        __syncthreads();
+        draw_any<DT, NT>(a, row, whole, g, wt, s.s.h);
+        return;
+    }
+    // the spans' weights above those bins
+    for (int i = tid; i < w.spans; i += NT) s.kept[i] = 0;
+    __syncthreads();
+    each_bin([&](int span, int i, u64 p, int j, u64 q) {
+        const u64 sum = wave_allreduce((i < first ? p : 0) + (j < first ? q : 0), Add());
+        if (lane == 0) s.kept[span] = sum;
+    });
+    // and their logits in them
+    whole.each([&](int tile, const float (&x)[kEach]) {
+#pragma unroll
+        for (int e = 0; e < kEach; e++) {
+            const double b = grid_of(x[e], g.per) - from;
+            add_candidate(s.near, &s.count, kNear, b >= first && b <= last && x[e] > -INFINITY, x[e], whole.index(tile) + e);
+        }
+    });
+    __syncthreads();
+    if (s.count > kNear) {
+        __syncthreads();
+        draw_any<DT, NT>(a, row, whole, g, wt, s.s.h);
+        return;
+    }
+    const int near = (int)s.count;
+    u64 border = 0;
+    auto keep_near = [&](u64 rank, u64 v) { atomicAdd(&s.kept[(index_of(rank) + r.first) / kSpan], v); };
+    if (g.by_p) {
+        // the same once more in finer bins, by the logarithm's place between the first and the last
+        const double y0 = -(from + first - 1) - wt.top * (g.per * 4.0), per_bin = kBins / (double)(last - first + 1);      // (4 log2 at the upper end)
+        auto fine_bin = [&](double y) {
+            const double b = (y0 - 4.0 * y) * per_bin;
+            return b <= 0.0 ? 0 : b >= kBins - 1 ? kBins - 1 : (int)b;
+        };
+        for (int i = tid; i < kBins; i += NT) s.fine[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < near; i += NT) {
+            const double y = wt.log2_of(value_of(s.near[i]));
+            atomicAdd(&s.fine[fine_bin(y)], wt.of_log2(y));
+        }
+        __syncthreads();
+        u64 over;
+        int bin = reach<NT, kBins / NT>([&](int i) { return s.fine[i]; }, want - above, s.waves, s.found, over, total);
+        if (bin < 0) bin = kBins;                      // (the sums were rounded: all of them)
+        __syncthreads();
+        for (int i = tid; i < (near + NT - 1) / NT * NT; i += NT) {
+            const u64 rank = i < near ? s.near[i] : 0;
+            const double y = rank ? wt.log2_of(value_of(rank)) : -100.0;
+            const int b = rank ? fine_bin(y) : kBins + 1;
+            if (b < bin && g.passes(y)) keep_near(rank, wt.of_log2(y));
+            add_candidate(s.fine, &s.count2, kBins, b == bin, value_of(rank), index_of(rank));      // (in the bins' place)
+        }
+        __syncthreads();
+        if (s.count2 > kBins) {                        // (many equal ones)
+            __syncthreads();
+            draw_any<DT, NT>(a, row, whole, g, wt, s.s.h);
+            return;
+        }
+        if (s.count2) border = border_in<NT>(s.fine, (int)s.count2, above + over, want, g, wt, s.waves, s.found, keep_near);
+    } else {
+        for (int i = tid; i < near; i += NT) {
+            const double y = wt.log2_of(value_of(s.near[i]));
+            if (g.passes(y)) keep_near(s.near[i], wt.of_log2(y));
+        }
+    }
+    __syncthreads();
+    u64 target, all;
+    const int span = pick_span(a, row, w.spans, s.waves, s.found, [&](int i) { return s.kept[i]; }, target, all);
+    draw_span(span, target, all, [&](float x, int i, double y) {
+        return rank_of(x, i) >= border && g.passes(y) && grid_of(x, g.per) - from <= last;
+    });
+}
+
+// Memory of a spread call: its parts for `rows` rows at base, and its size.
+size_t spread_layout(Spread& w, void* base, int64_t rows, int64_t V) {
+    w.spans = (int)((V + 7 + kSpan - 1) / kSpan);
+    char* p = (char*)base;
+    auto take = [&](auto*& to, int64_t n) {
+        to = reinterpret_cast<std::remove_reference_t<decltype(to)>>(p);
+        p += (n * (int64_t)sizeof(*to) + 255) / 256 * 256;
+    };
+    take(w.largest, rows * w.spans);
+    take(w.group, rows * w.spans * kSpanThreads);
+    take(w.mass, rows * w.spans);
+    take(w.bins, rows * w.spans * kLogBins);
+    return (size_t)(p - (char*)base);
+}
+
+constexpr int kShort = kHeld * kShortThreads * kEach - 8, kLong = kHeld * kRowThreads * kEach - 8;
+
+template <int DT> void launch_sample(const SampleArgs& a, const Spread* w, hipStream_t s) {
+    const unsigned rows = (unsigned)a.rows;
+    if (w) {
+        hipLaunchKernelGGL(k_sample_spans<DT>, dim3(rows * (unsigned)w->spans), dim3(kSpanThreads), 0, s, a, *w);
+        hipLaunchKernelGGL(k_sample_pick<DT>, dim3(rows), dim3(kRowThreads), 0, s, a, *w);
+    } else if (a.V <= kShort) {
+        hipLaunchKernelGGL((k_sample_row<DT, kShortThreads, true>), dim3(rows), dim3(kShortThreads), 0, s, a);
+    } else if (a.V <= kLong) {
+        hipLaunchKernelGGL((k_sample_row<DT, kRowThreads, true>), dim3(rows), dim3(kRowThreads), 0, s, a);
+    } else {
+        hipLaunchKernelGGL((k_sample_row<DT, kRowThreads, false>), dim3(rows), dim3(kRowThreads), 0, s, a);
     }
 }
 
@@ -367,7 +1192,17 @@ template <int DT> __global__ __launch_bounds__(kThreads) void k_sample_row(Sampl
 
 using namespace tohip;
 
-extern "C" void sample_forward(const Tensor* Logits, const Tensor* Uniform, const Tensor* Temperature,
+extern "C" {
+
+size_t sample_workspace_bytes(int rows, int columns) {
+    if (rows < 1 || columns <= kLong || columns > kSpans * kSpan - 8 ||
+        (int64_t)rows * ((columns + 7) / kSpan + 1) * kSpanThreads >= (int64_t(1) << 32))
+        return 0;
+    Spread w;
+    return spread_layout(w, nullptr, rows, columns);
+}
+
+void sample_forward(const Tensor* Logits, const Tensor* Uniform, const Tensor* Temperature,
                                const Tensor* TopK, const Tensor* TopP, const Tensor* MinP, Tensor* Token,
                                Tensor* LogProb, const SampleParams* params, Tensor* Workspace) {
     const char* name = "sample_forward";
@@ -396,7 +1231,7 @@ extern "C" void sample_forward(const Tensor* Logits, const Tensor* Uniform, cons
         return;
     }
     a.V = params->vocab ? params->vocab : (int)a.ld;
-    if (a.V > kMaxTiles * kTile - 16) { set_error("%s: more than %d columns", name, kMaxTiles * kTile - 16); return; }
+    if (a.V > kMaxTiles * kRowThreads * kEach - 16) { set_error("%s: more than %d columns", name, kMaxTiles * kRowThreads * kEach - 16); return; }
     if ((uintptr_t)Logits->data % dt_bytes(dt)) { set_error("%s: Logits must be aligned to their type", name); return; }
     auto vector = [&](const Tensor* t, int d0, int d1, const char* what) {
         if (!t || (t->ndim == 1 && t->shape[0] == a.rows && ((int)t->dtype == d0 || (int)t->dtype == d1))) return true;
@@ -418,6 +1253,7 @@ extern "C" void sample_forward(const Tensor* Logits, const Tensor* Uniform, cons
         for (int j = 0; j < i; j++)
             if (overlaps(outs[i], outs[j])) { set_error("%s: Token, LogProb and Workspace must not overlap", name); return; }
     }
+    if (a.rows >= (1 << 22)) { set_error("%s: more than %d rows", name, (1 << 22) - 1); return; }
     if (!ensure_device()) return;
     if (!a.rows) return;
     a.x = Logits->data;
@@ -434,9 +1270,23 @@ extern "C" void sample_forward(const Tensor* Logits, const Tensor* Uniform, cons
     while ((int64_t(1) << bits) < a.V) bits++;
     a.shift = std::min(51, 62 - bits);
     DeviceScope scope;
-    const dim3 grid((unsigned)a.rows);
-    if (dt == kF16) hipLaunchKernelGGL(k_sample_row<kF16>, grid, dim3(kThreads), 0, stream(), a);
-    else if (dt == kBF16) hipLaunchKernelGGL(k_sample_row<kBF16>, grid, dim3(kThreads), 0, stream(), a);
-    else hipLaunchKernelGGL(k_sample_row<kF32>, grid, dim3(kThreads), 0, stream(), a);
+    // Rows that a block holds in registers are done by it in one launch; longer ones are spread.
+    Spread w = {};
+    const size_t bytes = sample_workspace_bytes(a.rows, a.V);
+    void* part = nullptr;
+    if (bytes) {
+        if (Workspace && tensor_bytes(Workspace) >= bytes && !((uintptr_t)Workspace->data & 15)) {
+            spread_layout(w, Workspace->data, a.rows, a.V);
+        } else if ((part = pool_alloc(bytes, true))) {
+            spread_layout(w, part, a.rows, a.V);
+        }
+    }
+    const Spread* spread = w.largest ? &w : nullptr;
+    if (dt == kF16) launch_sample<kF16>(a, spread, stream());
+    else if (dt == kBF16) launch_sample<kBF16>(a, spread, stream());
+    else launch_sample<kF32>(a, spread, stream());
     check_launch(name);
+    if (part) pool_free(part);
 }
+
+}  // extern "C"

@@ -1139,13 +1139,17 @@ class Sample(Ops):
     0 takes the largest logit.  The k largest logits are kept, of those the ones whose larger ones
     weigh less than p of all those, and of these the ones of at least min_p times the largest
     weight; equal logits rank by index.  Gives [token (``dtype``), logprob (float32)], both [rows].
-    ``vocab`` restricts the draw to the first columns.  Device tensors only."""
+    ``vocab`` restricts the draw to the first columns; a ``workspace`` of ``workspace_bytes(rows,
+    tokens)`` serves calls under graph capture.  Device tensors only."""
 
     def __init__(self, inputs, outputs, vocab=0, dtype="int32", version="1"):
         super().__init__(inputs, outputs)
         self.vocab = int(vocab)
         self.dtype = dtype
         self.version = version
+
+    def workspace_bytes(self, rows, tokens):
+        return int(self.lib.sample_workspace_bytes(int(rows), int(tokens)))
 
     def forward(self, logits: Tensor, uniform: Tensor, temperature: Tensor = None, top_k: Tensor = None,
                 top_p: Tensor = None, min_p: Tensor = None, workspace: Tensor = None):

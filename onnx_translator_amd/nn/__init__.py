@@ -235,6 +235,7 @@ class Ops:
                     _sig(lib, "prefix_cache_attention_forward", None, [P] * 9 + [V, P])
                     _sig(lib, "cache_plan_forward", None, [P] * 11 + [V])
                     _sig(lib, "sample_forward", None, [P] * 8 + [V, P])
+                    _sig(lib, "sample_workspace_bytes", ctypes.c_size_t, [ctypes.c_int, ctypes.c_int])
                     lib.init_cos_lut()
                     cls._lib = lib
                     cls._lib_initialized = True

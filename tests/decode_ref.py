@@ -20,6 +20,7 @@ class Dev(attention_ref.Dev):
                            ("sample_forward", [P] * 8 + [V, P])):
             f = getattr(self.lib, name)
             f.argtypes, f.restype = args, None
+        self.lib.sample_workspace_bytes.argtypes, self.lib.sample_workspace_bytes.restype = [ctypes.c_int] * 2, ctypes.c_size_t
 
 
 # ------------------------------------------------------------------------ plans ---

@@ -4,7 +4,7 @@ import math
 import numpy as np
 import pytest
 
-from tests.decode_ref import SampleProblem
+from tests.decode_ref import Dev, SampleProblem
 
 pytestmark = pytest.mark.gpu
 
@@ -50,7 +50,7 @@ def test_flat_rows(hip, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("v", [10, 5000, 20011])
+@pytest.mark.parametrize("v", [10, 5000, 20011, 40013])
 def test_equal_logits(hip, v, dtype):
     """Ties rank by index, at the top-k and the top-p border alike."""
     rng = np.random.default_rng(v)
@@ -82,11 +82,16 @@ def test_greedy(hip, dtype, t):
     x[3, 0] = 50.0
     tokens, lps = SampleProblem(x, u, dtype, t=t, k=5, p=0.5, m=0.1).check(hip)
     assert tokens[1:4].tolist() == [70, 8999, 0] and not lps.any()
+    wide = np.full((6, 70001), -5.0)
+    wide[:, 30000:39000] = x
+    tokens, lps = SampleProblem(wide, u, dtype, t=t, k=5, p=0.5, m=0.1).check(hip)
+    assert tokens[1:4].tolist() == [30070, 38999, 30000] and not lps.any()
 
 
+@pytest.mark.parametrize("v", [3001, 40003])
 @pytest.mark.parametrize("t", [1e-30, 1e-3, 50.0, 1e30, math.inf])
-def test_temperatures(hip, t):
-    x, u = logits(4, 3001, seed=4)
+def test_temperatures(hip, t, v):
+    x, u = logits(4, v, seed=4)
     SampleProblem(x, u, t=t).check(hip)
     SampleProblem(x, u, t=t, k=17).check(hip)
     SampleProblem(x, u, t=t, p=0.8317).check(hip)
@@ -94,16 +99,17 @@ def test_temperatures(hip, t):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("filters", list(FILTERS))
-def test_masked_logits(hip, dtype, filters):
+@pytest.mark.parametrize("v", [5003, 50003])
+def test_masked_logits(hip, v, dtype, filters):
     """-inf and NaN are never drawn; a row of nothing else gives -1."""
-    x, u = logits(6, 5003, seed=5)
+    x, u = logits(6, v, seed=5)
     rng = np.random.default_rng(6)
-    x[0, rng.random(5003) < 0.9] = -np.inf
+    x[0, rng.random(v) < 0.9] = -np.inf
     x[1] = -np.inf
     x[2] = np.nan
     x[3] = -np.inf
     x[3, 4321] = -3.0                                # one left
-    x[4, rng.random(5003) < 0.5] = np.nan
+    x[4, rng.random(v) < 0.5] = np.nan
     x[5, :5000] = -np.inf
     u[:] = [0.999, 0.5, 0.5, 0.9, 0.99, 0.9]
     tokens, lps = SampleProblem(x, u, dtype, t=[1.0, 1.0, 0.0, 0.7, 1.0, 1.0], **FILTERS[filters]).check(hip)
@@ -114,15 +120,20 @@ def test_masked_logits(hip, dtype, filters):
 @pytest.mark.parametrize("dtype", TYPES)
 def test_infinite_logits(hip, dtype):
     """+inf takes everything, several share alike."""
-    x, u = logits(4, 2000, seed=7)
-    x[:, [17, 900, 1500]] = np.inf
+    for v in (2000, 40001):
+        x, u = logits(4, v, seed=7)
+        x[:, [17, 900, 1500]] = np.inf
+        _infinite(hip, x, u, dtype)
+    low = np.full((2, 50), float(np.finfo(np.float16).min) if dtype == "float16" else -3e38)
+    SampleProblem(low, [0.3, 0.9], dtype, p=[1.0, 0.517]).check(hip)
+
+
+def _infinite(hip, x, u, dtype):
     for u0, want in ((0.0, 17), (0.4, 900), (0.9, 1500)):
         u[:] = u0
         for f in ({}, dict(p=0.99), dict(m=0.3), dict(k=3)):
             assert (SampleProblem(x, u, dtype, **f).check(hip)[0] == want).all()
         assert (SampleProblem(x, u, dtype, k=1).check(hip)[0] == 17).all()
-    low = np.full((2, 50), float(np.finfo(np.float16).min) if dtype == "float16" else -3e38)
-    SampleProblem(low, [0.3, 0.9], dtype, p=[1.0, 0.517]).check(hip)
 
 
 @pytest.mark.parametrize("u_type", ["float32", "float64"])
@@ -147,7 +158,7 @@ def test_settings_out_of_range(hip):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("columns,vocab", [(100, 99), (1001, 1), (9000, 8191), (8200, 8199)])
+@pytest.mark.parametrize("columns,vocab", [(100, 99), (1001, 1), (9000, 8191), (8200, 8199), (40000, 32761), (50000, 32760), (50001, 49999)])
 def test_part_of_the_columns(hip, dtype, columns, vocab):
     """Columns behind the vocabulary are no tokens, whatever they hold."""
     x, u = logits(4, columns, seed=columns)
@@ -178,10 +189,9 @@ def test_logits_off_their_alignment(hip):
     import torch
     from oracle import oracle as O
     from onnx_translator_amd.nn.Operators import CSampleParams
-    from tests.decode_ref import Dev
     for dtype, code in ((torch.float16, O.F16), (torch.bfloat16, O.BF16), (torch.float32, O.F32)):
         name = str(dtype).replace("torch.", "")
-        for v, skip in ((997, 0), (997, 1), (8193, 3), (20001, 5)):
+        for v, skip in ((997, 0), (997, 1), (8193, 3), (20001, 5), (32757, 7), (33001, 1), (50021, 3)):
             x, u = logits(3, v, seed=v + skip)
             p = SampleProblem(x, u, name, k=[0, 30, 7], p=[0.9, 1.0, 0.8])
             flat = torch.full((skip + 3 * v,), float("inf"), dtype=dtype, device="cuda")
@@ -196,6 +206,29 @@ def test_logits_off_their_alignment(hip):
                 dev.held.append(xt)
             assert (got == p.run(hip)[0]).all(), (name, v, skip)
             p.check(hip)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_very_many_columns(hip, dtype):
+    """More than a spread row may have: a block per row."""
+    v = 2100001
+    Dev(hip)
+    assert not hip.lib.sample_workspace_bytes(2, v)
+    x, u = logits(2, v, seed=13)
+    SampleProblem(x, u, dtype, k=[30, 0], p=[0.9, 0.8], t=[1.0, 0.9]).check(hip)
+
+
+@pytest.mark.parametrize("rows,v", [(3, 40000), (40, 33000)])
+def test_workspaces(hip, rows, v):
+    """The caller's, one too small (the pool serves) and the pool's: the same tokens."""
+    x, u = logits(rows, v, seed=14, tall=4)
+    p = SampleProblem(x, u, "bfloat16", p=np.linspace(0.5, 1.1, rows), m=np.linspace(0, 0.01, rows))
+    a = p.check(hip)
+    need = hip.lib.sample_workspace_bytes(rows, v)
+    assert need and not hip.lib.sample_workspace_bytes(rows, 32000)
+    for size in (need, need - 1, need + 1000):
+        b = p.run(hip, workspace=size)
+        assert (a[0] == b[0]).all() and (a[1] == b[1]).all(), size
 
 
 def test_the_distribution(hip):
