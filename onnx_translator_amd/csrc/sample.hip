@@ -89,13 +89,14 @@ struct Weights {
 };
 
 // ---- sums ---------------------------------------------------------------------------------
-template <int CTRL, int ROWS> __device__ __forceinline__ u64 lanes_before(u64 v) {      // (0 where there is none)
-    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xF, false);
-    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xF, false);
-    return ((u64)hi << 32) | lo;
+template <int CTRL, int ROWS> __device__ __forceinline__ unsigned lanes_before(unsigned v) {      // (0 where there is none)
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 lanes_before(u64 v) {
+    return ((u64)lanes_before<CTRL, ROWS>((unsigned)(v >> 32)) << 32) | lanes_before<CTRL, ROWS>((unsigned)v);
 }
 // Sums of the wave's lanes up to and with each.
-__device__ __forceinline__ u64 wave_scan(u64 v) {
+template <class T> __device__ __forceinline__ T wave_scan(T v) {
     v += lanes_before<0x111, 0xF>(v);                  // row_shr 1, 2, 4, 8: in rows of 16 lanes
     v += lanes_before<0x112, 0xF>(v);
     v += lanes_before<0x114, 0xF>(v);
@@ -480,14 +481,30 @@ template <int DT, int NT, bool HELD> struct SampleRow : RowChunks<DT> {
                 __builtin_amdgcn_sched_barrier(0);
             }
         } else {
-            uint4 next[PER];
-            raw(0, next);
-            for (int tile = 0; tile < tiles; tile++) {
-                float x[kEach];
+            // Eight chunks of a thread at once: a CU has a microsecond's way to memory, and one or two
+            // chunks of each thread on it are a tenth of what it could have.
+            constexpr int BATCH = 8 / PER;
+            for (int tile0 = 0; tile0 < tiles; tile0 += BATCH) {
+                uint4 q[BATCH][PER];
+                const int lo = tile0 * kTile - this->first;
+                if (lo >= 0 && lo + BATCH * kTile <= this->V) {
 #pragma unroll
-                for (int c = 0; c < PER; c++) Chunks::open(next[c], x + c * Chunks::VEC);
-                if (tile + 1 < tiles) raw(tile + 1, next);
-                f(tile, x);
+                    for (int i = 0; i < BATCH; i++)
+#pragma unroll
+                        for (int c = 0; c < PER; c++) q[i][c] = this->whole(index(tile0 + i) + c * Chunks::VEC);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < BATCH; i++)
+                        if (tile0 + i < tiles) raw(tile0 + i, q[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) {
+                    if (tile0 + i >= tiles) break;
+                    float x[kEach];
+#pragma unroll
+                    for (int c = 0; c < PER; c++) Chunks::open(q[i][c], x + c * Chunks::VEC);
+                    f(tile0 + i, x);
+                }
             }
         }
     }
@@ -669,34 +686,72 @@ template <int NT, class V> __device__ __forceinline__ float kth_bound(V visit, u
 }
 
 // Among the `count` ranks of the border's bin (weights above it: `above`) the last that top-p keeps;
-// kept(rank, weight) for those that min-p lets pass too.
+// kept(rank, weight), for every lane of a wave, with the weight 0 where it is not kept.  bins: LDS of
+// kBins.  Logits of 16 bits have few values, so many may be equal there: then as many are kept as
+// their weight goes into what is wanted, and the last one's index is found by counting.
 template <int NT, class F> __device__ __forceinline__ u64 border_in(u64* list, int count, u64 above, u64 want, const Settings& g, const Weights& w, u64* waves,
-                                                     u64* found, F kept) {
-    int n = 64;
-    while (n < count) n *= 2;
-    for (int i = count + (int)threadIdx.x; i < n; i += NT) list[i] = 0;
-    sort_falling<NT>(list, n);
+                                                     u64* found, unsigned* bins, int V, F kept) {
+    const int tid = (int)threadIdx.x;
     constexpr int E = kMost / NT;
-    u64 v[E], sum = 0, total;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int i = E * (int)threadIdx.x + e;
-        v[e] = i < count ? w.of(value_of(list[i])) : 0;
-        sum += v[e];
+    float lo = INFINITY, hi = -INFINITY;
+    for (int i = tid; i < count; i += NT) {
+        const float x = value_of(list[i]);
+        lo = fminf(lo, x);
+        hi = fmaxf(hi, x);
     }
-    if (threadIdx.x == 0) found[0] = ~0ull;
-    u64 before = above + Block<NT>::before(sum, waves, total);
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int i = E * (int)threadIdx.x + e;
-        if (i < count && before < want) {
-            atomicMin(&found[0], list[i]);
-            if (g.passes(w.log2_of(value_of(list[i])))) kept(list[i], v[e]);
+    lo = Block<NT>::reduce(lo, waves, Min());
+    hi = Block<NT>::reduce(hi, waves, Max());
+    u64 total, before;
+    if (lo == hi && count > 64) {
+        const u64 each = w.of(hi);
+        const int n = (int)min((want - above + each - 1) / each, (u64)count);        // (each > 0: the bin's weights pass want)
+        // the n-th smallest index: its bin of indices, then among that bin's
+        const int per = (V + kBins - 1) / kBins;
+        for (int i = tid; i < kBins; i += NT) bins[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < count; i += NT) atomicAdd(&bins[index_of(list[i]) / per], 1u);
+        __syncthreads();
+        const int bin = reach<NT, kBins / NT>([&](int i) { return (u64)bins[i]; }, (u64)n, waves, found, before, total);
+        __syncthreads();
+        unsigned* some_ = (unsigned*)(found + 1);
+        if (tid == 0) *some_ = 0;
+        __syncthreads();
+        for (int i = tid; i < count; i += NT)          // (at most kBins: in the bins' place)
+            if (index_of(list[i]) / per == bin) bins[atomicAdd(some_, 1u)] = (unsigned)index_of(list[i]);
+        __syncthreads();
+        const int some = (int)*some_, nth = n - (int)before;
+        for (int i = tid; i < some; i += NT) {
+            int less = 0;
+            for (int j = 0; j < some; j++) less += bins[j] < bins[i];
+            if (less == nth - 1) found[0] = rank_of(hi, (int)bins[i]);
         }
-        before += v[e];
+        __syncthreads();
+    } else {
+        int n = 64;
+        while (n < count) n *= 2;
+        for (int i = count + tid; i < n; i += NT) list[i] = 0;
+        sort_falling<NT>(list, n);
+        u64 v[E], sum = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            v[e] = E * tid + e < count ? w.of(value_of(list[E * tid + e])) : 0;
+            sum += v[e];
+        }
+        if (tid == 0) found[0] = ~0ull;
+        before = above + Block<NT>::before(sum, waves, total);
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            if (E * tid + e < count && before < want) atomicMin(&found[0], list[E * tid + e]);
+            before += v[e];
+        }
+        __syncthreads();
     }
-    __syncthreads();
     const u64 border = found[0];
+    for (int i = tid; i < (count + 63) / 64 * 64; i += NT) {
+        const u64 rank = i < count ? list[i] : 0;
+        const float x = value_of(rank);
+        kept(rank, rank && rank >= border && g.passes(w.log2_of(x)) ? w.of(x) : 0);
+    }
     __syncthreads();
     return border;
 }
@@ -736,6 +791,7 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
     }
     const Weights w = {finite(top), g.per, a.shift};
 
+    do {
     // ---- top-k, or min-p alone: few candidates, where few are above what none kept is below
     if (g.by_k || (!g.by_p && g.m > 0.0)) {
         float least = -INFINITY;
@@ -757,9 +813,7 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
             draw_candidates<NT>(a, row, g, w, s.c);
             return;
         }
-        __syncthreads();
-        draw_any<DT, NT>(a, row, r, g, w, s.h);
-        return;
+        break;
     }
     // ---- no filter, or top-p: the weights by their logarithm, then those above the border's bin by
     // tile, and the bin's own one by one
@@ -786,8 +840,7 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
         want = g.want(sum);
         bin = reach<NT, kBins / NT>([&](int i) { return h.bins[i]; }, want, h.waves, h.found, above, total);
         if (bin == kBins - 1) {                        // (among weights below 2^-40)
-            draw_any<DT, NT>(a, row, r, g, w, h);
-            return;
+            break;
         }
         __syncthreads();
         if (tid == 0) h.tile_ties[0] = 0;              // the bin's count; its ranks go where the bins were
@@ -826,13 +879,18 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
     if (g.by_p) {
         const int count = (int)h.tile_ties[0];
         if (count > kBins) {                           // (many equal ones)
-            draw_any<DT, NT>(a, row, r, g, w, h);
-            return;
+            break;
         }
-        border = border_in<NT>(h.bins, count, above, want, g, w, h.waves, h.found,
-                               [&](u64 rank, u64 v) { atomicAdd(&h.tile_mass[(index_of(rank) + r.first) / r.kTile], v); });
+        border = border_in<NT>(h.bins, count, above, want, g, w, h.waves, h.found, h.tile_ties, a.V, [&](u64 rank, u64 v) {
+            if (v) atomicAdd(&h.tile_mass[(index_of(rank) + r.first) / r.kTile], v);
+        });
     }
     draw_tile<DT, NT>(a, row, r, g, w, border, -FLT_MAX, h);
+    return;
+    } while (false);
+    // ---- too many candidates
+    __syncthreads();
+    draw_any<DT, NT>(a, row, r, g, w, s.h);
 }
 
 // ---- a row spread over blocks -----------------------------------------------------------------
@@ -842,7 +900,7 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
 // by the weights' logarithm; of every 16 the largest value.  A block per row goes on from those:
 // with top-k the few logits that can be kept, else the span that the draw falls into, and for a
 // border the logits whose logarithm is the border's.
-constexpr int kSpanThreads = 256, kSpan = 16 * kSpanThreads;
+constexpr int kSpanThreads = 256, kSpan = 16 * kSpanThreads, kPickThreads = 512;
 constexpr int kSpans = 512;                            // of a row at most
 constexpr int kLogBins = 128;                          // four to a factor of two, from a span's largest down
 constexpr int kNear = 12288;                           // logits of the border's bins
@@ -888,17 +946,22 @@ template <int DT> __global__ __launch_bounds__(kSpanThreads) void k_sample_spans
     u64 sum = 0;
     if (top > -INFINITY) {
         const Weights wt = {finite(top), g.per, a.shift};
-        if (!logs) {
-            sum = wt.sum(x);
-        } else {
-            const double from = grid_of(top, g.per);
+        const double from = logs ? grid_of(top, g.per) : 0.0;
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const u64 v = wt.of(x[e]);
-                const double b = __builtin_fmin(grid_of(x[e], g.per) - from, kLogBins - 1);
-                if (v) atomicAdd(&bins[(int)b], v);
-                sum += v;
+        for (int e0 = 0; e0 < 16; e0 += 4) {           // (four at a time: eight waves' registers on a SIMD)
+            float z[4] = {x[e0], x[e0 + 1], x[e0 + 2], x[e0 + 3]};
+            if (!logs) {
+                sum += wt.sum(z);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const u64 v = wt.of(z[e]);
+                    const double b = __builtin_fmin(grid_of(z[e], g.per) - from, kLogBins - 1);
+                    if (v) atomicAdd(&bins[(int)b], v);
+                    sum += v;
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     sum = B::reduce(sum, waves, Add());                // (and the bins are filled)
@@ -908,9 +971,9 @@ template <int DT> __global__ __launch_bounds__(kSpanThreads) void k_sample_spans
 
 // The span in which the sums of mass(span) pass the target, and the target within it.
 template <class M> __device__ __forceinline__ int pick_span(const SampleArgs& a, int64_t row, int spans, u64* waves, u64* found, M mass, u64& target, u64& all) {
-    const int i = 2 * (int)threadIdx.x;                // (at most 2 kRowThreads)
+    const int i = 2 * (int)threadIdx.x;                // (at most 2 kPickThreads)
     const u64 p = i < spans ? mass(i) : 0, q = i + 1 < spans ? mass(i + 1) : 0;
-    const u64 before = Block<kRowThreads>::before(p + q, waves, all);
+    const u64 before = Block<kPickThreads>::before(p + q, waves, all);
     target = draw_target(a, row, all);
     if (before <= target && target < before + p) { found[0] = (u64)i; found[1] = target - before; }
     else if (before + p <= target && target < before + p + q) { found[0] = (u64)i + 1; found[1] = target - before - p; }
@@ -919,23 +982,40 @@ template <class M> __device__ __forceinline__ int pick_span(const SampleArgs& a,
     return (int)found[0];
 }
 
+// The smallest key whose value holds(value) is true of, which it is of all larger ones: sixty-four
+// keys at a time.  (That of a NaN above all values: there is none.)
+template <class F> __device__ __forceinline__ uint32_t first_key(F holds) {
+    const uint32_t lane = threadIdx.x & 63, top = 0xFF800000u, bottom = 0x007FFFFFu;      // +inf, -inf
+    uint32_t not_yet = 0;
+#pragma unroll
+    for (int shift = 26; shift >= -4; shift -= 6) {
+        const int s = shift < 0 ? 0 : shift;
+        const uint32_t key = not_yet + (lane << s);
+        const bool yes = (shift < 0 && lane > 3) || key > top || (key > bottom && holds(of_key(key)));
+        const unsigned long long no = ~__ballot(yes);              // (lane 0's among them)
+        not_yet += (uint32_t)(63 - __builtin_clzll(no | 1)) << s;
+    }
+    return not_yet + 1;
+}
+
 struct PickShared {
     union {
-        SampleShared<kRowThreads> s;
+        SampleShared<kPickThreads> s;
         struct {
-            u64 waves[kRowThreads / 64], fine[kBins], row_bins[kLogBins];
+            u64 waves[kPickThreads / 64], fine[kBins], row_bins[kLogBins];
             u64 near[kNear];
         };
     };
     u64 kept[kSpans], found[2];
     unsigned count, count2;
 };
-static_assert(kSpan == 4 * kRowThreads, "logits of a thread in the drawn span");
+constexpr int kOwn = 8;                                // logits of a thread in the drawn span
+static_assert(kSpan == kOwn * kPickThreads, "the drawn span");
 
-template <int DT> __global__ __launch_bounds__(kRowThreads) void k_sample_pick(SampleArgs a, Spread w) {
+template <int DT> __global__ __launch_bounds__(kPickThreads) void k_sample_pick(SampleArgs a, Spread w) {
     __shared__ PickShared s;
-    typedef Block<kRowThreads> B;
-    constexpr int NT = kRowThreads, VEC = RowChunks<DT>::VEC;
+    typedef Block<kPickThreads> B;
+    constexpr int NT = kPickThreads, VEC = RowChunks<DT>::VEC;
     const int64_t row = blockIdx.x;
     const int tid = (int)threadIdx.x, lane = tid & 63;
     const float* largest = w.largest + row * w.spans;
@@ -949,24 +1029,23 @@ template <int DT> __global__ __launch_bounds__(kRowThreads) void k_sample_pick(S
         return;
     }
     const RowChunks<DT> r(a, row);
-    // A thread's four neighbouring logits of a span, and the first one's index.
-    auto logits = [&](int span, float (&x)[4]) {
-        const int i = span * kSpan + 4 * tid - r.first;
+    // A thread's neighbouring logits of a span, and the first one's index.
+    auto logits = [&](int span, float (&x)[kOwn]) {
+        const int i = span * kSpan + kOwn * tid - r.first, lo = span * kSpan + kOwn * (tid & ~63) - r.first;
+        uint4 q[kOwn / VEC];
+        r.chunks(__builtin_amdgcn_readfirstlane(lo), __builtin_amdgcn_readfirstlane(lo) + 64 * kOwn, [&](int c) { return i + c * VEC; }, q);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float v = i + e >= 0 && i + e < a.V ? (float)ld_d<DT>(a.x, row * a.ld + i + e) : -INFINITY;
-            x[e] = v != v ? -INFINITY : v;
-        }
+        for (int c = 0; c < kOwn / VEC; c++) RowChunks<DT>::open(q[c], x + c * VEC);
         return i;
     };
     if (g.greedy) {
         int at = 0x7FFFFFFF;
         for (int i = tid; i < w.spans; i += NT) at = largest[i] == top ? min(at, i) : at;
-        float x[4];
+        float x[kOwn];
         const int i = logits(B::reduce(at, s.waves, Min()), x);
         at = 0x7FFFFFFF;
 #pragma unroll
-        for (int e = 3; e >= 0; e--) at = x[e] == top ? i + e : at;
+        for (int e = kOwn - 1; e >= 0; e--) at = x[e] == top ? i + e : at;
         at = B::reduce(at, s.waves, Min());
         if (tid == 0) put_token(a, row, at, 0.0f);
         return;
@@ -978,11 +1057,11 @@ template <int DT> __global__ __launch_bounds__(kRowThreads) void k_sample_pick(S
     auto against_top = [&](u64 v, double factor) { return (u64)__builtin_rint((double)v * factor); };
     // Draws in a span among what keep(x, index, log2 of the weight) says.
     auto draw_span = [&](int span, u64 target, u64 all, auto keep) {
-        float x[4];
-        u64 v[4], mine = 0, total;
+        float x[kOwn];
+        u64 v[kOwn], mine = 0, total;
         const int i = logits(span, x);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
+        for (int e = 0; e < kOwn; e++) {
             const double y = wt.log2_of(x[e]);
             v[e] = x[e] > -INFINITY && keep(x[e], i + e, y) ? wt.of_log2(y) : 0;
             mine += v[e];
@@ -990,7 +1069,7 @@ template <int DT> __global__ __launch_bounds__(kRowThreads) void k_sample_pick(S
         u64 before = B::before(mine, s.waves, total);
         if (target >= total) target = total - 1;       // (its sum against its own largest value was rounded once more)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
+        for (int e = 0; e < kOwn; e++) {
             if (before <= target && target < before + v[e]) put_drawn(a, row, i + e, wt.log2_of(x[e]), all);
             before += v[e];
         }
@@ -1002,6 +1081,7 @@ template <int DT> __global__ __launch_bounds__(kRowThreads) void k_sample_pick(S
         draw_span(span, target, all, [](float, int, double) { return true; });
         return;
     }
+    do {
     const SampleRow<DT, NT, false> whole(a, row);
     if (g.by_k) {
         // ---- the few logits that can be among the k largest
@@ -1036,9 +1116,7 @@ template <int DT> __global__ __launch_bounds__(kRowThreads) void k_sample_pick(S
             draw_candidates<NT>(a, row, g, wt, s.s.c);
             return;
         }
-        __syncthreads();
-        draw_any<DT, NT>(a, row, whole, g, wt, s.s.h);
-        return;
+        break;
     }
 
     // ---- top-p, min-p: the row's weights by their logarithm
@@ -1082,9 +1160,7 @@ template <int DT> __global__ __launch_bounds__(kRowThreads) void k_sample_pick(S
         above = B::reduce(sum, s.waves, Add());
     }
     if (last >= kLogBins - 1) {                        // (among weights below 2^-31 of the largest)
-        __syncthreads();
-        draw_any<DT, NT>(a, row, whole, g, wt, s.s.h);
-        return;
+        break;
     }
     // the spans' weights above those bins
     for (int i = tid; i < w.spans; i += NT) s.kept[i] = 0;
@@ -1093,23 +1169,45 @@ template <int DT> __global__ __launch_bounds__(kRowThreads) void k_sample_pick(S
         const u64 sum = wave_allreduce((i < first ? p : 0) + (j < first ? q : 0), Add());
         if (lane == 0) s.kept[span] = sum;
     });
-    // and their logits in them
+    // and their logits in them, by the values that bound these bins; a wave finds the places of a
+    // tile's all at once
+    const float lo = of_key(first_key([&](float x) { return grid_of(x, g.per) - from <= last; }));
+    const float hi = of_key(first_key([&](float x) { return grid_of(x, g.per) - from < first; }));
+    const bool open_end = !(hi == hi);                 // (none is above)
     whole.each([&](int tile, const float (&x)[kEach]) {
+        unsigned in = 0;
+#pragma unroll
+        for (int e = 0; e < kEach; e++) in |= x[e] >= lo && (open_end || x[e] < hi) ? 1u << e : 0;
+        const unsigned n = (unsigned)__builtin_popcount(in), upto = wave_scan(n), sum = (unsigned)__builtin_amdgcn_readlane((int)upto, 63);
+        if (!sum) return;
+        unsigned at = lane == 0 ? atomicAdd(&s.count, sum) : 0;
+        at = (unsigned)__builtin_amdgcn_readfirstlane((int)at) + upto - n;
 #pragma unroll
         for (int e = 0; e < kEach; e++) {
-            const double b = grid_of(x[e], g.per) - from;
-            add_candidate(s.near, &s.count, kNear, b >= first && b <= last && x[e] > -INFINITY, x[e], whole.index(tile) + e);
+            if (in >> e & 1) {
+                if (at < kNear) s.near[at] = rank_of(x[e], whole.index(tile) + e);
+                at++;
+            }
         }
     });
     __syncthreads();
     if (s.count > kNear) {
-        __syncthreads();
-        draw_any<DT, NT>(a, row, whole, g, wt, s.s.h);
-        return;
+        break;
     }
     const int near = (int)s.count;
     u64 border = 0;
-    auto keep_near = [&](u64 rank, u64 v) { atomicAdd(&s.kept[(index_of(rank) + r.first) / kSpan], v); };
+    auto span_of = [&](u64 rank) { return (index_of(rank) + r.first) / kSpan; };
+    // Adds a wave's weights to their spans, mostly one or two (lanes adding to one place wait for each other).
+    auto keep = [&](u64 rank, u64 v) {
+        const int span = v ? span_of(rank) : -1;
+        for (unsigned long long todo = __ballot(v != 0); todo;) {
+            const int of = __builtin_amdgcn_readlane(span, __builtin_ctzll(todo));
+            const u64 sum = wave_allreduce(span == of ? v : 0, Add());
+            if (lane == 0) atomicAdd(&s.kept[of], sum);
+            todo &= ~__ballot(span == of);
+        }
+    };
+    const int near_all = (near + NT - 1) / NT * NT;    // (whole waves)
     if (g.by_p) {
         // the same once more in finer bins, by the logarithm's place between the first and the last
         const double y0 = -(from + first - 1) - wt.top * (g.per * 4.0), per_bin = kBins / (double)(last - first + 1);      // (4 log2 at the upper end)
@@ -1128,32 +1226,37 @@ template <int DT> __global__ __launch_bounds__(kRowThreads) void k_sample_pick(S
         int bin = reach<NT, kBins / NT>([&](int i) { return s.fine[i]; }, want - above, s.waves, s.found, over, total);
         if (bin < 0) bin = kBins;                      // (the sums were rounded: all of them)
         __syncthreads();
-        for (int i = tid; i < (near + NT - 1) / NT * NT; i += NT) {
+        for (int i = tid; i < near_all; i += NT) {
             const u64 rank = i < near ? s.near[i] : 0;
             const double y = rank ? wt.log2_of(value_of(rank)) : -100.0;
             const int b = rank ? fine_bin(y) : kBins + 1;
-            if (b < bin && g.passes(y)) keep_near(rank, wt.of_log2(y));
+            keep(rank, b < bin && g.passes(y) ? wt.of_log2(y) : 0);
             add_candidate(s.fine, &s.count2, kBins, b == bin, value_of(rank), index_of(rank));      // (in the bins' place)
         }
         __syncthreads();
         if (s.count2 > kBins) {                        // (many equal ones)
-            __syncthreads();
-            draw_any<DT, NT>(a, row, whole, g, wt, s.s.h);
-            return;
+            break;
         }
-        if (s.count2) border = border_in<NT>(s.fine, (int)s.count2, above + over, want, g, wt, s.waves, s.found, keep_near);
+        if (s.count2) border = border_in<NT>(s.fine, (int)s.count2, above + over, want, g, wt, s.waves, s.found, (unsigned*)s.near, a.V, keep);
     } else {
-        for (int i = tid; i < near; i += NT) {
-            const double y = wt.log2_of(value_of(s.near[i]));
-            if (g.passes(y)) keep_near(s.near[i], wt.of_log2(y));
+        for (int i = tid; i < near_all; i += NT) {
+            const u64 rank = i < near ? s.near[i] : 0;
+            const double y = rank ? wt.log2_of(value_of(rank)) : -100.0;
+            keep(rank, rank && g.passes(y) ? wt.of_log2(y) : 0);
         }
     }
     __syncthreads();
     u64 target, all;
     const int span = pick_span(a, row, w.spans, s.waves, s.found, [&](int i) { return s.kept[i]; }, target, all);
     draw_span(span, target, all, [&](float x, int i, double y) {
-        return rank_of(x, i) >= border && g.passes(y) && grid_of(x, g.per) - from <= last;
+        return x >= lo && rank_of(x, i) >= border && g.passes(y);
     });
+    return;
+    } while (false);
+    // ---- too many candidates
+    __syncthreads();
+    const SampleRow<DT, NT, false> whole(a, row);
+    draw_any<DT, NT>(a, row, whole, g, wt, s.s.h);
 }
 
 // Memory of a spread call: its parts for `rows` rows at base, and its size.
@@ -1177,7 +1280,7 @@ template <int DT> void launch_sample(const SampleArgs& a, const Spread* w, hipSt
     const unsigned rows = (unsigned)a.rows;
     if (w) {
         hipLaunchKernelGGL(k_sample_spans<DT>, dim3(rows * (unsigned)w->spans), dim3(kSpanThreads), 0, s, a, *w);
-        hipLaunchKernelGGL(k_sample_pick<DT>, dim3(rows), dim3(kRowThreads), 0, s, a, *w);
+        hipLaunchKernelGGL(k_sample_pick<DT>, dim3(rows), dim3(kPickThreads), 0, s, a, *w);
     } else if (a.V <= kShort) {
         hipLaunchKernelGGL((k_sample_row<DT, kShortThreads, true>), dim3(rows), dim3(kShortThreads), 0, s, a);
     } else if (a.V <= kLong) {
