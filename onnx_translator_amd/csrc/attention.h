@@ -162,6 +162,10 @@ struct AttnPlan {
 void launch_attention_f16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);
 void launch_attention_bf16(const AttnArgs& a, const AttnPlan& p, hipStream_t s);
 void launch_attention_f32(const AttnArgs& a, const AttnPlan& p, hipStream_t s);
+// Rows over a shared prefix and over their own keys, as partial results of both.
+void launch_prefix_f16(const AttnArgs& pre, const AttnPlan& p0, const AttnArgs& own, const AttnPlan& p1, hipStream_t s);
+void launch_prefix_bf16(const AttnArgs& pre, const AttnPlan& p0, const AttnArgs& own, const AttnPlan& p1, hipStream_t s);
+void launch_prefix_f32(const AttnArgs& pre, const AttnPlan& p0, const AttnArgs& own, const AttnPlan& p1, hipStream_t s);
 
 constexpr float kLog2e = 1.4426950408889634f;
 

@@ -122,8 +122,9 @@ struct AttnBlocks {
     int resident;                      // blocks on the GPU at once
 };
 
-// Whether the matrix kernels take the call; its block shape in p.
-bool attention_blocks(const AttnArgs& a, int es, bool paged, AttnPlan& p, AttnBlocks& k) {
+// Whether the matrix kernels take the call; its block shape in p.  rows: that the caller wants of a
+// block (0: by the call's own).
+bool attention_blocks(const AttnArgs& a, int es, bool paged, AttnPlan& p, AttnBlocks& k, int rows = 0) {
     const int vec = 16 / es, dm = a.Dk > a.Dv ? a.Dk : a.Dv;
     const int64_t per = paged ? (int64_t)a.T : (int64_t)a.Sq;      // tokens of a sequence at most
     if (!(dm <= 256 && a.Dk % vec == 0 && a.Dv % vec == 0 && per * a.G < 0x7FFFFF00 && a.kt * es < (1 << 26) &&
@@ -131,7 +132,7 @@ bool attention_blocks(const AttnArgs& a, int es, bool paged, AttnPlan& p, AttnBl
         return false;
     p.d = dm <= 64 ? 64 : dm <= 128 ? 128 : 256;
     const int64_t mean = paged ? ((int64_t)a.T * a.G + a.B - 1) / a.B : per * a.G;      // rows of a sequence
-    p.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 128;
+    p.rows = rows ? rows : mean <= 16 ? 16 : mean <= 32 ? 32 : 128;
     auto units_of = [&](int rows) {
         const int64_t t = paged ? (int64_t)a.T * a.G / rows + a.B : (per * a.G + rows - 1) / rows;
         return t * (paged ? 1 : a.B) * a.Hkv;
@@ -141,7 +142,7 @@ bool attention_blocks(const AttnArgs& a, int es, bool paged, AttnPlan& p, AttnBl
     // 256 538; of 64 values per head 120 and 100.  256 blocks over 300 .. 1500 keys: 35.6,
     // twice as many of 128 rows 33.7).  Not where a tile of their keys may lie on more pages
     // than a wave holds numbers of (pages of one key; tiles begin at multiples of 32).
-    if (p.rows == 128 && p.d * es <= 256 && es == 2 && (!paged || kKeys256 <= kTablePages * (int64_t)a.ps) &&
+    if (!rows && p.rows == 128 && p.d * es <= 256 && es == 2 && (!paged || kKeys256 <= kTablePages * (int64_t)a.ps) &&
         units_of(256) >= 2 * num_cus())
         p.rows = 256;
     k.units = units_of(p.rows);
@@ -237,14 +238,47 @@ void run_prefixed(AttnArgs& own, int dt, int64_t own_kv, int64_t prefix_kv, cons
     AttnPlan p0 = {kPaged, 0, 0, 0, false}, p1 = p0;
     AttnBlocks k0, k1;
     if (attention_blocks(pre, es, true, p0, k0) && attention_blocks(own, es, true, p1, k1)) {
-        int64_t share0 = attention_share(p0, k0, prefix_kv, kMaxSplits - 32), share1 = attention_share(p1, k1, own_kv, 32);
+        const int64_t rows = (int64_t)own.T * own.G;           // of a key head
+        const int cus = num_cus();
+        auto tiles_of = [&](int n) { return (rows + n - 1) / n * own.Hkv; };
+        // Time on the whole GPU of the prefix's products (64 keys of a block of 128 rows: 1.7 us with
+        // two blocks on a CU, at 128 values per head) and of the own keys' bytes, in us: lengths
+        // differ, so about half of the longest.
+        const double step = 1.7 * p0.d / 128, pre_us = (double)tiles_of(128) * (double)prefix_kv / 64 * step / (2 * cus);
+        const double own_us = 0.5 * own.B * own.Hkv * (double)own_kv * (own.Dk + own.Dv) * es / 4.5e6;
+        int64_t share0 = attention_share(p0, k0, prefix_kv, kMaxSplits - 32);
+        if (p0.rows == 32 && p1.rows == 16) attention_blocks(own, es, true, p1, k1, 32);      // (one launch for both)
+        int64_t share1 = attention_share(p1, k1, own_kv, 32);
         if (p0.rows >= 128) {
-            // two blocks for every CU's place: each split writes and reads a partial row of Dv
-            // float32 for what it saves in time
-            const int64_t split = std::max<int64_t>(1, 2 * num_cus() / (((int64_t)own.T * own.G + p0.rows - 1) / p0.rows * own.Hkv));
-            share0 = std::max<int64_t>((prefix_kv + split - 1) / split, 128);
-            share0 = std::max(share0, (prefix_kv + kMaxSplits - 33) / (kMaxSplits - 32));
-            share0 = (share0 + 31) / 32 * 32;
+            p0.rows = 0;
+            if (es == 2 && p0.d * es <= 256 && kKeys256 <= kTablePages * (int64_t)own.ps && pre_us > 2 * own_us) {
+                // Products are all there is: blocks of 256 rows, one to a CU, all of one length, in as
+                // many splits as fill the last round of them best.
+                double best = 0.7;
+                for (int n = 1; n <= 8; n++) {
+                    const int64_t blocks = tiles_of(256) * n;
+                    const double full = (double)blocks / (double)((blocks + cus - 1) / cus * cus) - 0.02 * n;
+                    if (full <= best || prefix_kv < 512 * n) continue;
+                    best = full;
+                    p0.rows = 256;
+                    share0 = (prefix_kv + n - 1) / n;
+                }
+            }
+            if (p0.rows) {
+                attention_blocks(pre, es, true, p0, k0, 256);
+            } else {
+                // Beside the own keys: blocks that take half of the time that both need, so that few
+                // partial results are written (each split writes and reads a row of Dv float32), but
+                // no more than fill the GPU where the prefix is all.
+                attention_blocks(pre, es, true, p0, k0, 128);
+                if (p1.rows == 256) {
+                    attention_blocks(own, es, true, p1, k1, 128);
+                    share1 = attention_share(p1, k1, own_kv, 32);
+                }
+                share0 = (int64_t)(64 * (pre_us + own_us) / (2 * step));
+                share0 = std::max<int64_t>({share0, prefix_kv * tiles_of(128) / (2 * cus), 256, (prefix_kv + 95) / 96});
+            }
+            share0 = (share0 + 127) / 128 * 128;
         }
         auto splits = [](int64_t kv, int64_t share) { return kv > share ? (kv + share - 1) / share : 1; };
         const int64_t each = own.rows * (own.Dv * 4 + 8);
@@ -268,13 +302,13 @@ void run_prefixed(AttnArgs& own, int dt, int64_t own_kv, int64_t prefix_kv, cons
             }
             part = pool_alloc((size_t)((n0 + n1) * each), true);
         }
-        if (part && launchable(p0, k0, n0) && launchable(p1, k1, n1)) {
+        if (part && launchable(p0, k0, n0 * 2) && launchable(p1, k1, n1 * 8)) {      // (both in one launch)
             AttnArgs all = own;
             all.nsplit = (int)(n0 + n1);
             all.parts = true;
             all.part_o = (float*)part;
             all.part_ml = (float2*)(all.part_o + all.nsplit * own.rows * own.Dv);
-            auto run = [&](AttnArgs& a, AttnPlan& p, const AttnBlocks& k, int64_t n, int64_t share, int64_t at) {
+            auto cut = [&](AttnArgs& a, AttnPlan& p, const AttnBlocks& k, int64_t n, int64_t share, int64_t at) {
                 a.nsplit = (int)n;
                 a.share = (int)share;
                 a.parts = true;
@@ -282,10 +316,10 @@ void run_prefixed(AttnArgs& own, int dt, int64_t own_kv, int64_t prefix_kv, cons
                 a.part_o = all.part_o + at * own.rows * own.Dv;
                 a.part_ml = all.part_ml + at * own.rows;
                 p.blocks = (unsigned)(k.units * n);
-                launch(a, p, dt);
             };
-            run(pre, p0, k0, n0, share0, 0);
-            run(own, p1, k1, n1, share1, n0);
+            cut(pre, p0, k0, n0, share0, 0);
+            cut(own, p1, k1, n1, share1, n0);
+            (dt == kF16 ? launch_prefix_f16 : dt == kBF16 ? launch_prefix_bf16 : launch_prefix_f32)(pre, p0, own, p1, stream());
             p1.blocks = 0;
             p1.join = true;
             launch(all, p1, dt);

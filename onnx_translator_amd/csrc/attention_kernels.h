@@ -350,9 +350,8 @@ template <bool PAGED> __device__ __forceinline__ AttnRow attn_row_at(const AttnA
     return w;
 }
 
-// false: nothing to do for this block (of `threads` threads).
-template <bool PAGED, int BM> __device__ __forceinline__ bool attn_block(const AttnArgs& a, int threads, AttnBlock& k) {
-    uint32_t bid = blockIdx.x;
+// Block `bid` of the call, of which this is thread `thread` of `threads`.  false: nothing to do for it.
+template <bool PAGED, int BM> __device__ __forceinline__ bool attn_block(const AttnArgs& a, uint32_t bid, int thread, int threads, AttnBlock& k) {
     k.hk = (int)(bid % (uint32_t)a.Hkv);
     bid /= (uint32_t)a.Hkv;
     k.split = (int)(bid % (uint32_t)a.nsplit);
@@ -394,7 +393,7 @@ template <bool PAGED, int BM> __device__ __forceinline__ bool attn_block(const A
         const int64_t at = (int64_t)k.klo + (int64_t)k.split * a.share;
         if (k.split + 1 < a.nsplit) k.khi = (int)min((int64_t)k.khi, at + a.share);      // the last one takes what is left
         if (at >= k.khi) {                     // no keys: it weighs nothing
-            for (int r = (int)threadIdx.x; r < k.rows; r += threads)
+            for (int r = thread; r < k.rows; r += threads)
                 a.part_ml[(int64_t)k.split * a.rows + attn_row_at<PAGED>(a, k, r).out] = make_float2(-INFINITY, 0.0f);
             return false;
         }
@@ -852,16 +851,15 @@ template <int DT, int D, bool PAGED, int MR, int W> struct AttnLoads {
 // by card or 1.0 PFLOP/s; the last 4096 of 16384 keys in pages of 16, 980 .. 1020 us (630 and
 // 1080 in the first hundred calls of an idle card, whose clock rises meanwhile).  With 64 values per head the
 // exponentials weigh twice as much.
-template <int DT, int D, bool PAGED, bool MASK, int W, int BN>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D * kElem<DT> <= 128 && W == 4 && !MASK ? 3 : D * kElem<DT> <= 256 ? 2 : 1))) void k_attn_tiles(AttnArgs a) {
+// (lds: four tiles of BN rows.)
+template <int DT, int D, bool PAGED, bool MASK, int W, int BN> TOHIP_INLINE __device__ void attn_tiles(const AttnArgs& a, uint32_t bid, char* lds, int& missing) {
     typedef AttnWave<DT, D, PAGED, MASK, 32, (D <= 128)> Wave;      // (as far as registers go)
     constexpr int RB = Wave::RB, NI = BN * RB / (1024 * W);
     static_assert(NI >= 1, "tile");
-    __shared__ __attribute__((aligned(1024))) char k0_[BN * RB], k1_[BN * RB], v0_[BN * RB], v1_[BN * RB];
-    __shared__ int missing;                    // a key's page was none of the cache's
+    char *k0_ = lds, *k1_ = lds + BN * RB, *v0_ = lds + 2 * BN * RB, *v1_ = lds + 3 * BN * RB;
     const int t = (int)threadIdx.x, wave = uniform(t >> 6);
     AttnBlock k;
-    if (!attn_block<PAGED, 32 * W>(a, 64 * W, k)) return;
+    if (!attn_block<PAGED, 32 * W>(a, bid, t, 64 * W, k)) return;
     Wave w;
     const AttnRow row = w.begin(a, k, wave * 32);
     AttnLoads<DT, D, PAGED, 32, W> ld;
@@ -907,6 +905,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D * kEle
     __syncthreads();
     if (wave * 32 < k.rows) w.end(a, k, wave * 32, row, missing != 0);
 }
+template <int DT, int D, bool PAGED, bool MASK, int W, int BN>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D * kElem<DT> <= 128 && W == 4 && !MASK ? 3 : D * kElem<DT> <= 256 ? 2 : 1))) void k_attn_tiles(AttnArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[4 * BN * D * kElem<DT>];
+    __shared__ int missing;                    // a key's page was none of the cache's
+    attn_tiles<DT, D, PAGED, MASK, W, BN>(a, blockIdx.x, lds, missing);
+}
 
 // Few rows: a block is one wave, so nothing waits for another.  K and V have two buffers of
 // 32 keys each; K's is filled again as soon as its scores are made and V's as soon as it is
@@ -917,13 +921,13 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D * kEle
 // than 64 values take 64 or 128 KB of LDS per wave and, for 256 values and 32 rows, more than 512
 // registers, so two waves or one run on a CU: 16 tokens of 16 heads over 130 .. 4096 keys of 4
 // heads reach 2.0 TB/s with 64 values, 2.2 with 128, 1.5 with 256.
-template <int DT, int D, bool PAGED, bool MASK, int MR>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D * kElem<DT> <= 256 ? 2 : 1))) void k_attn_few(AttnArgs a) {
+// (lds: four tiles of 32 rows.)
+template <int DT, int D, bool PAGED, bool MASK, int MR> TOHIP_INLINE __device__ void attn_few(const AttnArgs& a, uint32_t bid, char* lds) {
     typedef AttnWave<DT, D, PAGED, MASK, MR, (MR == 16 || D <= 128)> Wave;      // (as far as registers go)
     constexpr int RB = Wave::RB, NI = 32 * RB / 1024;
-    __shared__ __attribute__((aligned(1024))) char k0_[32 * RB], k1_[32 * RB], v0_[32 * RB], v1_[32 * RB];
+    char *k0_ = lds, *k1_ = lds + 32 * RB, *v0_ = lds + 64 * RB, *v1_ = lds + 96 * RB;
     AttnBlock k;
-    if (!attn_block<PAGED, MR>(a, 64, k)) return;
+    if (!attn_block<PAGED, MR>(a, bid, (int)threadIdx.x, 64, k)) return;
     Wave w;
     const AttnRow row = w.begin(a, k, 0);
     AttnLoads<DT, D, PAGED, MR, 1> ld;
@@ -978,6 +982,88 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D * kElem<DT
         }
     }
     w.end(a, k, 0, row, PAGED && ld.worst < 0);
+}
+template <int DT, int D, bool PAGED, bool MASK, int MR>
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D * kElem<DT> <= 256 ? 2 : 1))) void k_attn_few(AttnArgs a) {
+    __shared__ __attribute__((aligned(1024))) char lds[128 * D * kElem<DT>];
+    attn_few<DT, D, PAGED, MASK, MR>(a, blockIdx.x, lds);
+}
+
+// ---- behind a shared prefix --------------------------------------------------------------
+// The rows of all sequences over the prefix (pre) and each sequence's over its own keys (own), in one
+// launch where both are cut into blocks of one size: the first `first` blocks are the prefix's.
+// One after the other, the second part would wait for the first one's last block; and where the
+// prefix is bound by its products and single tokens by their keys' bytes, they run beside each other.
+template <int DT, int D, int MR>
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void k_prefix_few(AttnArgs pre, AttnArgs own, unsigned first) {
+    __shared__ __attribute__((aligned(1024))) char lds[128 * D * kElem<DT>];
+    if (blockIdx.x < first) attn_few<DT, D, true, false, MR>(pre, blockIdx.x, lds);
+    else attn_few<DT, D, true, false, MR>(own, blockIdx.x - first, lds);
+}
+template <int DT, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D * kElem<DT> <= 128 ? 3 : 2))) void k_prefix_tiles(AttnArgs pre, AttnArgs own, unsigned first) {
+    __shared__ __attribute__((aligned(1024))) char lds[256 * D * kElem<DT>];
+    __shared__ int missing;
+    if (blockIdx.x < first) attn_tiles<DT, D, true, false, 4, 64>(pre, blockIdx.x, lds, missing);
+    else attn_tiles<DT, D, true, false, 4, 64>(own, blockIdx.x - first, lds, missing);
+}
+// Few rows as one of a block's four waves that know nothing of each other, in a quarter of the LDS of
+// its tiles: one buffer for K and one for V, filled again as soon as they are read.  (Eight such waves
+// on a CU have as many bytes on their way as five with four buffers.)
+template <int DT, int D, int MR> TOHIP_INLINE __device__ void attn_few_wave(const AttnArgs& a, uint32_t bid, char* lds) {
+    typedef AttnWave<DT, D, true, false, MR, (MR == 16 || D <= 128)> Wave;
+    constexpr int RB = Wave::RB, NI = 32 * RB / 1024;
+    char *kt = lds, *vt = lds + 32 * RB;
+    AttnBlock k;
+    if (!attn_block<true, MR>(a, bid, (int)(threadIdx.x & 63), 64, k)) return;
+    Wave w;
+    const AttnRow row = w.begin(a, k, 0);
+    AttnLoads<DT, D, true, MR, 1> ld;
+    ld.begin(a, k, 0);
+    auto step = [&](int j0, bool next) TOHIP_INLINE {
+        float x[Wave::NP];
+        wait_loads<NI>();                      // (V's are on their way)
+        __builtin_amdgcn_sched_barrier(0);
+        w.products(kt, 0, x);
+        if (next) ld.template load<false, NI>(a, kt, j0 + 32);
+        __builtin_amdgcn_sched_barrier(0);
+        w.close(a, j0, x);
+        w.weigh(x);
+        if (next) wait_loads<NI>();
+        else wait_loads<0>();
+        __builtin_amdgcn_sched_barrier(0);
+        typename Wave::Weights p;
+        w.pack(x, p);
+        w.add(vt, 0, p);
+        if (next) {
+            ld.template load<true, NI>(a, vt, j0 + 32);
+            ld.template find<32>(a, j0 + 64);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (k.klo < k.khi) {
+        ld.template find<32>(a, k.klo);
+        w.have_q();
+        ld.template load<false, NI>(a, kt, k.klo);
+        ld.template load<true, NI>(a, vt, k.klo);
+        ld.template find<32>(a, k.klo + 32);
+        int j0 = k.klo;
+        for (; j0 + 32 < k.khi; j0 += 32) step(j0, true);
+        step(j0, false);
+    }
+    w.end(a, k, 0, row, ld.worst < 0);
+}
+template <int DT, int D, int MR>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k_prefix_both(AttnArgs pre, AttnArgs own, unsigned first, unsigned own_blocks) {
+    __shared__ __attribute__((aligned(1024))) char lds[256 * D * kElem<DT>];
+    __shared__ int missing;
+    if (blockIdx.x < first) {
+        attn_tiles<DT, D, true, false, 4, 64>(pre, blockIdx.x, lds, missing);
+    } else {
+        const int wave = uniform((int)threadIdx.x >> 6);
+        const unsigned bid = (blockIdx.x - first) * 4 + (unsigned)wave;
+        if (bid < own_blocks) attn_few_wave<DT, D, MR>(own, bid, lds + wave * 64 * D * kElem<DT>);
+    }
 }
 
 // ---- the splits of a row together -----------------------------------------------------
@@ -1157,6 +1243,33 @@ template <int DT> void launch_attention(const AttnArgs& a, const AttnPlan& p, hi
         if (paged) hipLaunchKernelGGL((k_attn_join<DT, true>), dim3(grid), dim3(256), 0, s, a);
         else hipLaunchKernelGGL((k_attn_join<DT, false>), dim3(grid), dim3(256), 0, s, a);
     }
+}
+
+// Both parts of a call behind a prefix (and not their join), in one launch where there is one for the
+// shapes of their blocks.
+template <int DT, int D> void launch_prefix_d(const AttnArgs& pre, const AttnPlan& p0, const AttnArgs& own, const AttnPlan& p1, hipStream_t s) {
+    const unsigned n = p0.blocks + p1.blocks;
+    if constexpr (D * kElem<DT> <= 256) {
+        if (p0.rows <= 32 && p0.rows == p1.rows) {
+            if (p0.rows == 16) hipLaunchKernelGGL((k_prefix_few<DT, D, 16>), dim3(n), dim3(64), 0, s, pre, own, p0.blocks);
+            else hipLaunchKernelGGL((k_prefix_few<DT, D, 32>), dim3(n), dim3(64), 0, s, pre, own, p0.blocks);
+            return;
+        }
+        if (p0.rows == 128) {
+            const unsigned some = p0.blocks + (p1.blocks + 3) / 4;
+            if (p1.rows == 128) hipLaunchKernelGGL((k_prefix_tiles<DT, D>), dim3(n), dim3(256), 0, s, pre, own, p0.blocks);
+            else if (p1.rows == 16) hipLaunchKernelGGL((k_prefix_both<DT, D, 16>), dim3(some), dim3(256), 0, s, pre, own, p0.blocks, p1.blocks);
+            else hipLaunchKernelGGL((k_prefix_both<DT, D, 32>), dim3(some), dim3(256), 0, s, pre, own, p0.blocks, p1.blocks);
+            return;
+        }
+    }
+    launch_tiles_of<DT, D, true, false>(pre, p0, s);
+    launch_tiles_of<DT, D, true, false>(own, p1, s);
+}
+template <int DT> void launch_prefix(const AttnArgs& pre, const AttnPlan& p0, const AttnArgs& own, const AttnPlan& p1, hipStream_t s) {
+    if (p0.d == 64) launch_prefix_d<DT, 64>(pre, p0, own, p1, s);
+    else if (p0.d == 128) launch_prefix_d<DT, 128>(pre, p0, own, p1, s);
+    else launch_prefix_d<DT, 256>(pre, p0, own, p1, s);
 }
 
 }  // namespace

@@ -131,9 +131,22 @@ def test_prefix_refuses(rec, kw, message):
 @pytest.mark.parametrize("kw", [dict(), dict(dt=O.F32), dict(ix=O.I64), dict(pix=O.I64), dict(ppages=(0,)), dict(pages=(3, 0)),
                                 dict(v=(12, 2, 16, 40)), dict(max_prefix=60, max_kv=9, scale=0.1)], ids=lambda v: str(v)[:60])
 def test_prefix_takes(rec, kw):
-    """Prefix, own keys, join."""
+    """Prefix and own keys in one launch, and their join."""
     launches, err = prefix(rec, **kw)
-    assert not err and len(launches) == 3 and launches[2].kernel.startswith("k_attn_join")
+    assert not err and len(launches) == 2 and launches[0].kernel.startswith("k_prefix") and launches[1].kernel.startswith("k_attn_join")
+
+
+@pytest.mark.parametrize("tokens,b,d,dt,kernels", [
+    (4, 4, 128, O.BF16, ["k_prefix_few<3, 128, 16>"]), (8, 8, 64, O.F32, ["k_prefix_few<4, 64, 32>"]),
+    (7, 1, 64, O.F16, ["k_prefix_few<2, 64, 32>"]), (64, 64, 128, O.BF16, ["k_prefix_both<3, 128, 16>"]),
+    (64, 10, 64, O.F16, ["k_prefix_both<2, 64, 32>"]), (300, 10, 64, O.F32, ["k_prefix_tiles<4, 64>"]),
+    (4096, 16, 128, O.BF16, ["k_attn_tiles<3, 128, true, false, 8, 128>"] * 2),
+    (64, 64, 128, O.F32, ["k_attn_tiles<4, 128, true, false, 4, 32>", "k_attn_few<4, 128, true, false, 16>"]),
+    (4, 4, 256, O.F16, ["k_attn_few<2, 256, true, false, 16>"] * 2)], ids=str)
+def test_prefix_kernels(rec, tokens, b, d, dt, kernels):
+    launches, err = prefix(rec, q=(tokens, 32, d), k=(2000, 8, 16, d), v=(2000, 8, 16, d), ppages=(512,), pages=(b, 8), start=(b + 1,),
+                           length=(b,), dt=dt)
+    assert not err and [l.kernel for l in launches[:-1]] == kernels and launches[-1].kernel.startswith("k_attn_join")
 
 
 @pytest.mark.parametrize("kw", [dict(q=(0, 8, 64)), dict(pages=(0, 4), start=(1,), length=(0,))], ids=["no tokens", "no sequences"])
@@ -151,7 +164,7 @@ def test_prefix_under_capture(rec):
             launches, err = prefix(rec, ws=ws)
             assert "needs a workspace" in err and not launches
         launches, err = prefix(rec, ws=two, ppages=(1000,))
-        assert not err and len(launches) == 3
+        assert not err and len(launches) == 2
         launches, err = prefix(rec, q=(10, 8, 63), k=(12, 2, 16, 63), v=(12, 2, 16, 63))
         assert not err and [l.kernel for l in launches] == ["k_prefix_rows<3>"]
     finally:
