@@ -246,14 +246,18 @@ void run_prefixed(AttnArgs& own, int dt, int64_t own_kv, int64_t prefix_kv, cons
         // differ, so about half of the longest.
         const double step = 1.7 * p0.d / 128, pre_us = (double)tiles_of(128) * (double)prefix_kv / 64 * step / (2 * cus);
         const double own_us = 0.5 * own.B * own.Hkv * (double)own_kv * (own.Dk + own.Dv) * es / 4.5e6;
-        int64_t share0 = attention_share(p0, k0, prefix_kv, kMaxSplits - 32);
+        // (three tiles at least: 4 tokens behind 2000 keys 14.9 us, 15.4 with two, 15.9 with four; 16
+        // behind 4097 in float32 23.5, 27.4 and 22.7)
+        int64_t share0 = std::max<int64_t>(attention_share(p0, k0, prefix_kv, kMaxSplits - 32), 96);
         if (p0.rows == 32 && p1.rows == 16) attention_blocks(own, es, true, p1, k1, 32);      // (one launch for both)
         int64_t share1 = attention_share(p1, k1, own_kv, 32);
         if (p0.rows >= 128) {
             p0.rows = 0;
-            if (es == 2 && p0.d * es <= 256 && kKeys256 <= kTablePages * (int64_t)own.ps && pre_us > 2 * own_us) {
+            if (es == 2 && p0.d * es <= 256 && kKeys256 <= kTablePages * (int64_t)own.ps && pre_us > std::max(2 * own_us, 100.0)) {
                 // Products are all there is: blocks of 256 rows, one to a CU, all of one length, in as
-                // many splits as fill the last round of them best.
+                // many splits as fill the last round of them best, and a launch for the own keys (2048
+                // tokens of 32 heads behind 16384 keys: 591 us, 647 by 128 rows and one launch; 704
+                // tokens of 24 behind 2501: 57 and 44).
                 double best = 0.7;
                 for (int n = 1; n <= 8; n++) {
                     const int64_t blocks = tiles_of(256) * n;
@@ -269,7 +273,8 @@ void run_prefixed(AttnArgs& own, int dt, int64_t own_kv, int64_t prefix_kv, cons
             } else {
                 // Beside the own keys: blocks that take half of the time that both need, so that few
                 // partial results are written (each split writes and reads a row of Dv float32), but
-                // no more than fill the GPU where the prefix is all.
+                // no more than fill the GPU where the prefix is all.  (64 tokens of 32 heads behind 8192
+                // keys: 46 us with 768 keys a split, 49 with 512, 51 with 1024.)
                 attention_blocks(pre, es, true, p0, k0, 128);
                 if (p1.rows == 256) {
                     attention_blocks(own, es, true, p1, k1, 128);

@@ -140,7 +140,7 @@ def test_prefix_takes(rec, kw):
     (4, 4, 128, O.BF16, ["k_prefix_few<3, 128, 16>"]), (8, 8, 64, O.F32, ["k_prefix_few<4, 64, 32>"]),
     (7, 1, 64, O.F16, ["k_prefix_few<2, 64, 32>"]), (64, 64, 128, O.BF16, ["k_prefix_both<3, 128, 16>"]),
     (64, 10, 64, O.F16, ["k_prefix_both<2, 64, 32>"]), (300, 10, 64, O.F32, ["k_prefix_tiles<4, 64>"]),
-    (4096, 16, 128, O.BF16, ["k_attn_tiles<3, 128, true, false, 8, 128>"] * 2),
+    (4096, 16, 128, O.BF16, ["k_attn_tiles<3, 128, true, false, 8, 128>"] * 2), (704, 12, 64, O.F16, ["k_prefix_tiles<2, 64>"]),
     (64, 64, 128, O.F32, ["k_attn_tiles<4, 128, true, false, 4, 32>", "k_attn_few<4, 128, true, false, 16>"]),
     (4, 4, 256, O.F16, ["k_attn_few<2, 256, true, false, 16>"] * 2)], ids=str)
 def test_prefix_kernels(rec, tokens, b, d, dt, kernels):
