@@ -259,158 +259,7 @@ template <int DT> struct RowChunks {
     }
 };
 
-// ---- few candidates --------------------------------------------------------------------------
-// Where the kept tokens are known to be among at most kMost candidates, these are ranked by value for
-// the filters and by index for the draw: up to kFew by counting the larger ones, which takes no
-// barrier between its reads (120 candidates: 2.4 us where a sort takes 5), more by sorting.
-constexpr int kMost = 2048, kFew = 256;
-
-template <int NT> struct Candidates {
-    u64 waves[Block<NT>::kWaves];
-    u64 rank[kMost], mass[kMost], order[kMost];
-    unsigned count;
-};
-
-// Adds the logits of a wave's lanes that are at least `least` to a list of at most `most` (every lane
-// calls); count goes on past it.
-__device__ __forceinline__ void add_candidate(u64* list, unsigned* count, unsigned most, bool in, float x, int i) {
-    const unsigned long long who = __ballot(in);
-    if (!who) return;
-    const int lane = (int)threadIdx.x & 63;
-    unsigned at = 0;
-    if (lane == __builtin_ctzll(who)) at = atomicAdd(count, (unsigned)__popcll(who));
-    at = (unsigned)__builtin_amdgcn_readlane((int)at, __builtin_ctzll(who)) + (unsigned)__popcll(who & ((1ull << lane) - 1));
-    if (in && at < most) list[at] = rank_of(x, i);
-}
-
-// n numbers in LDS, n a power of two, in falling order.
-template <int NT> __device__ __forceinline__ void sort_falling(u64* v, int n) {
-    for (int size = 2; size <= n; size *= 2) {
-        for (int step = size / 2; step > 0; step /= 2) {
-            __syncthreads();
-            for (int t = (int)threadIdx.x; t < n / 2; t += NT) {
-                const int i = 2 * t - (t & (step - 1)), j = i + step;
-                const u64 x = v[i], y = v[j];
-                if ((x < y) == ((i & size) == 0)) {
-                    v[i] = y;
-                    v[j] = x;
-                }
-            }
-        }
-    }
-    __syncthreads();
-}
-
-// Draws from the c.count <= kMost candidates of top-k or of min-p alone (they hold all that those keep).
-template <int NT> __device__ __forceinline__ void draw_candidates(const SampleArgs& a, int64_t row, const Settings& g, const Weights& w,
-                                                                  Candidates<NT>& c) {
-    const int tid = (int)threadIdx.x;
-    __syncthreads();
-    const int count = (int)c.count, most = g.by_k && g.k < count ? (int)g.k : count;
-    if (count <= kFew) {
-        // a candidate per thread; the larger ones and their weights, then the kept ones before it
-        const u64 mine = tid < count ? c.rank[tid] : 0;
-        const double y = mine ? w.log2_of(value_of(mine)) : -100.0;
-        const u64 own = mine ? w.of_log2(y) : 0;
-        if (tid < count) c.mass[tid] = own;
-        __syncthreads();
-        int larger = 0;
-        u64 above = 0;
-        if (tid < (count + 63) / 64 * 64) {
-#pragma unroll 4
-            for (int j = 0; j < count; j++) {
-                const bool l = c.rank[j] > mine;
-                larger += l;
-                above += l ? c.mass[j] : 0;
-            }
-        }
-        const bool ranked = mine && larger < most;
-        u64 total = 0;
-        if (g.by_p) total = Block<NT>::reduce(ranked ? own : 0, c.waves, Add());
-        const bool keep = ranked && (!g.by_p || above < g.want(total)) && g.passes(y);
-        if (tid < count) c.order[tid] = keep ? own : 0;
-        const u64 all = Block<NT>::reduce(keep ? own : 0, c.waves, Add());
-        const u64 target = draw_target(a, row, all);
-        u64 before = 0;
-        if (keep) {
-#pragma unroll 4
-            for (int j = 0; j < count; j++) before += (uint32_t)c.rank[j] > (uint32_t)mine ? c.order[j] : 0;      // (~index)
-            if (before <= target && target < before + own) put_drawn(a, row, index_of(mine), y, all);
-        }
-        return;
-    }
-    int n = 2 * kFew;
-    while (n < count) n *= 2;
-    for (int i = count + tid; i < n; i += NT) c.rank[i] = 0;
-    sort_falling<NT>(c.rank, n);
-    // neighbouring ranks in a thread
-    constexpr int E = kMost / NT;
-    u64 v[E], sum = 0, total, kept_here = 0;
-    double y[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int i = E * tid + e;
-        y[e] = i < most ? w.log2_of(value_of(c.rank[i])) : -100.0;
-        v[e] = i < most ? w.of_log2(y[e]) : 0;
-        sum += v[e];
-    }
-    u64 before = Block<NT>::before(sum, c.waves, total);
-    const u64 want = g.by_p ? g.want(total) : ~0ull;
-    bool keep[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        keep[e] = E * tid + e < most && before < want && g.passes(y[e]);
-        before += v[e];
-        kept_here += keep[e];
-    }
-    // (ranks are kept up to some rank, so their numbers are the kept ones')
-    const int kept = (int)Block<NT>::reduce(kept_here, c.waves, Add());
-    n = 64;
-    while (n < kept) n *= 2;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int i = E * tid + e;
-        if (i >= n) continue;
-        c.order[i] = keep[e] ? ((u64)(uint32_t)c.rank[i] << 32) | (unsigned)i : 0;      // (~index: falling order is rising index)
-        c.mass[i] = keep[e] ? v[e] : 0;
-    }
-    sort_falling<NT>(c.order, n);
-    int who[E];
-    sum = 0;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int i = E * tid + e;
-        who[e] = i < kept ? (int)(uint32_t)c.order[i] : -1;
-        v[e] = who[e] >= 0 ? c.mass[who[e]] : 0;
-        sum += v[e];
-    }
-    before = Block<NT>::before(sum, c.waves, total);
-    const u64 target = draw_target(a, row, total);
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        if (before <= target && target < before + v[e])
-            put_drawn(a, row, index_of(c.rank[who[e]]), w.log2_of(value_of(c.rank[who[e]])), total);
-        before += v[e];
-    }
-}
-
-// ---- any number of candidates, in one block ---------------------------------------------------
-constexpr int kEach = 8;                               // logits of a thread in a tile, in index order
-constexpr int kHeld = 4;                               // tiles that a block holds in registers
 constexpr int kBins = 2048;
-constexpr int kMaxTiles = 2048, kRowThreads = 1024, kShortThreads = 256;      // (16 M columns)
-
-template <int NT> struct Histograms {
-    u64 waves[Block<NT>::kWaves];
-    u64 bins[kBins];
-    u64 tile_mass[kMaxTiles];
-    uint32_t tile_ties[kMaxTiles];
-    u64 found[2];
-};
-template <int NT> union SampleShared {
-    Histograms<NT> h;
-    Candidates<NT> c;
-};
 
 // The first of n sums (thread t has those from n / NT t on, by at(i)) up to and with which they reach
 // `want` (from 1 on): its number and the sum before it; -1: they do not.  found: LDS of two.
@@ -437,6 +286,251 @@ template <int NT, int N, class AT> __device__ __forceinline__ int reach(AT at, u
     before = found[1];
     return (int)found[0];
 }
+
+// ---- few candidates --------------------------------------------------------------------------
+// Where the kept tokens are known to be among at most kMost candidates these go on without the row.
+// Up to kFew are ranked by counting the larger ones, which takes no barrier between its reads; of
+// more the border is found in bins of the value, and only its bin's are ranked (600 candidates: two
+// sorts took 25 us).
+constexpr int kMost = 2048, kFew = 128;
+
+template <int NT> struct Candidates {
+    u64 waves[Block<NT>::kWaves], found[2];
+    u64 rank[kMost], bins[kBins];
+    u64 few[kMost];                    // ranks; up to kFew: with their amounts behind them
+    unsigned count, few_count;
+};
+
+// Adds the logits of a wave's lanes that the bits of `in` name to a list of at most `most` (every lane
+// calls: their places are found all at once); count goes on past it.
+template <int N, class I> __device__ __forceinline__ void add_candidates(u64* list, unsigned* count, unsigned most, unsigned in, const float (&x)[N], I index) {
+    const unsigned n = (unsigned)__builtin_popcount(in), upto = wave_scan(n), sum = (unsigned)__builtin_amdgcn_readlane((int)upto, 63);
+    if (!sum) return;
+    unsigned at = ((int)threadIdx.x & 63) == 0 ? atomicAdd(count, sum) : 0;
+    at = (unsigned)__builtin_amdgcn_readfirstlane((int)at) + upto - n;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        if (in >> e & 1) {
+            if (at < most) list[at] = rank_of(x[e], index(e));
+            at++;
+        }
+    }
+}
+
+// f(rank, amount) for n ranks and amounts in LDS (which have room for a multiple of eight), eight reads
+// of each at a time: one after the other they wait for LDS 128 cycles each.
+template <class F> __device__ __forceinline__ void each_few(const u64* rank, const u64* amount, int n, F f) {
+    for (int j = 0; j < n; j += 8) {
+        u64 r[8], v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) r[e] = rank[j + e];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = amount[j + e];
+#pragma unroll
+        for (int e = 0; e < 8; e++) f(r[e], j + e < n ? v[e] : 0);
+    }
+}
+
+// n numbers in LDS, n a power of two, in falling order.  (Pairs at most 64 apart lie in one wave's part.)
+template <int NT> __device__ __forceinline__ void sort_falling(u64* v, int n) {
+    __syncthreads();
+    for (int size = 2; size <= n; size *= 2) {
+        for (int step = size / 2; step > 0; step /= 2) {
+            if (step >= 64) __syncthreads();
+            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            for (int t = (int)threadIdx.x; t < n / 2; t += NT) {
+                const int i = 2 * t - (t & (step - 1)), j = i + step;
+                const u64 x = v[i], y = v[j];
+                if ((x < y) == ((i & size) == 0)) {
+                    v[i] = y;
+                    v[j] = x;
+                }
+            }
+            if (step == 64) __syncthreads();
+        }
+    }
+    __syncthreads();
+}
+
+// Of the ranks in a list, from the largest down, the last one before which amounts of less than `want`
+// lie, `base` among them (0: all are such).  amount(rank): 0 for one that does not count.  lo, hi: bounds
+// of their values.  bins: LDS of kBins, few of kMost.
+template <int NT, class A> __device__ __forceinline__ u64 border_of(u64* list, int count, float lo, float hi, u64 base, u64 want, A amount, u64* bins, u64* few,
+                                                    unsigned* few_count, u64* waves, u64* found) {
+    const int tid = (int)threadIdx.x;
+    u64 above = base, total;
+    int n = count;
+    u64* from = list;
+    if (count > kFew) {
+        const float scale = (float)(kBins - 1) / (hi - lo);
+        auto bin_of = [&](u64 rank) {                  // (NaN of equal or infinite ones: bin 0)
+            const float f = (hi - value_of(rank)) * scale;
+            return f > 0.0f ? (int)fminf(f, kBins - 1) : 0;
+        };
+        __syncthreads();
+        for (int i = tid; i < kBins; i += NT) bins[i] = 0;
+        if (tid == 0) *few_count = 0;
+        __syncthreads();
+        for (int i = tid; i < count; i += NT) {
+            const u64 v = amount(list[i]);
+            if (v) atomicAdd(&bins[bin_of(list[i])], v);
+        }
+        __syncthreads();
+        const int bin = reach<NT, kBins / NT>([&](int i) { return bins[i]; }, want - base, waves, found, above, total);
+        above += base;
+        if (bin < 0) return 0;
+        for (int i = tid; i < count; i += NT)
+            if (bin_of(list[i]) == bin && amount(list[i])) few[atomicAdd(few_count, 1u)] = list[i];
+        __syncthreads();
+        n = (int)*few_count;
+        from = few;
+    }
+    if (tid == 0) found[0] = ~0ull;
+    if (n <= kFew) {
+        const u64 mine = tid < n ? from[tid] : 0, own = mine ? amount(mine) : 0;
+        u64* amounts = few + kFew;
+        if (tid < n) amounts[tid] = own;
+        __syncthreads();
+        u64 before = above, all = above;
+        if (tid < (n + 63) / 64 * 64) {
+            each_few(from, amounts, n, [&](u64 rank, u64 v) {
+                before += rank > mine ? v : 0;
+                all += v;
+            });
+        }
+        if (tid == 0) found[1] = all;
+        if (own && before < want) atomicMin(&found[0], mine);
+        __syncthreads();
+        const u64 border = found[1] < want ? 0 : found[0];
+        __syncthreads();
+        return border;
+    }
+    int m = 2 * kFew;
+    while (m < n) m *= 2;
+    for (int i = n + tid; i < m; i += NT) few[i] = 0;
+    sort_falling<NT>(few, m);
+    constexpr int E = kMost / NT;
+    u64 v[E], sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        v[e] = E * tid + e < n ? amount(few[E * tid + e]) : 0;
+        sum += v[e];
+    }
+    u64 before = above + Block<NT>::before(sum, waves, total);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        if (v[e] && before < want) atomicMin(&found[0], few[E * tid + e]);
+        before += v[e];
+    }
+    __syncthreads();
+    const u64 border = found[0];
+    __syncthreads();
+    return border;
+}
+
+// Draws from the c.count <= kMost candidates of top-k or of min-p alone (they hold all that those keep;
+// none is below `least`).
+template <int NT> __device__ __forceinline__ void draw_candidates(const SampleArgs& a, int64_t row, const Settings& g, const Weights& w, float least, float top,
+                                                                  Candidates<NT>& c) {
+    const int tid = (int)threadIdx.x;
+    __syncthreads();
+    const int count = (int)c.count, most = g.by_k && g.k < count ? (int)g.k : count;
+    if (count <= kFew) {
+        // a candidate per thread; the larger ones and their weights, then the kept ones before it
+        u64 *mass = c.few, *kept = c.few + kFew;
+        const u64 mine = tid < count ? c.rank[tid] : 0;
+        const double y = mine ? w.log2_of(value_of(mine)) : -100.0;
+        const u64 own = mine ? w.of_log2(y) : 0;
+        if (tid < (count + 7) / 8 * 8) {
+            c.rank[tid] = mine;                        // (0 behind the last)
+            mass[tid] = own;
+        }
+        __syncthreads();
+        int larger = 0;
+        u64 above = 0;
+        if (tid < (count + 63) / 64 * 64) {
+            each_few(c.rank, mass, count, [&](u64 rank, u64 v) {
+                larger += rank > mine;
+                above += rank > mine ? v : 0;
+            });
+        }
+        const bool ranked = mine && larger < most;
+        u64 total = 0;
+        if (g.by_p) total = Block<NT>::reduce(ranked ? own : 0, c.waves, Add());
+        const bool keep = ranked && (!g.by_p || above < g.want(total)) && g.passes(y);
+        if (tid < count) kept[tid] = keep ? own : 0;
+        const u64 all = Block<NT>::reduce(keep ? own : 0, c.waves, Add());
+        const u64 target = draw_target(a, row, all);
+        u64 before = 0;
+        if (keep) {
+            each_few(c.rank, kept, count, [&](u64 rank, u64 v) { before += (uint32_t)rank > (uint32_t)mine ? v : 0; });      // (~index)
+            if (before <= target && target < before + own) put_drawn(a, row, index_of(mine), y, all);
+        }
+        return;
+    }
+    if (!(least > -INFINITY)) {                        // (few logits in all)
+        least = top;
+        for (int i = tid; i < count; i += NT) least = fminf(least, value_of(c.rank[i]));
+        least = Block<NT>::reduce(least, c.waves, Min());
+    }
+    u64 border = 0, total;
+    if (most < count)
+        border = border_of<NT>(c.rank, count, least, top, 0, (u64)most, [](u64) { return (u64)1; }, c.bins, c.few, &c.few_count, c.waves, c.found);
+    if (g.by_p) {
+        auto weight = [&](u64 rank) { return rank >= border ? w.of(value_of(rank)) : 0; };
+        u64 sum = 0;
+        for (int i = tid; i < count; i += NT) sum += weight(c.rank[i]);
+        sum = Block<NT>::reduce(sum, c.waves, Add());
+        const u64 by_p = border_of<NT>(c.rank, count, least, top, 0, g.want(sum), weight, c.bins, c.few, &c.few_count, c.waves, c.found);
+        border = by_p > border ? by_p : border;
+    }
+    // the kept weights by index, then those of the bin that the target falls into
+    const int per = (a.V + kBins - 1) / kBins;
+    auto kept = [&](u64 rank) {
+        const double y = w.log2_of(value_of(rank));
+        return rank >= border && g.passes(y) ? w.of_log2(y) : 0;
+    };
+    __syncthreads();
+    for (int i = tid; i < kBins; i += NT) c.bins[i] = 0;
+    if (tid == 0) c.few_count = 0;
+    __syncthreads();
+    u64 sum = 0;
+    for (int i = tid; i < count; i += NT) {
+        const u64 v = kept(c.rank[i]);
+        if (v) atomicAdd(&c.bins[index_of(c.rank[i]) / per], v);
+        sum += v;
+    }
+    const u64 all = Block<NT>::reduce(sum, c.waves, Add()), target = draw_target(a, row, all);
+    u64 before;
+    const int bin = reach<NT, kBins / NT>([&](int i) { return c.bins[i]; }, target + 1, c.waves, c.found, before, total);
+    for (int i = tid; i < count; i += NT)
+        if (index_of(c.rank[i]) / per == bin && kept(c.rank[i])) c.few[atomicAdd(&c.few_count, 1u)] = c.rank[i];
+    __syncthreads();
+    const int n = (int)c.few_count;
+    for (int i = tid; i < n; i += NT) {
+        const u64 mine = c.few[i], own = kept(mine);
+        u64 at = before;
+        for (int j = 0; j < n; j++) at += (uint32_t)c.few[j] > (uint32_t)mine ? kept(c.few[j]) : 0;
+        if (at <= target && target < at + own) put_drawn(a, row, index_of(mine), w.log2_of(value_of(mine)), all);
+    }
+}
+
+// ---- any number of candidates, in one block ---------------------------------------------------
+constexpr int kEach = 8;                               // logits of a thread in a tile, in index order
+constexpr int kHeld = 4;                               // tiles that a block holds in registers
+constexpr int kMaxTiles = 2048, kRowThreads = 1024, kShortThreads = 256;      // (16 M columns)
+
+template <int NT> struct Histograms {
+    u64 waves[Block<NT>::kWaves];
+    u64 bins[kBins];
+    u64 tile_mass[kMaxTiles];
+    uint32_t tile_ties[kMaxTiles];
+    u64 found[2];
+};
+template <int NT> union SampleShared {
+    Histograms<NT> h;
+    Candidates<NT> c;
+};
 
 // A row in tiles, from its first chunk on; HELD: all of them (at most kHeld) stay in registers.
 template <int DT, int NT, bool HELD> struct SampleRow : RowChunks<DT> {
@@ -804,13 +898,14 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
         if (tid == 0) s.c.count = 0;
         __syncthreads();
         r.each([&](int tile, const float (&x)[kEach]) {
+            unsigned in = 0;
 #pragma unroll
-            for (int e = 0; e < kEach; e++)
-                add_candidate(s.c.rank, &s.c.count, kMost, x[e] >= least && x[e] > -INFINITY, x[e], r.index(tile) + e);
+            for (int e = 0; e < kEach; e++) in |= x[e] >= least && x[e] > -INFINITY ? 1u << e : 0;
+            add_candidates(s.c.rank, &s.c.count, kMost, in, x, [&](int e) { return r.index(tile) + e; });
         });
         __syncthreads();
         if (s.c.count <= kMost) {
-            draw_candidates<NT>(a, row, g, w, s.c);
+            draw_candidates<NT>(a, row, g, w, least, top, s.c);
             return;
         }
         break;
@@ -852,13 +947,15 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
         if (!g.by_p) {
             sum = w.sum(x);
         } else {
+            unsigned in = 0;
 #pragma unroll
             for (int e = 0; e < kEach; e++) {
                 const double y = w.log2_of(x[e]);
                 const int b = log_bin(y);
                 if (b < bin && g.passes(y)) sum += w.of_log2(y);
-                add_candidate(h.bins, &h.tile_ties[0], kBins, b == bin, x[e], r.index(tile) + e);
+                in |= b == bin ? 1u << e : 0;
             }
+            add_candidates(h.bins, &h.tile_ties[0], kBins, in, x, [&](int e) { return r.index(tile) + e; });
         }
         if constexpr (HELD) {
             mass[tile] = sum;
@@ -1099,21 +1196,24 @@ template <int DT> __global__ __launch_bounds__(kPickThreads) void k_sample_pick(
         __syncthreads();
         for (int i0 = 0; i0 < groups && s.s.c.count <= kMost; i0 += NT) {
             const int i = i0 + tid;
-            const bool in = i < groups && group[i] >= least && group[i] > -INFINITY;
-            if (!__ballot(in)) continue;
+            const bool near = i < groups && group[i] >= least && group[i] > -INFINITY;
+            if (!__ballot(near)) continue;
+            float x[16];
+            unsigned in = 0;
+            const int span = i / kSpanThreads, of = i % kSpanThreads;
+            if (near) {
+                uint4 q[16 / VEC];
+                r.chunks(span_index<DT>(r, span, of, 0), span_index<DT>(r, span, of, 16 / VEC - 1) + VEC, [&](int c) { return span_index<DT>(r, span, of, c); }, q);
 #pragma unroll
-            for (int c = 0; c < 16 / VEC; c++) {
-                float x[VEC];
-                const int at = span_index<DT>(r, i / kSpanThreads, i % kSpanThreads, c);
-                RowChunks<DT>::open(in ? r.part(at) : uint4{0, 0, 0, 0}, x);
+                for (int c = 0; c < 16 / VEC; c++) RowChunks<DT>::open(q[c], x + c * VEC);
 #pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    add_candidate(s.s.c.rank, &s.s.c.count, kMost, in && x[e] >= least && x[e] > -INFINITY, x[e], at + e);
+                for (int e = 0; e < 16; e++) in |= x[e] >= least && x[e] > -INFINITY ? 1u << e : 0;
             }
+            add_candidates(s.s.c.rank, &s.s.c.count, kMost, in, x, [&](int e) { return span_index<DT>(r, span, of, e / VEC) + e % VEC; });
         }
         __syncthreads();
         if (s.s.c.count <= kMost) {
-            draw_candidates<NT>(a, row, g, wt, s.s.c);
+            draw_candidates<NT>(a, row, g, wt, least, top, s.s.c);
             return;
         }
         break;
@@ -1178,17 +1278,7 @@ template <int DT> __global__ __launch_bounds__(kPickThreads) void k_sample_pick(
         unsigned in = 0;
 #pragma unroll
         for (int e = 0; e < kEach; e++) in |= x[e] >= lo && (open_end || x[e] < hi) ? 1u << e : 0;
-        const unsigned n = (unsigned)__builtin_popcount(in), upto = wave_scan(n), sum = (unsigned)__builtin_amdgcn_readlane((int)upto, 63);
-        if (!sum) return;
-        unsigned at = lane == 0 ? atomicAdd(&s.count, sum) : 0;
-        at = (unsigned)__builtin_amdgcn_readfirstlane((int)at) + upto - n;
-#pragma unroll
-        for (int e = 0; e < kEach; e++) {
-            if (in >> e & 1) {
-                if (at < kNear) s.near[at] = rank_of(x[e], whole.index(tile) + e);
-                at++;
-            }
-        }
+        add_candidates(s.near, &s.count, kNear, in, x, [&](int e) { return whole.index(tile) + e; });
     });
     __syncthreads();
     if (s.count > kNear) {
@@ -1231,7 +1321,8 @@ template <int DT> __global__ __launch_bounds__(kPickThreads) void k_sample_pick(
             const double y = rank ? wt.log2_of(value_of(rank)) : -100.0;
             const int b = rank ? fine_bin(y) : kBins + 1;
             keep(rank, b < bin && g.passes(y) ? wt.of_log2(y) : 0);
-            add_candidate(s.fine, &s.count2, kBins, b == bin, value_of(rank), index_of(rank));      // (in the bins' place)
+            const float x[1] = {value_of(rank)};
+            add_candidates(s.fine, &s.count2, kBins, b == bin ? 1u : 0, x, [&](int) { return index_of(rank); });      // (in the bins' place)
         }
         __syncthreads();
         if (s.count2 > kBins) {                        // (many equal ones)
