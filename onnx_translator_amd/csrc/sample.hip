@@ -796,7 +796,7 @@ template <int NT, class F> __device__ __forceinline__ u64 border_in(u64* list, i
     lo = Block<NT>::reduce(lo, waves, Min());
     hi = Block<NT>::reduce(hi, waves, Max());
     u64 total, before;
-    if (lo == hi && count > 64) {
+    if (lo == hi && count > kFew) {
         const u64 each = w.of(hi);
         const int n = (int)min((want - above + each - 1) / each, (u64)count);        // (each > 0: the bin's weights pass want)
         // the n-th smallest index: its bin of indices, then among that bin's
@@ -819,6 +819,11 @@ template <int NT, class F> __device__ __forceinline__ u64 border_in(u64* list, i
             for (int j = 0; j < some; j++) less += bins[j] < bins[i];
             if (less == nth - 1) found[0] = rank_of(hi, (int)bins[i]);
         }
+        __syncthreads();
+    } else if (count <= kFew) {
+        // (behind the list is room)
+        const u64 b = border_of<NT>(list, count, lo, hi, above, want, [&](u64 rank) { return w.of(value_of(rank)); }, list, list + kMost / 2, nullptr, waves, found);
+        if (tid == 0) found[0] = b;
         __syncthreads();
     } else {
         int n = 64;
@@ -850,6 +855,22 @@ template <int NT, class F> __device__ __forceinline__ u64 border_in(u64* list, i
     return border;
 }
 
+// The smallest key whose value holds(value) is true of, which it is of all larger ones: sixty-four
+// keys at a time.  (That of a NaN above all values: there is none.)
+template <class F> __device__ __forceinline__ uint32_t first_key(F holds) {
+    const uint32_t lane = threadIdx.x & 63, top = 0xFF800000u, bottom = 0x007FFFFFu;      // +inf, -inf
+    uint32_t not_yet = 0;
+#pragma unroll
+    for (int shift = 26; shift >= -4; shift -= 6) {
+        const int s = shift < 0 ? 0 : shift;
+        const uint32_t key = not_yet + (lane << s);
+        const bool yes = (shift < 0 && lane > 3) || key > top || (key > bottom && holds(of_key(key)));
+        const unsigned long long no = ~__ballot(yes);              // (lane 0's among them)
+        not_yet += (uint32_t)(63 - __builtin_clzll(no | 1)) << s;
+    }
+    return not_yet + 1;
+}
+
 // Bins of a weight's logarithm from the largest down.
 __device__ __forceinline__ int log_bin(double y) { return min((int)(y * -51.0), kBins - 1); }      // (51 to a factor of two: 40 of them)
 
@@ -864,10 +885,13 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
 
     // ---- the largest value
     float most = -INFINITY;
-    r.each([&](int, const float (&x)[kEach]) {
+    auto largest = [](const float (&x)[kEach]) {
+        float v = x[0];
 #pragma unroll
-        for (int e = 0; e < kEach; e++) most = fmaxf(most, x[e]);
-    });
+        for (int e = 1; e < kEach; e++) v = fmaxf(v, x[e]);
+        return v;
+    };
+    r.each([&](int, const float (&x)[kEach]) { most = fmaxf(most, largest(x)); });
     const float top = B::reduce(most, s.h.waves, Max());
     if (top == -INFINITY) {
         if (tid == 0) put_token(a, row, -1, -INFINITY);
@@ -890,8 +914,14 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
     if (g.by_k || (!g.by_p && g.m > 0.0)) {
         float least = -INFINITY;
         if (g.by_k) {
-            const float lo = B::reduce(most > -INFINITY ? most : top, s.h.waves, Min());
-            least = kth_bound<NT>([&](auto f) { f(most); }, (u64)g.k, lo, top, s.h);
+            // (groups: a thread's logits of a tile)
+            float lo = top;
+            r.each([&](int, const float (&x)[kEach]) {
+                const float v = largest(x);
+                lo = v > -INFINITY ? fminf(lo, v) : lo;
+            });
+            lo = B::reduce(lo, s.h.waves, Min());
+            least = kth_bound<NT>([&](auto f) { r.each([&](int, const float (&x)[kEach]) { f(largest(x)); }); }, (u64)g.k, lo, top, s.h);
         }
         if (g.m > 0.0 && !g.by_p) least = fmaxf(least, g.least(top));
         __syncthreads();
@@ -942,6 +972,13 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
         __syncthreads();
     }
     u64 mass[HELD ? kHeld : 1];
+    // (the bin's logits are those from lo on and below hi)
+    float lo = 0.0f, hi = 0.0f;
+    if (g.by_p) {
+        lo = of_key(first_key([&](float x) { return log_bin(w.log2_of(x)) <= bin; }));
+        hi = of_key(first_key([&](float x) { return log_bin(w.log2_of(x)) < bin; }));
+        if (!(hi == hi)) hi = INFINITY;                // (none is above: the first bin, in which a +inf is)
+    }
     r.each([&](int tile, const float (&x)[kEach]) {
         u64 sum = 0;
         if (!g.by_p) {
@@ -950,10 +987,12 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
             unsigned in = 0;
 #pragma unroll
             for (int e = 0; e < kEach; e++) {
-                const double y = w.log2_of(x[e]);
-                const int b = log_bin(y);
-                if (b < bin && g.passes(y)) sum += w.of_log2(y);
-                in |= b == bin ? 1u << e : 0;
+                const bool above_bin = bin > 0 && x[e] >= hi;
+                in |= x[e] >= lo && !above_bin ? 1u << e : 0;
+                if (above_bin) {
+                    const double y = w.log2_of(x[e]);
+                    if (g.passes(y)) sum += w.of_log2(y);
+                }
             }
             add_candidates(h.bins, &h.tile_ties[0], kBins, in, x, [&](int e) { return r.index(tile) + e; });
         }
@@ -1077,22 +1116,6 @@ template <class M> __device__ __forceinline__ int pick_span(const SampleArgs& a,
     __syncthreads();
     target = found[1];
     return (int)found[0];
-}
-
-// The smallest key whose value holds(value) is true of, which it is of all larger ones: sixty-four
-// keys at a time.  (That of a NaN above all values: there is none.)
-template <class F> __device__ __forceinline__ uint32_t first_key(F holds) {
-    const uint32_t lane = threadIdx.x & 63, top = 0xFF800000u, bottom = 0x007FFFFFu;      // +inf, -inf
-    uint32_t not_yet = 0;
-#pragma unroll
-    for (int shift = 26; shift >= -4; shift -= 6) {
-        const int s = shift < 0 ? 0 : shift;
-        const uint32_t key = not_yet + (lane << s);
-        const bool yes = (shift < 0 && lane > 3) || key > top || (key > bottom && holds(of_key(key)));
-        const unsigned long long no = ~__ballot(yes);              // (lane 0's among them)
-        not_yet += (uint32_t)(63 - __builtin_clzll(no | 1)) << s;
-    }
-    return not_yet + 1;
 }
 
 struct PickShared {
