@@ -89,7 +89,7 @@ def test_plan_of_many_tokens(rec):
     """Positions and slots of many rows are a launch of their own, within the runtime's work-items."""
     for rows in (4097, (1 << 31) - 1):
         launches, err = plan(rec, pos=(rows,))
-        assert not err and [l.kernel for l in launches] == ["k_plan<false>", "k_plan_tokens"]
+        assert not err and [l.kernel for l in launches] == ["k_plan<512, false, true>", "k_plan_tokens<true>"]
         assert launches[1].grid[0] * launches[1].block >= rows
 
 
