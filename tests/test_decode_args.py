@@ -220,6 +220,51 @@ def test_sample_takes(rec, kw):
     assert not err and launches
 
 
+def _kernels(r):
+    launches, err = r
+    assert not err
+    return [l.kernel for l in launches]
+
+
+@pytest.mark.parametrize("v,kernels", [
+    (1, ["k_sample_row<2, 256, true>"]), (8184, ["k_sample_row<2, 256, true>"]), (8185, ["k_sample_row<2, 1024, true>"]),
+    (32760, ["k_sample_row<2, 1024, true>"]), (32761, ["k_sample_spans<2>", "k_sample_pick<2>"]),
+    (2097144, ["k_sample_spans<2>", "k_sample_pick<2>"]), (2097145, ["k_sample_row<2, 1024, false>"])], ids=str)
+def test_sample_kernels(rec, v, kernels):
+    """Rows in a block's registers, spread over blocks, or a block's that reads them again."""
+    assert _kernels(sample(rec, x=(6, v))) == kernels
+
+
+def test_sample_without_memory(rec):
+    """Without a workspace captured calls, and calls that get no memory, keep a row in a block."""
+    whole = ["k_sample_row<3, 1024, false>"]
+    x = dict(x=(6, 131072), dt=O.BF16)
+    rec.no_memory(True)
+    try:
+        assert _kernels(sample(rec, **x)) == whole
+    finally:
+        rec.no_memory(False)
+    rec.lib.sample_workspace_bytes.restype = ctypes.c_size_t
+    need = rec.lib.sample_workspace_bytes(6, 131072)
+    rec.capturing(True)
+    try:
+        assert _kernels(sample(rec, **x)) == whole
+        assert _kernels(sample(rec, ws=(need - 1,), **x)) == whole
+        assert _kernels(sample(rec, ws=(need,), **x)) == ["k_sample_spans<3>", "k_sample_pick<3>"]
+    finally:
+        rec.capturing(False)
+
+
+def test_sample_of_many_rows(rec):
+    n = (1 << 22) - 1
+    rows = lambda m: {k: (m,) for k in ("u", "t", "k", "p", "m", "token", "lp")}      # noqa: E731
+    assert _kernels(sample(rec, x=(n, 9), **rows(n))) == ["k_sample_row<2, 256, true>"]
+    launches, err = sample(rec, x=(n + 1, 9), **rows(n + 1))
+    assert "rows" in err and not launches
+    # (a launch of its spans would be past the runtime's work-items)
+    assert _kernels(sample(rec, x=(1 << 20, 100000), **rows(1 << 20))) == ["k_sample_row<2, 1024, false>"]
+
+
 def test_sample_of_nothing(rec):
     assert sample(rec, **{n: (0,) for n in ("u", "t", "k", "p", "m", "token", "lp")}, x=(0, 100)) == ([], "")
 

@@ -148,8 +148,13 @@ def test_uniform_numbers_outside(hip, u_type):
 
 def test_settings_out_of_range(hip):
     """k below 1: all; p of 0 or less: the largest alone; p of 1 and more, NaN: all; m above 1: the largest."""
-    x, u = logits(6, 3000, seed=9)
-    SampleProblem(x, u, k=[0, -5, 3000, 3001, 1 << 30, 2]).check(hip)
+    for v in (3000, 12000, 40000):
+        _out_of_range(hip, *logits(6, v, seed=9))
+
+
+def _out_of_range(hip, x, u):
+    v = x.shape[1]
+    SampleProblem(x, u, k=[0, -5, v, v + 1, 1 << 30, 2]).check(hip)
     tokens, _ = SampleProblem(x, u, p=[0.0, -1.0, -math.inf, 1.0, 3.0, math.nan]).check(hip)
     assert (tokens[:3] == x[:3].argmax(1)).all()
     tokens, _ = SampleProblem(x, u, m=[1.0, 2.0, math.inf, 0.0, -1.0, math.nan]).check(hip)
@@ -229,6 +234,43 @@ def test_workspaces(hip, rows, v):
     for size in (need, need - 1, need + 1000):
         b = p.run(hip, workspace=size)
         assert (a[0] == b[0]).all() and (a[1] == b[1]).all(), size
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_captured_without_a_workspace(hip, dtype):
+    """A block per row that reads it again: the tokens of the eager call, replay after replay."""
+    import ctypes
+    import torch
+    from oracle import oracle as O
+    from onnx_translator_amd.nn.Operators import CSampleParams
+    x, u = logits(7, 45001, seed=15)
+    x[5] = np.round(x[5])                            # many equal ones
+    x[6, 100:] = -np.inf
+    p = SampleProblem(x, u, dtype, t=[1.0, 0.0, 0.8, 1.2, 1.0, 1.0, 1.0], k=[0, 0, 50, 3000, 0, 0, 0], p=[1.0, 1.0, 0.9, 0.9, 0.7, 0.7117, 0.9],
+                      m=[0.0, 0.0, 0.0, 0.0, 0.05, 0.0, 0.0])
+    want = p.check(hip)[0]
+    t = [p.x.cuda(), *(torch.from_numpy(v).cuda() for v in (p.u, p.t, p.k, p.p, p.m)), torch.zeros(7, dtype=torch.int32, device="cuda")]
+    code = {torch.float16: O.F16, torch.bfloat16: O.BF16, torch.float32: O.F32, torch.int64: O.I64, torch.int32: O.I32}
+    side = torch.cuda.Stream()
+    with Dev(hip) as dev:
+        w = [hip.lib.tensor_wrap_device(ctypes.c_void_p(v.data_ptr()), (ctypes.c_int * v.dim())(*v.shape), v.dim(), code[v.dtype]) for v in t]
+        dev.held += w
+        prm = CSampleParams(0)
+        hip.lib.tensor_ops_hip_set_stream(ctypes.c_void_p(side.cuda_stream))
+        try:
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                dev.call("sample_forward", *w, O.PT(), ctypes.byref(prm), O.PT())
+            for _ in range(4):
+                t[-1].fill_(-9)
+                torch.cuda.synchronize()
+                g.replay()
+                torch.cuda.synchronize()
+                assert (t[-1].cpu().numpy() == want).all()
+        finally:
+            torch.cuda.synchronize()
+            hip.lib.tensor_ops_hip_set_stream(None)
 
 
 def test_the_distribution(hip):
