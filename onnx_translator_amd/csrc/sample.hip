@@ -289,9 +289,9 @@ template <int NT, int N, class AT> __device__ __forceinline__ int reach(AT at, u
 
 // ---- few candidates --------------------------------------------------------------------------
 // Where the kept tokens are known to be among at most kMost candidates these go on without the row.
-// Up to kFew are ranked by counting the larger ones, which takes no barrier between its reads; of
-// more the border is found in bins of the value, and only its bin's are ranked (600 candidates: two
-// sorts took 25 us).
+// Up to kFew are ranked by counting the larger ones, which takes no barrier between its reads (100
+// candidates: 5 us; with one read after the other 14); of more the border is found in bins of the
+// value, and only its bin's are ranked (500 candidates: 6 us; two sorts took 25).
 constexpr int kMost = 2048, kFew = 128;
 
 template <int NT> struct Candidates {
@@ -874,7 +874,9 @@ template <class F> __device__ __forceinline__ uint32_t first_key(F holds) {
 // Bins of a weight's logarithm from the largest down.
 __device__ __forceinline__ int log_bin(double y) { return min((int)(y * -51.0), kBins - 1); }      // (51 to a factor of two: 40 of them)
 
-// A block per row.  HELD: the row is read once, into registers.
+// A block per row.  HELD: the row is read once, into registers.  Bound by one CU's double products and
+// LDS atomics where top-p weighs the whole row (32000 logits: 42 us, of them 9 for the histogram,
+// 6 .. 10 for the second pass), else by its chain of barriers (top-k of 50: 12 us, greedy 6).
 template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sample_row(SampleArgs a) {
     __shared__ SampleShared<NT> s;
     typedef Block<NT> B;
@@ -910,119 +912,110 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
     const Weights w = {finite(top), g.per, a.shift};
 
     do {
-    // ---- top-k, or min-p alone: few candidates, where few are above what none kept is below
-    if (g.by_k || (!g.by_p && g.m > 0.0)) {
-        float least = -INFINITY;
-        if (g.by_k) {
-            // (groups: a thread's logits of a tile)
-            float lo = top;
-            r.each([&](int, const float (&x)[kEach]) {
-                const float v = largest(x);
-                lo = v > -INFINITY ? fminf(lo, v) : lo;
+        // ---- top-k, or min-p alone: few candidates, where few are above what none kept is below
+        if (g.by_k || (!g.by_p && g.m > 0.0)) {
+            float least = -INFINITY;
+            if (g.by_k) {
+                // (groups: a thread's logits of a tile)
+                float lo = top;
+                r.each([&](int, const float (&x)[kEach]) {
+                    const float v = largest(x);
+                    lo = v > -INFINITY ? fminf(lo, v) : lo;
+                });
+                lo = B::reduce(lo, s.h.waves, Min());
+                least = kth_bound<NT>([&](auto f) { r.each([&](int, const float (&x)[kEach]) { f(largest(x)); }); }, (u64)g.k, lo, top, s.h);
+            }
+            if (g.m > 0.0 && !g.by_p) least = fmaxf(least, g.least(top));
+            __syncthreads();
+            if (tid == 0) s.c.count = 0;
+            __syncthreads();
+            r.each([&](int tile, const float (&x)[kEach]) {
+                unsigned in = 0;
+#pragma unroll
+                for (int e = 0; e < kEach; e++) in |= x[e] >= least && x[e] > -INFINITY ? 1u << e : 0;
+                add_candidates(s.c.rank, &s.c.count, kMost, in, x, [&](int e) { return r.index(tile) + e; });
             });
-            lo = B::reduce(lo, s.h.waves, Min());
-            least = kth_bound<NT>([&](auto f) { r.each([&](int, const float (&x)[kEach]) { f(largest(x)); }); }, (u64)g.k, lo, top, s.h);
-        }
-        if (g.m > 0.0 && !g.by_p) least = fmaxf(least, g.least(top));
-        __syncthreads();
-        if (tid == 0) s.c.count = 0;
-        __syncthreads();
-        r.each([&](int tile, const float (&x)[kEach]) {
-            unsigned in = 0;
-#pragma unroll
-            for (int e = 0; e < kEach; e++) in |= x[e] >= least && x[e] > -INFINITY ? 1u << e : 0;
-            add_candidates(s.c.rank, &s.c.count, kMost, in, x, [&](int e) { return r.index(tile) + e; });
-        });
-        __syncthreads();
-        if (s.c.count <= kMost) {
-            draw_candidates<NT>(a, row, g, w, least, top, s.c);
-            return;
-        }
-        break;
-    }
-    // ---- no filter, or top-p: the weights by their logarithm, then those above the border's bin by
-    // tile, and the bin's own one by one
-    Histograms<NT>& h = s.h;
-    u64 border = 0;
-    int bin = kBins;
-    u64 above = 0, want = 0;
-    if (g.by_p) {
-        __syncthreads();
-        for (int i = tid; i < kBins; i += NT) h.bins[i] = 0;
-        __syncthreads();
-        r.each([&](int, const float (&x)[kEach]) {
-#pragma unroll
-            for (int e = 0; e < kEach; e++) {
-                const double y = w.log2_of(x[e]);
-                const u64 v = w.of_log2(y);
-                if (v) atomicAdd(&h.bins[log_bin(y)], v);
+            __syncthreads();
+            if (s.c.count <= kMost) {
+                draw_candidates<NT>(a, row, g, w, least, top, s.c);
+                return;
             }
-        });
-        __syncthreads();
-        u64 sum = 0, total;
-        for (int i = tid; i < kBins; i += NT) sum += h.bins[i];
-        sum = B::reduce(sum, h.waves, Add());
-        want = g.want(sum);
-        bin = reach<NT, kBins / NT>([&](int i) { return h.bins[i]; }, want, h.waves, h.found, above, total);
-        if (bin == kBins - 1) {                        // (among weights below 2^-40)
             break;
         }
-        __syncthreads();
-        if (tid == 0) h.tile_ties[0] = 0;              // the bin's count; its ranks go where the bins were
-        __syncthreads();
-    }
-    u64 mass[HELD ? kHeld : 1];
-    // (the bin's logits are those from lo on and below hi)
-    float lo = 0.0f, hi = 0.0f;
-    if (g.by_p) {
-        lo = of_key(first_key([&](float x) { return log_bin(w.log2_of(x)) <= bin; }));
-        hi = of_key(first_key([&](float x) { return log_bin(w.log2_of(x)) < bin; }));
-        if (!(hi == hi)) hi = INFINITY;                // (none is above: the first bin, in which a +inf is)
-    }
-    r.each([&](int tile, const float (&x)[kEach]) {
-        u64 sum = 0;
-        if (!g.by_p) {
-            sum = w.sum(x);
-        } else {
-            unsigned in = 0;
+        // ---- no filter, or top-p: the weights by their logarithm, then those above the border's bin by
+        // tile, and the bin's own one by one
+        Histograms<NT>& h = s.h;
+        u64 border = 0;
+        int bin = kBins;
+        u64 above = 0, want = 0;
+        if (g.by_p) {
+            __syncthreads();
+            for (int i = tid; i < kBins; i += NT) h.bins[i] = 0;
+            __syncthreads();
+            r.each([&](int, const float (&x)[kEach]) {
 #pragma unroll
-            for (int e = 0; e < kEach; e++) {
-                const bool above_bin = bin > 0 && x[e] >= hi;
-                in |= x[e] >= lo && !above_bin ? 1u << e : 0;
-                if (above_bin) {
+                for (int e = 0; e < kEach; e++) {
                     const double y = w.log2_of(x[e]);
-                    if (g.passes(y)) sum += w.of_log2(y);
+                    const u64 v = w.of_log2(y);
+                    if (v) atomicAdd(&h.bins[log_bin(y)], v);
                 }
-            }
-            add_candidates(h.bins, &h.tile_ties[0], kBins, in, x, [&](int e) { return r.index(tile) + e; });
-        }
-        if constexpr (HELD) {
-            mass[tile] = sum;
-        } else {
+            });
+            __syncthreads();
+            u64 sum = 0, total;
+            for (int i = tid; i < kBins; i += NT) sum += h.bins[i];
             sum = B::reduce(sum, h.waves, Add());
-            if (tid == 0) h.tile_mass[tile] = sum;
+            want = g.want(sum);
+            bin = reach<NT, kBins / NT>([&](int i) { return h.bins[i]; }, want, h.waves, h.found, above, total);
+            if (bin == kBins - 1) break;                   // (among weights below 2^-40)
+            __syncthreads();
+            if (tid == 0) h.tile_ties[0] = 0;              // the bin's count; its ranks go where the bins were
+            __syncthreads();
         }
-    });
-    if constexpr (HELD) {
+        const int lane = tid & 63;
+        for (int i = tid; i < r.tiles; i += NT) h.tile_mass[i] = 0;
+        __syncthreads();
+        // (the bin's logits are those from lo on and below hi)
+        float lo = 0.0f, hi = 0.0f;
+        if (g.by_p) {
+            lo = of_key(first_key([&](float x) { return log_bin(w.log2_of(x)) <= bin; }));
+            hi = of_key(first_key([&](float x) { return log_bin(w.log2_of(x)) < bin; }));
+            if (!(hi == hi)) hi = INFINITY;                // (none is above: the first bin, in which a +inf is)
+        }
+        r.each([&](int tile, const float (&x)[kEach]) {
+            u64 sum = 0;
+            if (!g.by_p) {
+                sum = w.sum(x);
+            } else {
+                unsigned in = 0, over = 0;
 #pragma unroll
-        for (int tile = 0; tile < kHeld; tile++) {
-            if (tile >= r.tiles) break;
-            const u64 sum = B::reduce(mass[tile], h.waves, Add());
-            if (tid == 0) h.tile_mass[tile] = sum;
-        }
-    }
-    __syncthreads();
-    if (g.by_p) {
-        const int count = (int)h.tile_ties[0];
-        if (count > kBins) {                           // (many equal ones)
-            break;
-        }
-        border = border_in<NT>(h.bins, count, above, want, g, w, h.waves, h.found, h.tile_ties, a.V, [&](u64 rank, u64 v) {
-            if (v) atomicAdd(&h.tile_mass[(index_of(rank) + r.first) / r.kTile], v);
+                for (int e = 0; e < kEach; e++) {
+                    const bool above_bin = bin > 0 && x[e] >= hi;
+                    over |= above_bin ? 1u << e : 0;
+                    in |= x[e] >= lo && !above_bin ? 1u << e : 0;
+                }
+                if (__ballot(over != 0)) {                 // (all of a wave's or none: eight branches take twice as long)
+#pragma unroll
+                    for (int e = 0; e < kEach; e++) {
+                        const double y = w.log2_of(x[e]);
+                        const u64 v = w.of_log2(y);
+                        sum += (over >> e & 1) && g.passes(y) ? v : 0;
+                    }
+                }
+                add_candidates(h.bins, &h.tile_ties[0], kBins, in, x, [&](int e) { return r.index(tile) + e; });
+            }
+            sum = wave_allreduce(sum, Add());
+            if (lane == 0 && sum) atomicAdd(&h.tile_mass[tile], sum);
         });
-    }
-    draw_tile<DT, NT>(a, row, r, g, w, border, -FLT_MAX, h);
-    return;
+        __syncthreads();
+        if (g.by_p) {
+            const int count = (int)h.tile_ties[0];
+            if (count > kBins) break;                  // (many equal ones)
+            border = border_in<NT>(h.bins, count, above, want, g, w, h.waves, h.found, h.tile_ties, a.V, [&](u64 rank, u64 v) {
+                if (v) atomicAdd(&h.tile_mass[(index_of(rank) + r.first) / r.kTile], v);
+            });
+        }
+        draw_tile<DT, NT>(a, row, r, g, w, border, -FLT_MAX, h);
+        return;
     } while (false);
     // ---- too many candidates
     __syncthreads();
@@ -1036,7 +1029,12 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
 // by the weights' logarithm; of every 16 the largest value.  A block per row goes on from those:
 // with top-k the few logits that can be kept, else the span that the draw falls into, and for a
 // border the logits whose logarithm is the border's.
-constexpr int kSpanThreads = 256, kSpan = 16 * kSpanThreads, kPickThreads = 512;
+// (64 x 131072 bfloat16 by top-p: 16 us for the spans and 68 for the rows, a block per row 250;
+// 256 x 131072 float32 by temperature: 37 us, 3.6 TB/s with 34 M weights in double on the way, and 7.5,
+// a block per row 113.  A row with a border: 25 us to find the logits in its bins, four operations
+// for each of 131072 on one CU, 10 for the finer bins, 5 for the border.)
+constexpr int kSpanThreads = 256, kSpan = 16 * kSpanThreads;
+constexpr int kPickThreads = 512;                      // (1024 have half the registers: spills cost every row 6 us)
 constexpr int kSpans = 512;                            // of a row at most
 constexpr int kLogBins = 128;                          // four to a factor of two, from a span's largest down
 constexpr int kNear = 12288;                           // logits of the border's bins
@@ -1202,170 +1200,164 @@ template <int DT> __global__ __launch_bounds__(kPickThreads) void k_sample_pick(
         return;
     }
     do {
-    const SampleRow<DT, NT, false> whole(a, row);
-    if (g.by_k) {
-        // ---- the few logits that can be among the k largest
-        const float* group = w.group + row * w.spans * kSpanThreads;
-        const int groups = w.spans * kSpanThreads;
-        float lo = top;
-        for (int i = tid; i < groups; i += NT) lo = group[i] > -INFINITY ? fminf(lo, group[i]) : lo;
-        lo = B::reduce(lo, s.waves, Min());
-        float least = kth_bound<NT>([&](auto f) {
-            for (int i = tid; i < groups; i += NT) f(group[i]);
-        }, (u64)g.k, lo, top, s.s.h);
-        if (g.m > 0.0 && !g.by_p) least = fmaxf(least, g.least(top));
-        __syncthreads();
-        if (tid == 0) s.s.c.count = 0;
-        __syncthreads();
-        for (int i0 = 0; i0 < groups && s.s.c.count <= kMost; i0 += NT) {
-            const int i = i0 + tid;
-            const bool near = i < groups && group[i] >= least && group[i] > -INFINITY;
-            if (!__ballot(near)) continue;
-            float x[16];
-            unsigned in = 0;
-            const int span = i / kSpanThreads, of = i % kSpanThreads;
-            if (near) {
-                uint4 q[16 / VEC];
-                r.chunks(span_index<DT>(r, span, of, 0), span_index<DT>(r, span, of, 16 / VEC - 1) + VEC, [&](int c) { return span_index<DT>(r, span, of, c); }, q);
+        const SampleRow<DT, NT, false> whole(a, row);
+        if (g.by_k) {
+            // ---- the few logits that can be among the k largest
+            const float* group = w.group + row * w.spans * kSpanThreads;
+            const int groups = w.spans * kSpanThreads;
+            float lo = top;
+            for (int i = tid; i < groups; i += NT) lo = group[i] > -INFINITY ? fminf(lo, group[i]) : lo;
+            lo = B::reduce(lo, s.waves, Min());
+            float least = kth_bound<NT>([&](auto f) {
+                for (int i = tid; i < groups; i += NT) f(group[i]);
+            }, (u64)g.k, lo, top, s.s.h);
+            if (g.m > 0.0 && !g.by_p) least = fmaxf(least, g.least(top));
+            __syncthreads();
+            if (tid == 0) s.s.c.count = 0;
+            __syncthreads();
+            for (int i0 = 0; i0 < groups && s.s.c.count <= kMost; i0 += NT) {
+                const int i = i0 + tid;
+                const bool near = i < groups && group[i] >= least && group[i] > -INFINITY;
+                if (!__ballot(near)) continue;
+                float x[16];
+                unsigned in = 0;
+                const int span = i / kSpanThreads, of = i % kSpanThreads;
+                if (near) {
+                    uint4 q[16 / VEC];
+                    r.chunks(span_index<DT>(r, span, of, 0), span_index<DT>(r, span, of, 16 / VEC - 1) + VEC, [&](int c) { return span_index<DT>(r, span, of, c); }, q);
 #pragma unroll
-                for (int c = 0; c < 16 / VEC; c++) RowChunks<DT>::open(q[c], x + c * VEC);
+                    for (int c = 0; c < 16 / VEC; c++) RowChunks<DT>::open(q[c], x + c * VEC);
 #pragma unroll
-                for (int e = 0; e < 16; e++) in |= x[e] >= least && x[e] > -INFINITY ? 1u << e : 0;
+                    for (int e = 0; e < 16; e++) in |= x[e] >= least && x[e] > -INFINITY ? 1u << e : 0;
+                }
+                add_candidates(s.s.c.rank, &s.s.c.count, kMost, in, x, [&](int e) { return span_index<DT>(r, span, of, e / VEC) + e % VEC; });
             }
-            add_candidates(s.s.c.rank, &s.s.c.count, kMost, in, x, [&](int e) { return span_index<DT>(r, span, of, e / VEC) + e % VEC; });
-        }
-        __syncthreads();
-        if (s.s.c.count <= kMost) {
-            draw_candidates<NT>(a, row, g, wt, least, top, s.s.c);
-            return;
-        }
-        break;
-    }
-
-    // ---- top-p, min-p: the row's weights by their logarithm
-    const double from = grid_of(top, g.per);
-    __syncthreads();
-    if (tid < kLogBins) s.row_bins[tid] = 0;
-    if (tid == 0) s.count = s.count2 = 0;
-    __syncthreads();
-    auto each_bin = [&](auto f) {                      // f(span, bin of the row, weight): a wave per span
-        for (int i = tid >> 6; i < w.spans; i += B::kWaves) {
-            const double y = wt.log2_of(largest[i]), below = grid_of(largest[i], g.per) - from;
-            const double factor = factor_of(y);
-            if (!(factor > 0.0 && below < kLogBins)) continue;
-            const u64* b = w.bins + (row * w.spans + i) * kLogBins;
-            f(i, (int)below + lane, against_top(b[lane], factor), (int)below + 64 + lane, against_top(b[lane + 64], factor));
-        }
-    };
-    u64 weights = 0;
-    each_bin([&](int, int i, u64 p, int j, u64 q) {
-        // (the last bin of a span holds all that is below: no less than the row's last)
-        if (p) atomicAdd(&s.row_bins[min(i, kLogBins - 1)], p);
-        if (q) atomicAdd(&s.row_bins[min(j, kLogBins - 1)], q);
-        weights += p + q;
-    });
-    weights = B::reduce(weights, s.waves, Add());
-    const u64 want = g.by_p ? g.want(weights) : ~0ull;
-    u64 above = 0, total;
-    int first = kLogBins, last = -1;                   // bins that a border may lie in
-    if (g.by_p) {
-        first = reach<NT, 1>([&](int i) { return i < kLogBins ? s.row_bins[i] : 0; }, want, s.waves, s.found, above, total);
-        if (first < 0) first = kLogBins - 1;
-        last = first;
-    }
-    if (g.m > 0.0) {
-        const double b = __builtin_fmin(-__builtin_floor(wt.top * (g.per * 4.0) + 4.0 * log2(g.m)) - from, kLogBins);
-        if ((int)b - 1 <= last || !g.by_p) first = min(first, max((int)b - 1, 0));
-        if (!g.by_p || (int)b - 1 <= last) last = max((int)b + 1, first);      // (min-p's, unless top-p's is well above)
-        if (g.by_p && (int)b - 1 > first) last = first;
-        // weights above the first bin
-        u64 sum = tid < kLogBins && tid < first ? s.row_bins[tid] : 0;
-        above = B::reduce(sum, s.waves, Add());
-    }
-    if (last >= kLogBins - 1) {                        // (among weights below 2^-31 of the largest)
-        break;
-    }
-    // the spans' weights above those bins
-    for (int i = tid; i < w.spans; i += NT) s.kept[i] = 0;
-    __syncthreads();
-    each_bin([&](int span, int i, u64 p, int j, u64 q) {
-        const u64 sum = wave_allreduce((i < first ? p : 0) + (j < first ? q : 0), Add());
-        if (lane == 0) s.kept[span] = sum;
-    });
-    // and their logits in them, by the values that bound these bins; a wave finds the places of a
-    // tile's all at once
-    const float lo = of_key(first_key([&](float x) { return grid_of(x, g.per) - from <= last; }));
-    const float hi = of_key(first_key([&](float x) { return grid_of(x, g.per) - from < first; }));
-    const bool open_end = !(hi == hi);                 // (none is above)
-    whole.each([&](int tile, const float (&x)[kEach]) {
-        unsigned in = 0;
-#pragma unroll
-        for (int e = 0; e < kEach; e++) in |= x[e] >= lo && (open_end || x[e] < hi) ? 1u << e : 0;
-        add_candidates(s.near, &s.count, kNear, in, x, [&](int e) { return whole.index(tile) + e; });
-    });
-    __syncthreads();
-    if (s.count > kNear) {
-        break;
-    }
-    const int near = (int)s.count;
-    u64 border = 0;
-    auto span_of = [&](u64 rank) { return (index_of(rank) + r.first) / kSpan; };
-    // Adds a wave's weights to their spans, mostly one or two (lanes adding to one place wait for each other).
-    auto keep = [&](u64 rank, u64 v) {
-        const int span = v ? span_of(rank) : -1;
-        for (unsigned long long todo = __ballot(v != 0); todo;) {
-            const int of = __builtin_amdgcn_readlane(span, __builtin_ctzll(todo));
-            const u64 sum = wave_allreduce(span == of ? v : 0, Add());
-            if (lane == 0) atomicAdd(&s.kept[of], sum);
-            todo &= ~__ballot(span == of);
-        }
-    };
-    const int near_all = (near + NT - 1) / NT * NT;    // (whole waves)
-    if (g.by_p) {
-        // the same once more in finer bins, by the logarithm's place between the first and the last
-        const double y0 = -(from + first - 1) - wt.top * (g.per * 4.0), per_bin = kBins / (double)(last - first + 1);      // (4 log2 at the upper end)
-        auto fine_bin = [&](double y) {
-            const double b = (y0 - 4.0 * y) * per_bin;
-            return b <= 0.0 ? 0 : b >= kBins - 1 ? kBins - 1 : (int)b;
-        };
-        for (int i = tid; i < kBins; i += NT) s.fine[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < near; i += NT) {
-            const double y = wt.log2_of(value_of(s.near[i]));
-            atomicAdd(&s.fine[fine_bin(y)], wt.of_log2(y));
-        }
-        __syncthreads();
-        u64 over;
-        int bin = reach<NT, kBins / NT>([&](int i) { return s.fine[i]; }, want - above, s.waves, s.found, over, total);
-        if (bin < 0) bin = kBins;                      // (the sums were rounded: all of them)
-        __syncthreads();
-        for (int i = tid; i < near_all; i += NT) {
-            const u64 rank = i < near ? s.near[i] : 0;
-            const double y = rank ? wt.log2_of(value_of(rank)) : -100.0;
-            const int b = rank ? fine_bin(y) : kBins + 1;
-            keep(rank, b < bin && g.passes(y) ? wt.of_log2(y) : 0);
-            const float x[1] = {value_of(rank)};
-            add_candidates(s.fine, &s.count2, kBins, b == bin ? 1u : 0, x, [&](int) { return index_of(rank); });      // (in the bins' place)
-        }
-        __syncthreads();
-        if (s.count2 > kBins) {                        // (many equal ones)
+            __syncthreads();
+            if (s.s.c.count <= kMost) {
+                draw_candidates<NT>(a, row, g, wt, least, top, s.s.c);
+                return;
+            }
             break;
         }
-        if (s.count2) border = border_in<NT>(s.fine, (int)s.count2, above + over, want, g, wt, s.waves, s.found, (unsigned*)s.near, a.V, keep);
-    } else {
-        for (int i = tid; i < near_all; i += NT) {
-            const u64 rank = i < near ? s.near[i] : 0;
-            const double y = rank ? wt.log2_of(value_of(rank)) : -100.0;
-            keep(rank, rank && g.passes(y) ? wt.of_log2(y) : 0);
+
+        // ---- top-p, min-p: the row's weights by their logarithm
+        const double from = grid_of(top, g.per);
+        __syncthreads();
+        if (tid < kLogBins) s.row_bins[tid] = 0;
+        if (tid == 0) s.count = s.count2 = 0;
+        __syncthreads();
+        auto each_bin = [&](auto f) {                      // f(span, bin of the row, weight): a wave per span
+            for (int i = tid >> 6; i < w.spans; i += B::kWaves) {
+                const double y = wt.log2_of(largest[i]), below = grid_of(largest[i], g.per) - from;
+                const double factor = factor_of(y);
+                if (!(factor > 0.0 && below < kLogBins)) continue;
+                const u64* b = w.bins + (row * w.spans + i) * kLogBins;
+                f(i, (int)below + lane, against_top(b[lane], factor), (int)below + 64 + lane, against_top(b[lane + 64], factor));
+            }
+        };
+        u64 weights = 0;
+        each_bin([&](int, int i, u64 p, int j, u64 q) {
+            // (the last bin of a span holds all that is below: no less than the row's last)
+            if (p) atomicAdd(&s.row_bins[min(i, kLogBins - 1)], p);
+            if (q) atomicAdd(&s.row_bins[min(j, kLogBins - 1)], q);
+            weights += p + q;
+        });
+        weights = B::reduce(weights, s.waves, Add());
+        const u64 want = g.by_p ? g.want(weights) : ~0ull;
+        u64 above = 0, total;
+        int first = kLogBins, last = -1;                   // bins that a border may lie in
+        if (g.by_p) {
+            first = reach<NT, 1>([&](int i) { return i < kLogBins ? s.row_bins[i] : 0; }, want, s.waves, s.found, above, total);
+            if (first < 0) first = kLogBins - 1;
+            last = first;
         }
-    }
-    __syncthreads();
-    u64 target, all;
-    const int span = pick_span(a, row, w.spans, s.waves, s.found, [&](int i) { return s.kept[i]; }, target, all);
-    draw_span(span, target, all, [&](float x, int i, double y) {
-        return x >= lo && rank_of(x, i) >= border && g.passes(y);
-    });
-    return;
+        if (g.m > 0.0) {
+            const double b = __builtin_fmin(-__builtin_floor(wt.top * (g.per * 4.0) + 4.0 * log2(g.m)) - from, kLogBins);
+            if ((int)b - 1 <= last || !g.by_p) first = min(first, max((int)b - 1, 0));
+            if (!g.by_p || (int)b - 1 <= last) last = max((int)b + 1, first);      // (min-p's, unless top-p's is well above)
+            if (g.by_p && (int)b - 1 > first) last = first;
+            // weights above the first bin
+            u64 sum = tid < kLogBins && tid < first ? s.row_bins[tid] : 0;
+            above = B::reduce(sum, s.waves, Add());
+        }
+        if (last >= kLogBins - 1) break;           // (among weights below 2^-31 of the largest)
+        // the spans' weights above those bins
+        for (int i = tid; i < w.spans; i += NT) s.kept[i] = 0;
+        __syncthreads();
+        each_bin([&](int span, int i, u64 p, int j, u64 q) {
+            const u64 sum = wave_allreduce((i < first ? p : 0) + (j < first ? q : 0), Add());
+            if (lane == 0) s.kept[span] = sum;
+        });
+        // and their logits in them, by the values that bound these bins; a wave finds the places of a
+        // tile's all at once
+        const float lo = of_key(first_key([&](float x) { return grid_of(x, g.per) - from <= last; }));
+        const float hi = of_key(first_key([&](float x) { return grid_of(x, g.per) - from < first; }));
+        const bool open_end = !(hi == hi);                 // (none is above)
+        whole.each([&](int tile, const float (&x)[kEach]) {
+            unsigned in = 0;
+#pragma unroll
+            for (int e = 0; e < kEach; e++) in |= x[e] >= lo && (open_end || x[e] < hi) ? 1u << e : 0;
+            add_candidates(s.near, &s.count, kNear, in, x, [&](int e) { return whole.index(tile) + e; });
+        });
+        __syncthreads();
+        if (s.count > kNear) break;
+        const int near = (int)s.count;
+        u64 border = 0;
+        auto span_of = [&](u64 rank) { return (index_of(rank) + r.first) / kSpan; };
+        // Adds a wave's weights to their spans, mostly one or two (lanes adding to one place wait for each other).
+        auto keep = [&](u64 rank, u64 v) {
+            const int span = v ? span_of(rank) : -1;
+            for (unsigned long long todo = __ballot(v != 0); todo;) {
+                const int of = __builtin_amdgcn_readlane(span, __builtin_ctzll(todo));
+                const u64 sum = wave_allreduce(span == of ? v : 0, Add());
+                if (lane == 0) atomicAdd(&s.kept[of], sum);
+                todo &= ~__ballot(span == of);
+            }
+        };
+        const int near_all = (near + NT - 1) / NT * NT;    // (whole waves)
+        if (g.by_p) {
+            // the same once more in finer bins, by the logarithm's place between the first and the last
+            const double y0 = -(from + first - 1) - wt.top * (g.per * 4.0), per_bin = kBins / (double)(last - first + 1);      // (4 log2 at the upper end)
+            auto fine_bin = [&](double y) {
+                const double b = (y0 - 4.0 * y) * per_bin;
+                return b <= 0.0 ? 0 : b >= kBins - 1 ? kBins - 1 : (int)b;
+            };
+            for (int i = tid; i < kBins; i += NT) s.fine[i] = 0;
+            __syncthreads();
+            for (int i = tid; i < near; i += NT) {
+                const double y = wt.log2_of(value_of(s.near[i]));
+                atomicAdd(&s.fine[fine_bin(y)], wt.of_log2(y));
+            }
+            __syncthreads();
+            u64 over;
+            int bin = reach<NT, kBins / NT>([&](int i) { return s.fine[i]; }, want - above, s.waves, s.found, over, total);
+            if (bin < 0) bin = kBins;                      // (the sums were rounded: all of them)
+            __syncthreads();
+            for (int i = tid; i < near_all; i += NT) {
+                const u64 rank = i < near ? s.near[i] : 0;
+                const double y = rank ? wt.log2_of(value_of(rank)) : -100.0;
+                const int b = rank ? fine_bin(y) : kBins + 1;
+                keep(rank, b < bin && g.passes(y) ? wt.of_log2(y) : 0);
+                const float x[1] = {value_of(rank)};
+                add_candidates(s.fine, &s.count2, kBins, b == bin ? 1u : 0, x, [&](int) { return index_of(rank); });      // (in the bins' place)
+            }
+            __syncthreads();
+            if (s.count2 > kBins) break;           // (many equal ones)
+            if (s.count2) border = border_in<NT>(s.fine, (int)s.count2, above + over, want, g, wt, s.waves, s.found, (unsigned*)s.near, a.V, keep);
+        } else {
+            for (int i = tid; i < near_all; i += NT) {
+                const u64 rank = i < near ? s.near[i] : 0;
+                const double y = rank ? wt.log2_of(value_of(rank)) : -100.0;
+                keep(rank, rank && g.passes(y) ? wt.of_log2(y) : 0);
+            }
+        }
+        __syncthreads();
+        u64 target, all;
+        const int span = pick_span(a, row, w.spans, s.waves, s.found, [&](int i) { return s.kept[i]; }, target, all);
+        draw_span(span, target, all, [&](float x, int i, double y) {
+            return x >= lo && rank_of(x, i) >= border && g.passes(y);
+        });
+        return;
     } while (false);
     // ---- too many candidates
     __syncthreads();
@@ -1390,6 +1382,9 @@ size_t spread_layout(Spread& w, void* base, int64_t rows, int64_t V) {
 
 constexpr int kShort = kHeld * kShortThreads * kEach - 8, kLong = kHeld * kRowThreads * kEach - 8;
 
+// Rows of up to kLong logits stay in a block's registers: one launch where two take 4 us more (32000
+// logits by top-k: 13.5 us, spread 19; but by temperature alone 16 and 10, by top-p 42 and 34, which
+// the host cannot know).  Short ones take a small block, whose barriers are cheaper.
 template <int DT> void launch_sample(const SampleArgs& a, const Spread* w, hipStream_t s) {
     const unsigned rows = (unsigned)a.rows;
     if (w) {
