@@ -447,10 +447,10 @@ typedef struct {
  * (Past + New, Past if refused, 0 if ended) are those of cache_attention_forward; Positions and
  * Slots [tokens] those of qk_norm_rotary_forward: the token's place in its request plus Offset
  * (one number, NULL: 0; a shared prefix, say) and page * page_size + place in the page, both -1
- * for a refused request's tokens and for rows behind the last request.  A position or slot that its type does not hold
- * is -1.  NextState receives the state after the step, with the requests refused in it.  KVLen may be Past
- * and NextState State (the same memory and type); nothing else may overlap.  int32 or int64
- * each, State and NextState int64. */
+ * for a refused request's tokens and for rows behind the last request.  A position or slot
+ * that its type does not hold is -1.  NextState receives the state after the step, with the
+ * requests refused in it.  KVLen may be Past and NextState State (the same memory and type);
+ * nothing else may overlap.  int32 or int64 each, State and NextState int64. */
 void cache_plan_forward(const Tensor* New, const Tensor* Past, const Tensor* Offset, const Tensor* State,
                         Tensor* Pages, Tensor* Free, Tensor* QStart, Tensor* KVLen, Tensor* Positions,
                         Tensor* Slots, Tensor* NextState, const CachePlanParams* params);

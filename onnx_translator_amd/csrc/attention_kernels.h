@@ -1025,6 +1025,7 @@ template <int DT, int D, int MR> TOHIP_INLINE __device__ void attn_few_wave(cons
         wait_loads<NI>();                      // (V's are on their way)
         __builtin_amdgcn_sched_barrier(0);
         w.products(kt, 0, x);
+        __builtin_amdgcn_sched_barrier(0);     // (the tile is read before it is filled again)
         if (next) ld.template load<false, NI>(a, kt, j0 + 32);
         __builtin_amdgcn_sched_barrier(0);
         w.close(a, j0, x);
@@ -1035,6 +1036,7 @@ template <int DT, int D, int MR> TOHIP_INLINE __device__ void attn_few_wave(cons
         typename Wave::Weights p;
         w.pack(x, p);
         w.add(vt, 0, p);
+        __builtin_amdgcn_sched_barrier(0);
         if (next) {
             ld.template load<true, NI>(a, vt, j0 + 32);
             ld.template find<32>(a, j0 + 64);
