@@ -559,11 +559,13 @@ template <int DT, int NT, bool HELD> struct SampleRow : RowChunks<DT> {
         for (int c = 0; c < PER; c++) Chunks::open(q[c], x + c * Chunks::VEC);
     }
     // f(tile, logits) for every tile in index order
-    template <class F> __device__ __forceinline__ void each(F f) const {
+    template <class F> __device__ __forceinline__ void each(F f) const { each(f, 0, tiles); }
+    // ... from tile `from` on (0 where they are held) and before `to`.
+    template <class F> __device__ __forceinline__ void each(F f, int from, int to) const {
         if constexpr (HELD) {
 #pragma unroll
             for (int tile = 0; tile < kHeld; tile++) {
-                if (tile >= tiles) break;
+                if (tile >= to) break;
                 float x[kEach];
 #pragma unroll
                 for (int c = 0; c < PER; c++) {
@@ -578,10 +580,10 @@ template <int DT, int NT, bool HELD> struct SampleRow : RowChunks<DT> {
             // Eight chunks of a thread at once: a CU has a microsecond's way to memory, and one or two
             // chunks of each thread on it are a tenth of what it could have.
             constexpr int BATCH = 8 / PER;
-            for (int tile0 = 0; tile0 < tiles; tile0 += BATCH) {
+            for (int tile0 = from; tile0 < to; tile0 += BATCH) {
                 uint4 q[BATCH][PER];
                 const int lo = tile0 * kTile - this->first;
-                if (lo >= 0 && lo + BATCH * kTile <= this->V) {
+                if (lo >= 0 && lo + BATCH * kTile <= this->V && tile0 + BATCH <= to) {
 #pragma unroll
                     for (int i = 0; i < BATCH; i++)
 #pragma unroll
@@ -589,11 +591,11 @@ template <int DT, int NT, bool HELD> struct SampleRow : RowChunks<DT> {
                 } else {
 #pragma unroll
                     for (int i = 0; i < BATCH; i++)
-                        if (tile0 + i < tiles) raw(tile0 + i, q[i]);
+                        if (tile0 + i < to) raw(tile0 + i, q[i]);
                 }
 #pragma unroll
                 for (int i = 0; i < BATCH; i++) {
-                    if (tile0 + i >= tiles) break;
+                    if (tile0 + i >= to) break;
                     float x[kEach];
 #pragma unroll
                     for (int c = 0; c < PER; c++) Chunks::open(q[i][c], x + c * Chunks::VEC);
@@ -1029,10 +1031,11 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
 // by the weights' logarithm; of every 16 the largest value.  A block per row goes on from those:
 // with top-k the few logits that can be kept, else the span that the draw falls into, and for a
 // border the logits whose logarithm is the border's.
-// (64 x 131072 bfloat16 by top-p: 16 us for the spans and 68 for the rows, a block per row 250;
+// (64 x 131072 bfloat16 by top-p: 16 us for the spans and 63 for the rows, a block per row 250;
 // 256 x 131072 float32 by temperature: 37 us, 3.6 TB/s with 34 M weights in double on the way, and 7.5,
 // a block per row 113.  A row with a border: 25 us to find the logits in its bins, four operations
-// for each of 131072 on one CU, 10 for the finer bins, 5 for the border.)
+// for each of 131072 on one CU, so of few rows several blocks do that, and the last one that is done
+// goes on; 10 for the finer bins, 5 for the border.)
 constexpr int kSpanThreads = 256, kSpan = 16 * kSpanThreads;
 constexpr int kPickThreads = 512;                      // (1024 have half the registers: spills cost every row 6 us)
 constexpr int kSpans = 512;                            // of a row at most
@@ -1042,8 +1045,20 @@ constexpr int kNear = 12288;                           // logits of the border's
 struct Spread {
     float *largest, *group;            // of each span, and of each 16 logits
     u64 *mass, *bins;                  // of each span
+    u64* near;                         // of each row, with several parts: the logits of its border's bins
+    unsigned *count, *done;            // how many those are, and parts that have added theirs
     int spans;                         // of a row
+    int parts;                         // blocks that look for a row's border's logits
 };
+// Parts of a row: no more blocks than CUs, and of many rows enough logits each to be worth the fences
+// between their blocks (by top-p, us with one part and with these: 1 x 250000 106 and 64; 16 x 131072
+// 77 and 62; 33 x 131072 79 and 65; 64 x 131072 85 and 78, 64 x 40000 41 and, with four, 47; 100 x
+// 131072 91 and 89, 100 x 40000 43 and, with two, 48; sixteen parts 60 and 64 for the first two).
+inline int parts_of(int64_t rows, int64_t V) {
+    if (rows <= 32) return 8;
+    if (rows <= 64) return (int)std::max<int64_t>(1, std::min<int64_t>(4, V / 24576));
+    return rows <= 128 && V >= 131072 ? 2 : 1;
+}
 
 // A logit's logarithm in bins, downwards, from that of 0 on: the same for all spans and launches.
 __device__ __forceinline__ double grid_of(float x, double per) { return -__builtin_floor(finite(x) * (per * 4.0)); }
@@ -1075,7 +1090,10 @@ template <int DT> __global__ __launch_bounds__(kSpanThreads) void k_sample_spans
     const int64_t at = row * w.spans + span;
     if (g.by_k) w.group[at * kSpanThreads + tid] = most;
     const float top = B::reduce(most, waves, Max());
-    if (tid == 0) w.largest[at] = top;
+    if (tid == 0) {
+        w.largest[at] = top;
+        if (span == 0) w.count[row] = w.done[row] = 0;
+    }
     if (!logs && !sums) return;
     u64 sum = 0;
     if (top > -INFINITY) {
@@ -1125,7 +1143,7 @@ struct PickShared {
         };
     };
     u64 kept[kSpans], found[2];
-    unsigned count, count2;
+    unsigned count, count2, base, turn;
 };
 constexpr int kOwn = 8;                                // logits of a thread in the drawn span
 static_assert(kSpan == kOwn * kPickThreads, "the drawn span");
@@ -1134,16 +1152,18 @@ template <int DT> __global__ __launch_bounds__(kPickThreads) void k_sample_pick(
     __shared__ PickShared s;
     typedef Block<kPickThreads> B;
     constexpr int NT = kPickThreads, VEC = RowChunks<DT>::VEC;
-    const int64_t row = blockIdx.x;
+    const int64_t row = blockIdx.x / (unsigned)w.parts;
+    const int part = (int)(blockIdx.x % (unsigned)w.parts);
     const int tid = (int)threadIdx.x, lane = tid & 63;
     const float* largest = w.largest + row * w.spans;
     const u64* mass = w.mass + row * w.spans;
     const Settings g(a, row);
+    if (part && (g.greedy || g.by_k || !g.filters())) return;      // (the first does these)
     float top = -INFINITY;
     for (int i = tid; i < w.spans; i += NT) top = fmaxf(top, largest[i]);
     top = B::reduce(top, s.waves, Max());
     if (top == -INFINITY) {
-        if (tid == 0) put_token(a, row, -1, -INFINITY);
+        if (tid == 0 && !part) put_token(a, row, -1, -INFINITY);
         return;
     }
     const RowChunks<DT> r(a, row);
@@ -1280,16 +1300,13 @@ template <int DT> __global__ __launch_bounds__(kPickThreads) void k_sample_pick(
             u64 sum = tid < kLogBins && tid < first ? s.row_bins[tid] : 0;
             above = B::reduce(sum, s.waves, Add());
         }
-        if (last >= kLogBins - 1) break;           // (among weights below 2^-31 of the largest)
-        // the spans' weights above those bins
-        for (int i = tid; i < w.spans; i += NT) s.kept[i] = 0;
-        __syncthreads();
-        each_bin([&](int span, int i, u64 p, int j, u64 q) {
-            const u64 sum = wave_allreduce((i < first ? p : 0) + (j < first ? q : 0), Add());
-            if (lane == 0) s.kept[span] = sum;
-        });
-        // and their logits in them, by the values that bound these bins; a wave finds the places of a
-        // tile's all at once
+        if (last >= kLogBins - 1) {                // (among weights below 2^-31 of the largest)
+            if (part) return;
+            break;
+        }
+        // the logits in those bins, by the values that bound these; a wave finds the places of a tile's
+        // all at once.  Each part's block looks through its tiles, and the last one that is done goes on
+        // with what all have found.
         const float lo = of_key(first_key([&](float x) { return grid_of(x, g.per) - from <= last; }));
         const float hi = of_key(first_key([&](float x) { return grid_of(x, g.per) - from < first; }));
         const bool open_end = !(hi == hi);                 // (none is above)
@@ -1298,9 +1315,36 @@ template <int DT> __global__ __launch_bounds__(kPickThreads) void k_sample_pick(
 #pragma unroll
             for (int e = 0; e < kEach; e++) in |= x[e] >= lo && (open_end || x[e] < hi) ? 1u << e : 0;
             add_candidates(s.near, &s.count, kNear, in, x, [&](int e) { return whole.index(tile) + e; });
+        }, part * ((whole.tiles + w.parts - 1) / w.parts), min((part + 1) * ((whole.tiles + w.parts - 1) / w.parts), whole.tiles));
+        __syncthreads();
+        if (w.parts > 1) {
+            u64* all = w.near + row * kNear;
+            if (tid == 0) s.base = atomicAdd(&w.count[row], s.count);
+            __syncthreads();
+            const unsigned base = s.base, n = min(s.count, base < kNear ? kNear - base : 0u);
+            for (unsigned i = tid; i < n; i += NT) all[base + i] = s.near[i];
+            __syncthreads();
+            if (tid == 0) {                        // (fences of one thread, for the block's loads and stores on either
+                // side of the barriers: of every wave they took 45 us more, as each writes a cache back)
+                __threadfence();
+                s.turn = atomicAdd(&w.done[row], 1u);
+                __threadfence();
+                s.count = atomicAdd(&w.count[row], 0u);
+            }
+            __syncthreads();
+            if (s.turn + 1 < (unsigned)w.parts) return;
+            for (unsigned i = tid; i < min(s.count, (unsigned)kNear); i += NT) s.near[i] = all[i];
+            __syncthreads();
+        }
+        if (s.count > kNear) break;
+        // the spans' weights above the bins
+        for (int i = tid; i < w.spans; i += NT) s.kept[i] = 0;
+        __syncthreads();
+        each_bin([&](int span, int i, u64 p, int j, u64 q) {
+            const u64 sum = wave_allreduce((i < first ? p : 0) + (j < first ? q : 0), Add());
+            if (lane == 0) s.kept[span] = sum;
         });
         __syncthreads();
-        if (s.count > kNear) break;
         const int near = (int)s.count;
         u64 border = 0;
         auto span_of = [&](u64 rank) { return (index_of(rank) + r.first) / kSpan; };
@@ -1377,6 +1421,10 @@ size_t spread_layout(Spread& w, void* base, int64_t rows, int64_t V) {
     take(w.group, rows * w.spans * kSpanThreads);
     take(w.mass, rows * w.spans);
     take(w.bins, rows * w.spans * kLogBins);
+    w.parts = parts_of(rows, V);
+    take(w.near, w.parts > 1 ? rows * kNear : 0);
+    take(w.count, rows);
+    take(w.done, rows);
     return (size_t)(p - (char*)base);
 }
 
@@ -1389,7 +1437,7 @@ template <int DT> void launch_sample(const SampleArgs& a, const Spread* w, hipSt
     const unsigned rows = (unsigned)a.rows;
     if (w) {
         hipLaunchKernelGGL(k_sample_spans<DT>, dim3(rows * (unsigned)w->spans), dim3(kSpanThreads), 0, s, a, *w);
-        hipLaunchKernelGGL(k_sample_pick<DT>, dim3(rows), dim3(kPickThreads), 0, s, a, *w);
+        hipLaunchKernelGGL(k_sample_pick<DT>, dim3(rows * (unsigned)w->parts), dim3(kPickThreads), 0, s, a, *w);
     } else if (a.V <= kShort) {
         hipLaunchKernelGGL((k_sample_row<DT, kShortThreads, true>), dim3(rows), dim3(kShortThreads), 0, s, a);
     } else if (a.V <= kLong) {

@@ -39,6 +39,17 @@ def test_large_vocabularies(hip, v, filters, dtype):
     SampleProblem(x, u, dtype, t=[1.0, 0.6, 1.5], **FILTERS[filters]).check(hip)
 
 
+@pytest.mark.parametrize("rows,v", [(1, 60000), (32, 40000), (33, 50021), (64, 98304), (65, 131072), (129, 131080)])
+def test_rows_in_parts(hip, rows, v):
+    """However many blocks look through a row; of every kind of row some, flat ones among them."""
+    x, u = logits(rows, v, seed=rows)
+    x[::5] *= 0.1
+    kind = np.arange(rows) % 6
+    of = lambda *values: np.asarray(values)[kind]        # noqa: E731
+    SampleProblem(x, u, "bfloat16", t=of(1.0, 1.0, 1.0, 1.0, 0.0, 1.0), k=of(0, 0, 0, 30, 0, 0),
+                  p=of(0.95, 0.5, 0.99, 1.0, 1.0, 1.0), m=of(0.0, 0.01, 0.0, 0.0, 0.0, 0.2)).check(hip)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_flat_rows(hip, dtype):
     """Nothing stands out: top-p keeps tens of thousands, top-k thousands."""
