@@ -761,7 +761,8 @@ template <int DT, int NT, class ROW> __device__ __forceinline__ void draw_any(co
 
 // A value that at least k logits are no less than, from the largest logits of some groups of them
 // (visit(f) calls f with the thread's): counted in bins between the least and the largest of these,
-// lo and top.  -inf: there are fewer groups.
+// lo and top.  -inf: there are fewer groups.  (Where these are equal or so near that scale is past
+// float32, the bins' edges say nothing and it is lo.)
 template <int NT, class V> __device__ __forceinline__ float kth_bound(V visit, u64 k, float lo, float top, Histograms<NT>& s) {
     const float scale = (float)(kBins - 1) / (top - lo);
     __syncthreads();
@@ -776,6 +777,7 @@ template <int NT, class V> __device__ __forceinline__ float kth_bound(V visit, u
     u64 before, total;
     const int bin = reach<NT, kBins / NT>([&](int i) { return s.bins[i]; }, k, s.waves, s.found, before, total);
     if (bin < 0) return -INFINITY;
+    if (!(scale < INFINITY)) return top < INFINITY ? lo : -INFINITY;
     const float edge = top - (float)(bin + 1) / scale;                 // (rounded: down by more than its own errors)
     const float least = edge - 1e-5f * (__builtin_fabsf(top) + __builtin_fabsf(lo));
     return least == least && top < INFINITY ? least : -INFINITY;

@@ -302,3 +302,17 @@ def test_repeatable(hip):
     for _ in range(5):
         b = p.run(hip)
         assert (a[0] == b[0]).all() and (a[1] == b[1]).all()
+
+
+@pytest.mark.parametrize("dtype", ("bfloat16", "float32"))
+@pytest.mark.parametrize("v", [1000, 9000, 40000, 131072])
+@pytest.mark.parametrize("high,low", [(1e-37, 0.0), (1e-39, 0.0), (0.0, -1e-37), (1e-37, -1e-37), (5e-36, 1e-36), (2e-35, 0.0), (1e-40, 1e-40)])
+def test_logits_that_differ_by_next_to_nothing(hip, high, low, v, dtype):
+    """Nearly equal logits around zero, down to subnormal ones: top-k keeps k of them, by value and index."""
+    x = np.full((6, v), low)
+    x[0, v // 2] = x[1, [3, v - 1]] = x[2, ::v // 9] = high
+    x[3, 5:15] = high
+    x[4, ::2] = high
+    u = np.array([0.02, 0.31, 0.52, 0.77, 0.93, 0.99], np.float32)
+    SampleProblem(x, u, dtype, k=[20, 20, 15, 7, 300, 1]).check(hip)
+    SampleProblem(x, u, dtype, k=[20, 1, 500, 11, 64, 600], p=[0.523, 0.9, 0.313, 0.771, 0.657, 0.41]).check(hip)
