@@ -1325,9 +1325,13 @@ template <int DT> __global__ __launch_bounds__(kPickThreads) void k_sample_pick(
             __syncthreads();
             const unsigned base = s.base, n = min(s.count, base < kNear ? kNear - base : 0u);
             for (unsigned i = tid; i < n; i += NT) all[base + i] = s.near[i];
+            // Each wave's stores are in this XCD's L2 before the barrier, which by itself waits for none
+            // that are on their way; then the fence of one thread writes that L2 back before `done`
+            // says so, and the last block's drops what its own caches hold from before.  (Fences of
+            // every wave took 45 us more, as each writes a cache back.)
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (tid == 0) {                        // (fences of one thread, for the block's loads and stores on either
-                // side of the barriers: of every wave they took 45 us more, as each writes a cache back)
+            if (tid == 0) {
                 __threadfence();
                 s.turn = atomicAdd(&w.done[row], 1u);
                 __threadfence();

@@ -316,3 +316,25 @@ def test_logits_that_differ_by_next_to_nothing(hip, high, low, v, dtype):
     u = np.array([0.02, 0.31, 0.52, 0.77, 0.93, 0.99], np.float32)
     SampleProblem(x, u, dtype, k=[20, 20, 15, 7, 300, 1]).check(hip)
     SampleProblem(x, u, dtype, k=[20, 1, 500, 11, 64, 600], p=[0.523, 0.9, 0.313, 0.771, 0.657, 0.41]).check(hip)
+
+
+@pytest.mark.parametrize("rows,v,k", [(1, 200003, 8), (20, 131072, 8), (64, 98304, 4), (100, 131072, 2)])
+def test_parts_of_a_row_hand_over_what_they_found(hip, rows, v, k):
+    """Blocks that look through one row each leave logits for the last of them in a workspace that holds an
+    earlier call's: two batches in turn, whose borders lie elsewhere, give the same results every time."""
+    import ctypes
+    from oracle import oracle as O
+    from onnx_translator_amd.nn.Operators import CSampleParams
+    with Dev(hip) as dev:
+        ws = dev.put(np.full(hip.lib.sample_workspace_bytes(rows, v), 255, np.uint8))
+        prm, calls = CSampleParams(0), []
+        for seed in range(2):
+            x, u = logits(rows, v, seed=seed, std=0.4 + 0.3 * seed, tall=2)
+            p = SampleProblem(x, u, "bfloat16", p=np.linspace(0.3 + 0.2 * seed, 0.9, rows), m=np.where(np.arange(rows) % k == 1, 0.05, 0.0))
+            want = p.check(hip)
+            out, lp = dev.put(np.full(rows, 77, np.int32)), dev.put(np.full(rows, 77, np.float32))
+            calls.append((want, out, lp, [dev.put(p.x), dev.put(p.u), O.PT(), O.PT(), dev.put(p.p), dev.put(p.m), out, lp, ctypes.byref(prm), ws]))
+        for i in range(40):
+            want, out, lp, args = calls[i % 2]
+            dev.call("sample_forward", *args)
+            assert (hip.dev_read(out, O.I32) == want[0]).all() and (hip.dev_read(lp, O.F32) == want[1]).all(), i
