@@ -1284,6 +1284,14 @@ template <int DT> __global__ __launch_bounds__(kPickThreads) void k_sample_pick(
             if (q) atomicAdd(&s.row_bins[min(j, kLogBins - 1)], q);
             weights += p + q;
         });
+        if (g.by_p) {                                      // and the spans that lie below the bins as a whole
+            for (int i = tid; i < w.spans; i += NT) {
+                if (grid_of(largest[i], g.per) - from < kLogBins) continue;
+                const u64 v = against_top(mass[i], factor_of(wt.log2_of(largest[i])));
+                if (v) atomicAdd(&s.row_bins[kLogBins - 1], v);
+                weights += v;
+            }
+        }
         weights = B::reduce(weights, s.waves, Add());
         const u64 want = g.by_p ? g.want(weights) : ~0ull;
         u64 above = 0, total;

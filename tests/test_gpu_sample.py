@@ -338,3 +338,73 @@ def test_parts_of_a_row_hand_over_what_they_found(hip, rows, v, k):
             want, out, lp, args = calls[i % 2]
             dev.call("sample_forward", *args)
             assert (hip.dev_read(out, O.I32) == want[0]).all() and (hip.dev_read(lp, O.F32) == want[1]).all(), i
+
+
+def _captured(hip, p, replays=2):
+    """Tokens of a call that is captured without a workspace (a block per row)."""
+    import ctypes
+    import torch
+    from oracle import oracle as O
+    from onnx_translator_amd.nn.Operators import CSampleParams
+    rows = len(p.x64)
+    code = {torch.float16: O.F16, torch.bfloat16: O.BF16, torch.float32: O.F32, torch.float64: O.F64, torch.int64: O.I64, torch.int32: O.I32}
+    t = [p.x.cuda() if isinstance(p.x, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(p.x)).cuda()]
+    t += [torch.from_numpy(v).cuda() if v is not None else None for v in (p.u, p.t, p.k, p.p, p.m)]
+    t += [torch.full((rows,), -9, dtype=torch.int32, device="cuda"), torch.zeros(rows, device="cuda")]
+    side = torch.cuda.Stream()
+    with Dev(hip) as dev:
+        w = [O.PT() if v is None else hip.lib.tensor_wrap_device(ctypes.c_void_p(v.data_ptr()), (ctypes.c_int * v.dim())(*v.shape), v.dim(), code[v.dtype])
+             for v in t]
+        dev.held += [x for x, v in zip(w, t) if v is not None]
+        prm = CSampleParams(p.vocab)
+        hip.lib.tensor_ops_hip_set_stream(ctypes.c_void_p(side.cuda_stream))
+        try:
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                dev.call("sample_forward", *w, ctypes.byref(prm), O.PT())
+            for _ in range(replays):
+                t[-2].fill_(-9)
+                torch.cuda.synchronize()
+                g.replay()
+                torch.cuda.synchronize()
+        finally:
+            torch.cuda.synchronize()
+            hip.lib.tensor_ops_hip_set_stream(None)
+        return t[-2].cpu().numpy().astype(np.int64), t[-1].cpu().numpy().astype(np.float64)
+
+
+@pytest.mark.parametrize("dtype", ("bfloat16", "float32"))
+@pytest.mark.parametrize("v", [40000, 131072, 2000003])
+def test_a_border_far_below_the_largest(hip, v, dtype):
+    """A peak and a tail 2^-32 of it and less that top-p keeps in part: the tail counts, whichever blocks
+    its logits lie in."""
+    rng = np.random.default_rng(v)
+    x = np.full((4, v), -22.2)
+    x[1] = rng.uniform(-23.5, -22.2, v)
+    x[2, :3000] = -20.5
+    x[3, ::2] = -24.0
+    x[:, 0], x[3, 0], x[3, 777] = 0.0, -22.2, 0.0
+    p = SampleProblem(x, np.zeros(4), dtype, p=np.ones(4), u_type="float64")
+    w = np.exp(p.x64 - p.x64.max(1, keepdims=True))
+    tail = w.sum(1) - 1
+    p.p = np.float32(1 - 0.4 * tail)
+    p.u = 1 - 0.3 * tail
+    tokens, lps = p.run(hip)
+    whole = _captured(hip, p)
+    assert (tokens == whole[0]).all() and (lps == whole[1]).all()
+    # Weights are rounded to 2^-s: a sum of theirs is off by n 2^-s / 2 at most, so what is kept by n 2^-s and a
+    # weight, on either side, and with it the sums over it and their share u.
+    step = v * 2.0 ** -min(51, 62 - math.ceil(math.log2(v)))
+    for r in range(4):
+        order = np.lexsort((np.arange(v), -p.x64[r]))
+        upto = np.cumsum(w[r, order])
+        kept = np.sort(order[:1 + int((upto[:-1] < float(p.p[r]) * upto[-1]).sum())])
+        before, total = np.concatenate([[0.0], np.cumsum(w[r, kept])]), w[r, kept].sum()
+        off = 6 * step + 4 * w[r, order[1]]
+        at = int(np.searchsorted(kept, tokens[r]))
+        low, high = before[at], before[min(at + 1, len(kept))]
+        assert low - off <= p.u[r] * total <= high + off, (r, tokens[r], low, high, p.u[r] * total, off)
+        want = p.x64[r, tokens[r]] - p.x64[r].max() - math.log(total)
+        assert abs(lps[r] - want) <= 2.0 ** -24 * abs(want) + 2.0 ** -26 + off
+        assert w[r, tokens[r]] < 0.5, "the peak's share is what the draw is past"
