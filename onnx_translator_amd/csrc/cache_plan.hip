@@ -328,9 +328,12 @@ extern "C" void cache_plan_forward(const Tensor* New, const Tensor* Past, const 
     const char* name = "cache_plan_forward";
     tensor_ops_hip_clear_error();
     if (!params) { set_error("%s: NULL params", name); return; }
+    const Tensor* needed[] = {New, Past, State, Pages, Free, QStart, KVLen, Positions, Slots, NextState};
+    for (const Tensor* t : needed)
+        if (!tensor_sane(t, name)) return;
     const Tensor* all[] = {New, Past, State, Pages, Free, QStart, KVLen, Positions, Slots, NextState, Offset};
     for (const Tensor* t : all) {
-        if (!t && t == Offset) continue;
+        if (!t) continue;              // (Offset)
         if (!tensor_sane(t, name)) return;
         if (t->size && !is_dev(classify(t->data))) { set_error("%s: every tensor must be device-resident", name); return; }
         if (!index_type(t)) { set_error("%s: every tensor must be int32 or int64", name); return; }

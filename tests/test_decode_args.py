@@ -76,6 +76,15 @@ def test_plan_refuses(rec, kw, message):
     assert message in err and not launches
 
 
+@pytest.mark.parametrize("absent", [i for i in range(11) if i != OFFSET])
+def test_plan_refuses_null_without_an_offset(rec, absent):
+    """An absent Offset makes no other tensor absent."""
+    shapes = [(5,), (5,), None, (3,), (5, 7), (40,), (6,), (5,), (12,), (12,), (3,)]
+    args = [rec.tensor(s, O.I64 if i in (STATE, NEXT) else O.I32) if s and i != absent else O.PT() for i, s in enumerate(shapes)]
+    launches, err = rec.call("cache_plan_forward", *args, ctypes.byref(Op.CCachePlanParams(16)))
+    assert "NULL tensor" in err and not launches
+
+
 @pytest.mark.parametrize("kw", [dict(), dict(offset=None), dict(ix=O.I64), dict(types={PAGES: O.I64, POS: O.I64}),
                                 dict(share=(PAST, LENGTH)), dict(share=(STATE, NEXT)), dict(new=(0,), past=(0,), pages=(0, 7), start=(1,), length=(0,)),
                                 dict(pos=(0,)), dict(pages=(5, 0)), dict(free=(1 << 28,), types={SLOTS: O.I64}), dict(page=1)],
