@@ -102,23 +102,24 @@ template <int NT, int N> __device__ __forceinline__ void block_scan(int64_t (&v)
 // loads go out together (512 requests, 7000 pages back: 11.1 us; sums, searches and loads one after
 // the other 18).
 template <int NT, class L, class S> __device__ __forceinline__ void spread(const int* sums, int from, int n, L load, S store) {
-    for (int k0 = from + (int)threadIdx.x; k0 < n; k0 += 4 * NT) {
+    // (unsigned: the last round of 2^31 - 2 pages goes past an int)
+    for (unsigned k0 = (unsigned)from + threadIdx.x; k0 < (unsigned)n; k0 += 4 * NT) {
         int at[4] = {};
 #pragma unroll
         for (int step = NT / 2; step > 0; step /= 2) {
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                if (sums[at[i] + step - 1] <= k0 + i * NT) at[i] += step;
+                if ((unsigned)sums[at[i] + step - 1] <= k0 + i * NT) at[i] += step;
         }
         int64_t x[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            if (sums[at[i]] <= k0 + i * NT) at[i]++;       // (at < NT where k < n)
-            x[i] = k0 + i * NT < n ? load(k0 + i * NT, at[i]) : 0;
+            if ((unsigned)sums[at[i]] <= k0 + i * NT) at[i]++;       // (at < NT where k < n)
+            x[i] = k0 + i * NT < (unsigned)n ? load((int)(k0 + i * NT), at[i]) : 0;
         }
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (k0 + i * NT < n) store(k0 + i * NT, at[i], x[i]);
+            if (k0 + i * NT < (unsigned)n) store((int)(k0 + i * NT), at[i], x[i]);
     }
 }
 

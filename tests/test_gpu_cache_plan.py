@@ -187,3 +187,28 @@ def test_a_service(hip):
         for p in w.values():
             lib.free_tensor(p)
         lib.tensor_ops_hip_set_stream(None)
+
+
+def test_nearly_all_that_an_int32_counts_comes_back(hip):
+    """One request gives 2^31 - 2 pages back: the places behind the last do not wrap around."""
+    from onnx_translator_amd.nn.Operators import CCachePlanParams
+    n, taken = (1 << 31) - 2, 5
+    pages = torch.arange(n, dtype=torch.int32, device="cuda")
+    free = torch.full((n + 1,), -3, dtype=torch.int32, device="cuda")
+    small = [torch.tensor(x, dtype=dt, device="cuda") for x, dt in
+             (([-1], torch.int32), ([n], torch.int32), ([taken, taken, 0], torch.int64), ([7, 7], torch.int32), ([7], torch.int32),
+              ([7, 7], torch.int32), ([7, 7], torch.int64), ([0, 0, 0], torch.int64))]
+    torch.cuda.synchronize()
+    new, past, state, start, length, pos, slots, after = small
+    with Dev(hip) as dev:
+        def wrap(x, shape=None):
+            shape = shape or tuple(x.shape)
+            dev.held.append(hip.lib.tensor_wrap_device(ctypes.c_void_p(x.data_ptr()), (ctypes.c_int * len(shape))(*shape), len(shape),
+                                                       O.I32 if x.dtype == torch.int32 else O.I64))
+            return dev.held[-1]
+        dev.call("cache_plan_forward", wrap(new), wrap(past), O.PT(), wrap(state), wrap(pages, (1, n)), wrap(free), wrap(start), wrap(length),
+                 wrap(pos), wrap(slots), wrap(after), ctypes.byref(CCachePlanParams(1)))
+        torch.cuda.synchronize()
+    assert after.tolist() == [taken, taken + n, 0] and length.tolist() == [0] and start.tolist() == [0, 0]
+    assert pos.tolist() == slots.tolist() == [-1, -1]
+    assert torch.equal(free[taken:], pages[:n + 1 - taken]) and torch.equal(free[:taken - 1], pages[n + 1 - taken:]) and int(free[taken - 1]) == -3
