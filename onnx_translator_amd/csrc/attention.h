@@ -33,7 +33,7 @@ struct AttnArgs {
     int mask_dt;                   // kU8 / kI8: 0 closes a key; else added to the score
     IndexVec len;                  // keys in use per batch (dense: p may be null) or sequence
     IndexVec pages, qstart;        // paged only
-    int64_t qstep;                 // entries of qstart from one sequence's to the next one's
+    const void* qend;              // of qstart's type, entry b: the row behind sequence b
     IndexVec prefix, plen;         // the rows' kernel of a shared prefix: its pages, its keys
     int prefix_pages;
     int B, Hq, Hkv, G, Sq, Skv, Dk, Dv;
@@ -72,7 +72,7 @@ __device__ __forceinline__ AttnSeq attn_seq_at(const AttnArgs& a, int b, int64_t
 }
 template <bool PAGED> __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, int b) {
     if constexpr (PAGED) {
-        return attn_seq_at(a, b, a.qstart[b * a.qstep], a.qstart[(b + 1) * a.qstep]);
+        return attn_seq_at(a, b, a.qstart[b], IndexVec{a.qend, a.qstart.is64}[b]);
     } else {
         AttnSeq s;
         s.b = b;

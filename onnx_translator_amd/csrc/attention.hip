@@ -95,7 +95,6 @@ bool cache_args(AttnArgs& a, const Tensor* Q, const Tensor* KCache, const Tensor
     a.fd_ps = make_fastdiv((uint32_t)a.ps);
     a.scale = scale != 0.0f ? scale : (float)(1.0 / std::sqrt((double)a.Dk));
     a.causal = 1;
-    a.qstep = 1;
     a.qh = a.Dk;
     a.qt = (int64_t)a.Hq * a.Dk;
     a.yh = a.Dv;
@@ -112,6 +111,7 @@ bool cache_args(AttnArgs& a, const Tensor* Q, const Tensor* KCache, const Tensor
     a.y = Y->data;
     a.pages = {Pages->data, (int)Pages->dtype == kI64};
     a.qstart = {QStart->data, (int)QStart->dtype == kI64};
+    a.qend = (const char*)QStart->data + dt_bytes((int)QStart->dtype);
     a.len = {KVLen->data, (int)KVLen->dtype == kI64};
     return true;
 }
@@ -229,7 +229,7 @@ void run_prefixed(AttnArgs& own, int dt, int64_t own_kv, int64_t prefix_kv, cons
     own.rows = (int64_t)own.T * own.Hq;
     own.nsplit = 1;
     AttnArgs pre = own;
-    pre.qstep = own.B;
+    pre.qend = (const char*)own.qstart.p + (size_t)own.B * (own.qstart.is64 ? 8 : 4);
     pre.B = 1;
     pre.pages = own.prefix;
     pre.len = own.plen;

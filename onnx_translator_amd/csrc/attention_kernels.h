@@ -303,7 +303,7 @@ template <int DT> constexpr float kLower = DT == kF16 ? 0x1p-6f : 1.0f;        /
 // (The slots of a sequence, one more than its whole tiles may need, follow from the starts
 // alone, so no list of tiles has to be made.)  64 sequences are tried at a time.
 template <int BM> __device__ __forceinline__ int64_t slot_base(const AttnArgs& a, int b) {
-    int64_t t0 = a.qstart[b * a.qstep];
+    int64_t t0 = a.qstart[b];
     t0 = t0 < 0 ? 0 : t0 > a.T ? a.T : t0;
     return t0 * a.G / BM + b;
 }
@@ -311,7 +311,7 @@ template <int BM> __device__ __forceinline__ AttnSeq slot_sequence(const AttnArg
     int lo = 0, n = a.B;                       // the answer is in [lo, lo + n)
     const int lane = (int)(threadIdx.x & 63);
     if (n < 64) {                              // all starts in one load
-        const int64_t v = a.qstart[min(lane, n) * a.qstep];
+        const int64_t v = IndexVec{lane < n ? a.qstart.p : a.qend, a.qstart.is64}[lane < n ? lane : n - 1];
         const int start = (int)(v < 0 ? 0 : v > a.T ? a.T : v);
         const bool le = lane < n && (int64_t)start * a.G / BM + lane <= t;
         const int b = max(0, (int)__popcll(__ballot(le)) - 1);
@@ -841,6 +841,24 @@ template <int DT, int D, bool PAGED, int MR, int W> struct AttnLoads {
     }
 };
 
+// The four tiles that a kernel keeps in LDS, N bytes each.  As variables of their own: as parts of one
+// array, or as a function's arguments, the compiler waits for loads into one tile before it reads
+// another and checks each address that a load writes to (cache attention, single tokens over up to
+// 300 keys: 55 us, else 59).
+template <int N> struct Tiles {
+    template <int I> TOHIP_INLINE __device__ char* at() const {
+        __shared__ __attribute__((aligned(1024))) char t[N];
+        return t;
+    }
+};
+// One behind the other in an array, for the kernels behind a prefix, whose code for two parts is as fast
+// with one as with the other (4 tokens behind 2000 keys 15.0 us, as variables 15.6; 3 in float16 behind
+// 4915 15.3 and 14.7) and whose waves divide it otherwise.
+template <int N> struct TilesAt {
+    char* lds;
+    template <int I> TOHIP_INLINE __device__ char* at() const { return lds + I * N; }
+};
+
 // Prompts: W waves of 32 rows share tiles of BN keys, two deep: while tile n is worked on, tile
 // n + 1 is on its way.  S' = K Q' leaves a query's scores in one lane pair, in the order in
 // which O' += V' P' takes its weights, so they never leave the registers; 32 rows per wave are
@@ -851,12 +869,13 @@ template <int DT, int D, bool PAGED, int MR, int W> struct AttnLoads {
 // by card or 1.0 PFLOP/s; the last 4096 of 16384 keys in pages of 16, 980 .. 1020 us (630 and
 // 1080 in the first hundred calls of an idle card, whose clock rises meanwhile).  With 64 values per head the
 // exponentials weigh twice as much.
-// (lds: four tiles of BN rows.)
-template <int DT, int D, bool PAGED, bool MASK, int W, int BN> TOHIP_INLINE __device__ void attn_tiles(const AttnArgs& a, uint32_t bid, char* lds, int& missing) {
+template <int DT, int D, bool PAGED, bool MASK, int W, int BN, class TILES>
+TOHIP_INLINE __device__ void attn_tiles(const AttnArgs& a, uint32_t bid, TILES tiles) {
     typedef AttnWave<DT, D, PAGED, MASK, 32, (D <= 128)> Wave;      // (as far as registers go)
     constexpr int RB = Wave::RB, NI = BN * RB / (1024 * W);
     static_assert(NI >= 1, "tile");
-    char *k0_ = lds, *k1_ = lds + BN * RB, *v0_ = lds + 2 * BN * RB, *v1_ = lds + 3 * BN * RB;
+    char *k0_ = tiles.template at<0>(), *k1_ = tiles.template at<1>(), *v0_ = tiles.template at<2>(), *v1_ = tiles.template at<3>();
+    __shared__ int missing;                    // a key's page was none of the cache's
     const int t = (int)threadIdx.x, wave = uniform(t >> 6);
     AttnBlock k;
     if (!attn_block<PAGED, 32 * W>(a, bid, t, 64 * W, k)) return;
@@ -907,9 +926,7 @@ template <int DT, int D, bool PAGED, bool MASK, int W, int BN> TOHIP_INLINE __de
 }
 template <int DT, int D, bool PAGED, bool MASK, int W, int BN>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D * kElem<DT> <= 128 && W == 4 && !MASK ? 3 : D * kElem<DT> <= 256 ? 2 : 1))) void k_attn_tiles(AttnArgs a) {
-    __shared__ __attribute__((aligned(1024))) char lds[4 * BN * D * kElem<DT>];
-    __shared__ int missing;                    // a key's page was none of the cache's
-    attn_tiles<DT, D, PAGED, MASK, W, BN>(a, blockIdx.x, lds, missing);
+    attn_tiles<DT, D, PAGED, MASK, W, BN>(a, blockIdx.x, Tiles<BN * D * kElem<DT>>());
 }
 
 // Few rows: a block is one wave, so nothing waits for another.  K and V have two buffers of
@@ -921,11 +938,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D * kEle
 // than 64 values take 64 or 128 KB of LDS per wave and, for 256 values and 32 rows, more than 512
 // registers, so two waves or one run on a CU: 16 tokens of 16 heads over 130 .. 4096 keys of 4
 // heads reach 2.0 TB/s with 64 values, 2.2 with 128, 1.5 with 256.
-// (lds: four tiles of 32 rows.)
-template <int DT, int D, bool PAGED, bool MASK, int MR> TOHIP_INLINE __device__ void attn_few(const AttnArgs& a, uint32_t bid, char* lds) {
+template <int DT, int D, bool PAGED, bool MASK, int MR, class TILES> TOHIP_INLINE __device__ void attn_few(const AttnArgs& a, uint32_t bid, TILES tiles) {
     typedef AttnWave<DT, D, PAGED, MASK, MR, (MR == 16 || D <= 128)> Wave;      // (as far as registers go)
     constexpr int RB = Wave::RB, NI = 32 * RB / 1024;
-    char *k0_ = lds, *k1_ = lds + 32 * RB, *v0_ = lds + 64 * RB, *v1_ = lds + 96 * RB;
+    char *k0_ = tiles.template at<0>(), *k1_ = tiles.template at<1>(), *v0_ = tiles.template at<2>(), *v1_ = tiles.template at<3>();
     AttnBlock k;
     if (!attn_block<PAGED, MR>(a, bid, (int)threadIdx.x, 64, k)) return;
     Wave w;
@@ -985,8 +1001,7 @@ template <int DT, int D, bool PAGED, bool MASK, int MR> TOHIP_INLINE __device__ 
 }
 template <int DT, int D, bool PAGED, bool MASK, int MR>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D * kElem<DT> <= 256 ? 2 : 1))) void k_attn_few(AttnArgs a) {
-    __shared__ __attribute__((aligned(1024))) char lds[128 * D * kElem<DT>];
-    attn_few<DT, D, PAGED, MASK, MR>(a, blockIdx.x, lds);
+    attn_few<DT, D, PAGED, MASK, MR>(a, blockIdx.x, Tiles<32 * D * kElem<DT>>());
 }
 
 // ---- behind a shared prefix --------------------------------------------------------------
@@ -997,15 +1012,14 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(D * kElem<DT
 template <int DT, int D, int MR>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void k_prefix_few(AttnArgs pre, AttnArgs own, unsigned first) {
     __shared__ __attribute__((aligned(1024))) char lds[128 * D * kElem<DT>];
-    if (blockIdx.x < first) attn_few<DT, D, true, false, MR>(pre, blockIdx.x, lds);
-    else attn_few<DT, D, true, false, MR>(own, blockIdx.x - first, lds);
+    if (blockIdx.x < first) attn_few<DT, D, true, false, MR>(pre, blockIdx.x, TilesAt<32 * D * kElem<DT>>{lds});
+    else attn_few<DT, D, true, false, MR>(own, blockIdx.x - first, TilesAt<32 * D * kElem<DT>>{lds});
 }
 template <int DT, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D * kElem<DT> <= 128 ? 3 : 2))) void k_prefix_tiles(AttnArgs pre, AttnArgs own, unsigned first) {
     __shared__ __attribute__((aligned(1024))) char lds[256 * D * kElem<DT>];
-    __shared__ int missing;
-    if (blockIdx.x < first) attn_tiles<DT, D, true, false, 4, 64>(pre, blockIdx.x, lds, missing);
-    else attn_tiles<DT, D, true, false, 4, 64>(own, blockIdx.x - first, lds, missing);
+    if (blockIdx.x < first) attn_tiles<DT, D, true, false, 4, 64>(pre, blockIdx.x, TilesAt<64 * D * kElem<DT>>{lds});
+    else attn_tiles<DT, D, true, false, 4, 64>(own, blockIdx.x - first, TilesAt<64 * D * kElem<DT>>{lds});
 }
 // Few rows as one of a block's four waves that know nothing of each other, in a quarter of the LDS of
 // its tiles: one buffer for K and one for V, filled again as soon as they are read.  (Eight such waves
@@ -1058,9 +1072,8 @@ template <int DT, int D, int MR> TOHIP_INLINE __device__ void attn_few_wave(cons
 template <int DT, int D, int MR>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k_prefix_both(AttnArgs pre, AttnArgs own, unsigned first, unsigned own_blocks) {
     __shared__ __attribute__((aligned(1024))) char lds[256 * D * kElem<DT>];
-    __shared__ int missing;
     if (blockIdx.x < first) {
-        attn_tiles<DT, D, true, false, 4, 64>(pre, blockIdx.x, lds, missing);
+        attn_tiles<DT, D, true, false, 4, 64>(pre, blockIdx.x, TilesAt<64 * D * kElem<DT>>{lds});
     } else {
         const int wave = uniform((int)threadIdx.x >> 6);
         const unsigned bid = (blockIdx.x - first) * 4 + (unsigned)wave;
