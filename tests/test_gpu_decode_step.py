@@ -306,3 +306,107 @@ def test_python_layer(hip):
         for r, x in enumerate(logits.numpy().astype(np.float64)):
             assert token.numpy()[r] in sample(x, float(u[r]), 1.0, 20, float(np.float32(0.9)))[0]
     assert state.numpy().tolist() == [3, 8, 0] and Ops._get_lib() is not None
+
+
+def test_a_replay_draws_what_its_logits_say(hip):
+    """The captured step's draw against an eager one on the very logits that the replay left, with a workspace
+    of its own: the same tokens and probabilities, in every step."""
+    lib = _lib(hip)
+    side = torch.cuda.Stream()
+    lib.tensor_ops_hip_set_stream(ctypes.c_void_p(side.cuda_stream))
+    s = Service(lib, seed=7)
+    own = {k: torch.empty_like(s.t[k]) for k in ("token", "chance", "ws2")}
+    w = {k: s._wrap(x) for k, x in own.items()}
+    drawn = 0
+    try:
+        with torch.cuda.stream(side):
+            s.step()
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                s.step()
+            for i in range(10):
+                s.arrivals()
+                g.replay()
+                own["token"].fill_(-7)
+                own["ws2"].fill_(255)
+                torch.cuda.synchronize()
+                lib.sample_forward(*(s.w[k] for k in ("logits", "u", "temperature", "k_of", "p_of", "m_of")), w["token"], w["chance"],
+                                   ctypes.byref(s.p[3]), w["ws2"])
+                assert not lib.tensor_ops_hip_last_error()
+                torch.cuda.synchronize()
+                assert torch.equal(own["token"], s.t["token"]) and torch.equal(own["chance"], s.t["chance"]), i
+                drawn += int(s.t["start"][-1])
+        assert drawn > 20
+    finally:
+        torch.cuda.synchronize()
+        s.free()
+        for p in w.values():
+            lib.free_tensor(p)
+        lib.tensor_ops_hip_set_stream(None)
+
+
+def test_two_graphs_at_once_leave_each_other_alone(hip):
+    """All results of two captured steps that run at once, attention among them, are those of the same
+    steps replayed one after the other."""
+    lib = _lib(hip)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    services, graphs = [Service(lib, seed=20 + i) for i in range(2)], []
+    kept = ("past", "state", "pages", "free", "k", "v")
+    names = ("start", "past", "state", "pages", "free", "pos", "places", "q", "k", "v", "y", "logits", "token", "chance")
+    try:
+        for st, s in zip(streams, services):
+            lib.tensor_ops_hip_set_stream(ctypes.c_void_p(st.cuda_stream))
+            with torch.cuda.stream(st):
+                s.step()
+                torch.cuda.synchronize()
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=st):
+                    s.step()
+                graphs.append(g)
+        for i in range(6):
+            old, want = [], []
+            for st, s, g in zip(streams, services, graphs):
+                s.arrivals()
+                old.append({k: s.t[k].clone() for k in kept})
+                s.t["y"].fill_(3.0)
+                torch.cuda.synchronize()
+                with torch.cuda.stream(st):
+                    g.replay()
+                torch.cuda.synchronize()
+                want.append({k: s.t[k].clone() for k in names})
+                for k, x in old[-1].items():
+                    s.t[k].copy_(x)
+                for k in ("q", "logits", "token", "chance", "y"):
+                    s.t[k].fill_(3)
+            torch.cuda.synchronize()
+            for st, g in zip(streams, graphs):
+                with torch.cuda.stream(st):
+                    g.replay()
+            torch.cuda.synchronize()
+            for s, x in zip(services, want):
+                for k in names:
+                    n = int(x["start"][-1]) if k in ("q", "y", "logits", "token", "chance") else None
+                    assert torch.equal(s.t[k][:n], x[k][:n]), (i, k)
+    finally:
+        torch.cuda.synchronize()
+        for s in services:
+            s.free()
+        lib.tensor_ops_hip_set_stream(None)
+
+
+def test_python_layer_without_tokens(hip):
+    """A step in which nobody brings a token, and a draw of no rows."""
+    def dev(a):
+        a = np.ascontiguousarray(a)
+        return Tensor(*a.shape, dtype=str(a.dtype), data=a).to_device()
+
+    state, pages, free = dev(np.array([3, 9, 0])), dev(np.array([[12, 13, -1], [14, -1, -1]], np.int32)), dev(np.arange(2, 11, dtype=np.int32))
+    for new, past, want, left in (([0, 0], [20, 5], [20, 5], [3, 9, 0]), ([-1, 0], [20, 5], [0, 5], [3, 11, 0]), ([-1, -1], [0, 5], [0, 0], [3, 12, 0])):
+        start, length, pos, places = Op.CachePlan([], [], 16).forward(dev(np.array(new, np.int32)), dev(np.array(past, np.int32)), state, pages,
+                                                                      free, 0)["tensor"]
+        assert start.numpy().tolist() == [0, 0, 0] and length.numpy().tolist() == want
+        assert pos.numpy().size == places.numpy().size == 0 and state.numpy().tolist() == left
+    assert free.numpy().tolist() == [12, 13, 14] + [5, 6, 7, 8, 9, 10]
+    token, chance = Op.Sample([], []).forward(dev(np.zeros((0, 100), np.float32)), dev(np.zeros(0, np.float32)))["tensor"]
+    assert token.numpy().size == chance.numpy().size == 0
