@@ -488,7 +488,9 @@ typedef struct {
  * (float32 [rows], may be NULL) receives the logarithm of the probability with which the token
  * was drawn (0 for a greedy row, -inf for Token -1).  Sums of weights are kept in 64-bit fixed
  * point, at least 2^-44 of the largest weight for up to 2^18 columns, in which their order does
- * not matter: the same call gives the same token.
+ * not matter: the same call gives the same token.  (A draw or a border of top-p nearer to a token's
+ * edge than that for each column may fall on its other side where a long row is not spread, below,
+ * or begins elsewhere in its 16 bytes.)
  *   Workspace (may be NULL): device memory of any type, 16-byte aligned, with which a call
  * spreads long rows over the GPU: sample_workspace_bytes(rows, tokens) bytes, 0 where a call of
  * that size needs none.  Without one an eager call takes them from the library's pool; a call

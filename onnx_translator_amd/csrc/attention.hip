@@ -242,8 +242,9 @@ void run_prefixed(AttnArgs& own, int dt, int64_t own_kv, int64_t prefix_kv, cons
         const int cus = num_cus();
         auto tiles_of = [&](int n) { return (rows + n - 1) / n * own.Hkv; };
         // Time on the whole GPU of the prefix's products (64 keys of a block of 128 rows: 1.7 us with
-        // two blocks on a CU, at 128 values per head) and of the own keys' bytes, in us: lengths
-        // differ, so about half of the longest.
+        // two blocks on a CU, at 128 values of 16 bits per head; float32 products take about seven times
+        // as long, which is left out: longer blocks than their prefix would need) and of the own
+        // keys' bytes, in us: lengths differ, so about half of the longest.
         const double step = 1.7 * p0.d / 128, pre_us = (double)tiles_of(128) * (double)prefix_kv / 64 * step / (2 * cus);
         const double own_us = 0.5 * own.B * own.Hkv * (double)own_kv * (own.Dk + own.Dv) * es / 4.5e6;
         // (three tiles at least: 4 tokens behind 2000 keys 14.9 us, 15.4 with two, 15.9 with four; 16
@@ -256,7 +257,7 @@ void run_prefixed(AttnArgs& own, int dt, int64_t own_kv, int64_t prefix_kv, cons
             if (es == 2 && p0.d * es <= 256 && kKeys256 <= kTablePages * (int64_t)own.ps && pre_us > std::max(2 * own_us, 100.0)) {
                 // Products are all there is: blocks of 256 rows, one to a CU, all of one length, in as
                 // many splits as fill the last round of them best, and a launch for the own keys (2048
-                // tokens of 32 heads behind 16384 keys: 591 us, 647 by 128 rows and one launch; 704
+                // tokens of 32 heads behind 16384 keys: 591 us, 647 by 128 rows and one launch; 608
                 // tokens of 24 behind 2501: 57 and 44).
                 double best = 0.7;
                 for (int n = 1; n <= 8; n++) {

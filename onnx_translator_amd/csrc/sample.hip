@@ -11,7 +11,11 @@
 // Weights are computed in double and summed as 64-bit fixed-point numbers: whole numbers, so
 // every order of adding gives the same sum, histograms may be filled by atomics and the borders
 // p and u fall where the sums in index order have them, whoever adds.  (In float32 sums a token
-// beside a border would depend on the order: of 131072 tokens one row in some thousands.)
+// beside a border would depend on the order: of 131072 tokens one row in some thousands.)  Rows that
+// are spread over blocks are summed span by span against the span's largest weight and rounded once
+// more when those sums are taken against the row's, by half of 2^-shift for each span or bin of a span: less
+// than the weights' own roundings add up to, but a border as near as that may fall on the other
+// side of a token than in a row that one block does, or with the spans that begin at another column.
 #include "attention.h"
 
 #include <algorithm>
@@ -58,7 +62,7 @@ struct Weights {
     // log2 of the weight, -100 for what weighs nothing in 64 bits (-inf among it)
     __device__ __forceinline__ double log2_of(float x) const { return __builtin_fmax((finite(x) - top) * per, -100.0); }
     // 2^y for -100 <= y <= 0, as the bits of 2^52 + the weight rounded to the nearest whole number:
-    // the polynomial through 2^f at the eleven Chebyshev points of |f| <= 1/2 (off by 2^-51.6 of
+    // the polynomial through 2^f at the eleven Chebyshev points of |f| <= 1/2 (off by 2^-51.5 of
     // itself), with whole part and shift put into its exponent.  Without a branch, and the factors
     // as scalars: else each costs two moves, more than the product.
     __device__ __forceinline__ u64 bits(double y) const {
@@ -880,7 +884,9 @@ __device__ __forceinline__ int log_bin(double y) { return min((int)(y * -51.0), 
 
 // A block per row.  HELD: the row is read once, into registers.  Bound by one CU's double products and
 // LDS atomics where top-p weighs the whole row (32000 logits: 42 us, of them 9 for the histogram,
-// 6 .. 10 for the second pass), else by its chain of barriers (top-k of 50: 12 us, greedy 6).
+// 6 .. 10 for the second pass), else by its chain of barriers (top-k of 50: 16 us, greedy 6).  Where
+// the row is read again for each pass (HELD false) the compiler spills 60 .. 160 bytes a thread of 1024
+// (131072 bfloat16 by top-p: 100 us one row, 117 64 rows; by temperature 42).
 template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sample_row(SampleArgs a) {
     __shared__ SampleShared<NT> s;
     typedef Block<NT> B;
@@ -1033,9 +1039,9 @@ template <int DT, int NT, bool HELD> __global__ __launch_bounds__(NT) void k_sam
 // by the weights' logarithm; of every 16 the largest value.  A block per row goes on from those:
 // with top-k the few logits that can be kept, else the span that the draw falls into, and for a
 // border the logits whose logarithm is the border's.
-// (64 x 131072 bfloat16 by top-p: 16 us for the spans and 63 for the rows, a block per row 250;
-// 256 x 131072 float32 by temperature: 37 us, 3.6 TB/s with 34 M weights in double on the way, and 7.5,
-// a block per row 113.  A row with a border: 25 us to find the logits in its bins, four operations
+// (64 x 131072 bfloat16 by top-p: 18 us for the spans and 60 for the rows, a block per row 117;
+// 256 x 131072 float32 by temperature: 39 us, 3.4 TB/s with 34 M weights in double on the way, which keep
+// the vector units busy for 78 % of it, and 8, a block per row 62.  A row with a border: 25 us to find the logits in its bins, four operations
 // for each of 131072 on one CU, so of few rows several blocks do that, and the last one that is done
 // goes on; 10 for the finer bins, 5 for the border.)
 constexpr int kSpanThreads = 256, kSpan = 16 * kSpanThreads;
@@ -1445,8 +1451,8 @@ size_t spread_layout(Spread& w, void* base, int64_t rows, int64_t V) {
 constexpr int kShort = kHeld * kShortThreads * kEach - 8, kLong = kHeld * kRowThreads * kEach - 8;
 
 // Rows of up to kLong logits stay in a block's registers: one launch where two take 4 us more (32000
-// logits by top-k: 13.5 us, spread 19; but by temperature alone 16 and 10, by top-p 42 and 34, which
-// the host cannot know).  Short ones take a small block, whose barriers are cheaper.
+// logits by top-k: 13.5 .. 16 us, spread 19; but by temperature alone 17 and 10, by top-p 42 and 34,
+// which the host cannot know).  Short ones take a small block, whose barriers are cheaper.
 template <int DT> void launch_sample(const SampleArgs& a, const Spread* w, hipStream_t s) {
     const unsigned rows = (unsigned)a.rows;
     if (w) {
