@@ -408,3 +408,15 @@ def test_a_border_far_below_the_largest(hip, v, dtype):
         want = p.x64[r, tokens[r]] - p.x64[r].max() - math.log(total)
         assert abs(lps[r] - want) <= 2.0 ** -24 * abs(want) + 2.0 ** -26 + off
         assert w[r, tokens[r]] < 0.5, "the peak's share is what the draw is past"
+
+
+@pytest.mark.parametrize("v", [2000, 40001])
+@pytest.mark.parametrize("t", [1e-30, 1e-9, 1e-3, math.inf])
+def test_infinite_logits_at_any_temperature(hip, t, v):
+    """+inf keeps its share where the others' distance from it, over the temperature, is past float64."""
+    x, u = logits(4, v, seed=17)
+    x[:, [17, 1500]] = np.inf
+    u[:] = [0.0, 0.49, 0.51, 0.99]
+    for f in ({}, dict(p=0.99), dict(m=0.3), dict(p=0.9, m=0.3), dict(k=3), dict(k=3, p=0.99)):
+        tokens, _ = SampleProblem(x, u, "float32", t=t, **f).run(hip)
+        assert tokens.tolist() == [17, 17, 1500, 1500], (f, tokens)
